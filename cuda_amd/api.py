@@ -18,10 +18,12 @@ flash_decode, paged decode). ``flash_attention`` is differentiable (README.md:
 reference instantiates it).
 """
 import ctypes
+import functools
 import math
 import os
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -31,6 +33,9 @@ __all__ = [
     "fused_gqa_forward", "fused_rope_flash_attention", "flash_decode", "async_flash_decode", "paged_attention",
     "paged_attention_forward", "fp8_paged_attention", "fp8_paged_attention_forward",
     "fused_microscaled_attention", "mx_scales_to_e8m0", "paged_kv_append",
+    "cross_attention", "cross_attention_forward", "cross_attention_forward_lse", "cross_attention_backward",
+    "relative_bias_attention", "relative_bias_attention_forward", "relative_bias_attention_forward_lse",
+    "relative_bias_attention_backward", "relative_bias_decode",
 ]
 
 _DT = {torch.bfloat16: _lib.CA_BF16, torch.float16: _lib.CA_F16, torch.float32: _lib.CA_F32}
@@ -283,6 +288,247 @@ def async_flash_decode(q, k, v, softmax_scale=None):
 
 
 flash_decode = async_flash_decode
+
+
+# ---------------------------------------------------------------------------
+# Cross attention and relative position bias (encoder-decoder models)
+# ---------------------------------------------------------------------------
+def _encdec_checks(q, k, v, kv_lens):
+    _check(q.is_cuda and k.is_cuda and v.is_cuda, "Inputs must be on CUDA")
+    _check(q.is_contiguous() and k.is_contiguous() and v.is_contiguous(), "Inputs must be contiguous")
+    _check(q.dim() == 4 and k.dim() == 4 and v.dim() == 4,
+           "Expected 4D tensors: [batch, num_heads, length, head_dim]")
+    _check(k.shape == v.shape, "K and V must have identical shapes")
+    b, hq, sq, d = q.shape
+    hkv, skv = k.shape[1], k.shape[2]
+    _check(k.shape[0] == b and k.shape[3] == d and hkv >= 1 and hq >= 1 and hq % hkv == 0,
+           "K, V must be [batch, num_kv_heads, kv_len, head_dim] with num_kv_heads dividing Q's heads")
+    _check(q.dtype == k.dtype == v.dtype, "Q, K, V must have the same dtype")
+    _check(d in (64, 128), "Only head_dim 64 and 128 are currently supported")
+    _check(k.device == q.device and v.device == q.device, "Inputs must be on one device")
+    if kv_lens is not None:
+        _check(kv_lens.is_cuda and kv_lens.device == q.device, "kv_lens must be on the inputs' device")
+        _check(kv_lens.dim() == 1 and kv_lens.numel() == b, "kv_lens must be [batch]")
+        _check(not kv_lens.is_floating_point() and not kv_lens.is_complex() and kv_lens.dtype != torch.bool,
+               "kv_lens must hold integers")
+        kv_lens = kv_lens.to(torch.int32).contiguous()
+    return b, hq, hkv, sq, skv, d, kv_lens
+
+
+@functools.lru_cache(maxsize=64)
+def _bucket_starts(num_buckets, is_causal, max_distance):
+    """First distance of each bucket of a side, as the C ABI takes them: the
+    first half of the side's buckets hold one distance each, the others
+    distances that grow as a power up to max_distance: bucket e + j starts at
+    the first n with (n / e) ** span >= (max_distance / e) ** j, e buckets
+    below it and span from it on, found in whole numbers."""
+    side = num_buckets if is_causal else num_buckets // 2
+    _check(1 <= num_buckets <= 256 and (is_causal or num_buckets % 2 == 0) and side >= 2,
+           "bias_table must have 2 to 256 buckets (4 or more, an even number, if not causal)")
+    e = side // 2
+    span = side - e
+    _check(e < max_distance <= 2048, f"max_distance must be in ({e}, 2048]")
+    starts = list(range(e))
+    for j in range(span):
+        power = max_distance ** j * e ** span
+        lo, hi = e, max_distance       # (hi reaches every border: j < span)
+        while lo < hi:
+            mid = (lo + hi) // 2
+            if mid ** span * e ** j >= power:
+                hi = mid
+            else:
+                lo = mid + 1
+        starts.append(lo)
+    return (ctypes.c_int32 * side)(*starts)
+
+
+def _bias_checks(q, bias_table, is_causal, max_distance):
+    _check(bias_table.is_cuda and bias_table.device == q.device, "bias_table must be on the inputs' device")
+    _check(bias_table.dim() == 2 and bias_table.shape[1] == q.shape[1], "bias_table must be [num_buckets, num_heads]")
+    _check(bias_table.dtype in _DT, "Unsupported scalar type for bias_table. Supported: Float, Float16, BFloat16.")
+    _check(isinstance(max_distance, int), "max_distance must be an integer")
+    starts = _bucket_starts(bias_table.shape[0], bool(is_causal), max_distance)
+    return bias_table.detach().to(torch.float32).contiguous(), starts
+
+
+def _encdec_forward(q, k, v, kv_lens, softmax_scale, want_lse, bias=None, is_causal=False):
+    """(out, lse or None); bias: (table, max_distance) or None."""
+    b, hq, hkv, sq, skv, d, lens = _encdec_checks(q, k, v, kv_lens)
+    what = "Cross Attention" if bias is None else "Relative Bias Attention"
+    dt = _dtype_code(q, what)
+    with torch.cuda.device(q.device):
+        if bias is not None:
+            table, starts = _bias_checks(q, bias[0], is_causal, bias[1])
+        q, k, v = _aligned(q), _aligned(k), _aligned(v)
+        out = torch.empty_like(q)
+        lse = torch.empty(b, hq, sq, dtype=torch.float32, device=q.device) if want_lse else None
+        lib = _lib.load()
+        if bias is None:
+            nbytes = lib.ca_cross_attention_workspace_bytes(dt, b, hq, hkv, sq, skv, d, int(want_lse))
+            ws, nbytes = _workspace(nbytes, q.device)
+            _lib.call("ca_cross_attention", dt, _ptr(q), _ptr(k), _ptr(v), _ptr(lens), _ptr(out), _ptr(lse),
+                      b, hq, hkv, sq, skv, d, _scale(softmax_scale, d), _ptr(ws), nbytes, _stream())
+        else:
+            nbytes = lib.ca_relative_bias_attention_workspace_bytes(dt, b, hq, hkv, sq, skv, d, int(bool(is_causal)))
+            ws, nbytes = _workspace(nbytes, q.device)
+            _lib.call("ca_relative_bias_attention", dt, _ptr(q), _ptr(k), _ptr(v), _ptr(table), starts,
+                      table.shape[0], _ptr(lens), _ptr(out), _ptr(lse), b, hq, hkv, sq, skv, d,
+                      _scale(softmax_scale, d), int(bool(is_causal)), _ptr(ws), nbytes, _stream())
+    return out, lse
+
+
+def _encdec_backward(dout, q, k, v, out, lse, kv_lens, softmax_scale, bias=None, is_causal=False):
+    """[dq, dk, dv] (with a bias, and dtable)."""
+    b, hq, hkv, sq, skv, d, lens = _encdec_checks(q, k, v, kv_lens)
+    for t in (dout, out, lse):
+        _check(t.is_cuda and t.device == q.device, "Inputs must be on one device")
+    _check(dout.shape == q.shape and out.shape == q.shape, "dout and out must have Q's shape")
+    _check(tuple(lse.shape) == (b, hq, sq), "lse must be [batch, num_heads, q_len]")
+    _check(out.dtype == q.dtype and dout.dtype == q.dtype, "q, k, v, out and dout must have the same dtype")
+    what = "Cross Attention Backward" if bias is None else "Relative Bias Attention Backward"
+    dt = _dtype_code(q, what)
+    with torch.cuda.device(q.device):
+        if bias is not None:
+            table, starts = _bias_checks(q, bias[0], is_causal, bias[1])
+        q, k, v, out, dout = (_aligned(t.contiguous()) for t in (q, k, v, out, dout))
+        lse = lse.to(torch.float32).contiguous()
+        dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+        n_buckets = 0 if bias is None else table.shape[0]
+        ws, nbytes = _workspace(_lib.load().ca_encoder_decoder_bwd_workspace_bytes(b, hq, sq, n_buckets), q.device)
+        if bias is None:
+            _lib.call("ca_cross_attention_bwd", dt, _ptr(q), _ptr(k), _ptr(v), _ptr(lens), _ptr(out), _ptr(dout),
+                      _ptr(lse), _ptr(dq), _ptr(dk), _ptr(dv), b, hq, hkv, sq, skv, d, _scale(softmax_scale, d),
+                      _ptr(ws), nbytes, _stream())
+            return [dq, dk, dv]
+        dtable = torch.empty_like(table)
+        _lib.call("ca_relative_bias_attention_bwd", dt, _ptr(q), _ptr(k), _ptr(v), _ptr(table), starts, n_buckets,
+                  _ptr(lens), _ptr(out), _ptr(dout), _ptr(lse), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dtable), b, hq,
+                  hkv, sq, skv, d, _scale(softmax_scale, d), int(bool(is_causal)), _ptr(ws), nbytes, _stream())
+    return [dq, dk, dv, dtable.to(bias[0].dtype)]
+
+
+def cross_attention_forward(q, k, v, kv_lens=None, softmax_scale=None):
+    """O = softmax(Q K^T * scale) V over keys of another length: a decoder's
+    queries q [B, Hq, Sq, D] against an encoder's k, v [B, Hkv, Skv, D] (Hkv a
+    divisor of Hq), of which sequence b has its first ``kv_lens[b]`` (integers
+    [B] on the device, taken into [0, Skv]; None: all). What k and v hold past
+    them is never used; a sequence without a key gives zeros. Any Sq from a
+    single token on; fp16 / bf16 / float32. No reference counterpart."""
+    return _encdec_forward(q, k, v, kv_lens, softmax_scale, False)[0]
+
+
+def cross_attention_forward_lse(q, k, v, kv_lens=None, softmax_scale=None):
+    """(O, LSE): cross_attention_forward and the natural-log logsumexp of every
+    row's scaled logits, [B, Hq, Sq] float32 (-inf for a row without a key)."""
+    return _encdec_forward(q, k, v, kv_lens, softmax_scale, True)
+
+
+def cross_attention_backward(dout, q, k, v, out, lse, kv_lens=None, softmax_scale=None):
+    """[dq, dk, dv] of cross_attention_forward, given its output, the gradient of
+    it and its LSE (as flash_attention_backward). dk and dv of a sequence's keys
+    past kv_lens are zeros."""
+    return _encdec_backward(dout, q, k, v, out, lse, kv_lens, softmax_scale)
+
+
+class _CrossAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, kv_lens, softmax_scale):
+        out, lse = cross_attention_forward_lse(q, k, v, kv_lens, softmax_scale)
+        ctx.save_for_backward(q, k, v, out, lse, kv_lens)
+        ctx.softmax_scale = softmax_scale
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse, kv_lens = ctx.saved_tensors
+        return (*cross_attention_backward(dout.contiguous(), q, k, v, out, lse, kv_lens, ctx.softmax_scale),
+                None, None)
+
+
+def cross_attention(q, k, v, kv_lens=None, softmax_scale=None):
+    """cross_attention_forward, differentiable with respect to q, k and v when any
+    of them requires grad."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
+        return _CrossAttention.apply(q, k, v, kv_lens, softmax_scale)
+    return cross_attention_forward(q, k, v, kv_lens, softmax_scale)
+
+
+def relative_bias_attention_forward(q, k, v, bias_table, kv_lens=None, is_causal=False, softmax_scale=None,
+                                    max_distance=128):
+    """Self-attention with a learned relative position bias: bias_table[bucket, h]
+    is added to the scaled logit of every query i and key j whose j - i lies in
+    the bucket.
+
+    q, k, v, kv_lens, softmax_scale: as cross_attention_forward (a model whose
+    logits are not scaled passes 1.0). bias_table: [num_buckets, Hq], fp16 / bf16
+    / float32; finite values are taken into [-32768, 32768], -inf masks. Causal:
+    keys j > i are masked and all buckets count i - j. Otherwise keys up to their
+    query (j <= i) have the first half of the buckets and those after it the
+    second, by |j - i|. Half of such a side's buckets hold one distance each
+    (from 0 on), the other half distances that grow as a power up to
+    max_distance (at most 2048); what lies beyond is in the last one. No
+    reference counterpart."""
+    return _encdec_forward(q, k, v, kv_lens, softmax_scale, False, (bias_table, max_distance), is_causal)[0]
+
+
+def relative_bias_attention_forward_lse(q, k, v, bias_table, kv_lens=None, is_causal=False, softmax_scale=None,
+                                        max_distance=128):
+    """(O, LSE): relative_bias_attention_forward and the natural-log logsumexp of
+    every row's biased logits, [B, Hq, Sq] float32."""
+    return _encdec_forward(q, k, v, kv_lens, softmax_scale, True, (bias_table, max_distance), is_causal)
+
+
+def relative_bias_attention_backward(dout, q, k, v, out, lse, bias_table, kv_lens=None, is_causal=False,
+                                     softmax_scale=None, max_distance=128):
+    """[dq, dk, dv, dtable] of relative_bias_attention_forward, given its output,
+    the gradient of it and its LSE. dtable, of bias_table's type, is summed over
+    the batch in an order that does not depend on timing."""
+    return _encdec_backward(dout, q, k, v, out, lse, kv_lens, softmax_scale, (bias_table, max_distance), is_causal)
+
+
+class _RelativeBiasAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, bias_table, kv_lens, is_causal, softmax_scale, max_distance):
+        out, lse = relative_bias_attention_forward_lse(q, k, v, bias_table, kv_lens, is_causal, softmax_scale,
+                                                       max_distance)
+        ctx.save_for_backward(q, k, v, out, lse, bias_table, kv_lens)
+        ctx.rest = is_causal, softmax_scale, max_distance
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse, table, kv_lens = ctx.saved_tensors
+        grads = relative_bias_attention_backward(dout.contiguous(), q, k, v, out, lse, table, kv_lens, *ctx.rest)
+        return (*grads, None, None, None, None)
+
+
+def relative_bias_attention(q, k, v, bias_table, kv_lens=None, is_causal=False, softmax_scale=None,
+                            max_distance=128):
+    """relative_bias_attention_forward, differentiable with respect to q, k, v and
+    bias_table when any of them requires grad."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, bias_table)):
+        return _RelativeBiasAttention.apply(q, k, v, bias_table, kv_lens, is_causal, softmax_scale, max_distance)
+    return relative_bias_attention_forward(q, k, v, bias_table, kv_lens, is_causal, softmax_scale, max_distance)
+
+
+def relative_bias_decode(q, k, v, bias_table, context_lens=None, softmax_scale=None, max_distance=128):
+    """The single-token form of causal relative_bias_attention: q [B, Hq, 1, D]
+    against a contiguous cache k, v [B, Hkv, S, D], the token of sequence b at
+    the position of the last of its first ``context_lens[b]`` keys (None: S), its
+    own among them. What the cache holds past them is never used."""
+    b, hq, hkv, sq, skv, d, lens = _encdec_checks(q, k, v, context_lens)
+    _check(sq == 1, "Query sequence length must be 1 for relative_bias_decode")
+    dt = _dtype_code(q, "Relative Bias Decode")
+    with torch.cuda.device(q.device):
+        table, starts = _bias_checks(q, bias_table, True, max_distance)
+        q, k, v = _aligned(q), _aligned(k), _aligned(v)
+        out = torch.empty_like(q)
+        ws, nbytes = _workspace(_lib.load().ca_flash_decode_workspace_bytes(dt, b, hq, hkv, skv, d), q.device)
+        _lib.call("ca_relative_bias_decode", dt, _ptr(q), _ptr(k), _ptr(v), _ptr(table), starts, table.shape[0],
+                  _ptr(lens), _ptr(out), b, hq, hkv, skv, d, _scale(softmax_scale, d), _ptr(ws), nbytes, _stream())
+    return out
 
 
 # ---------------------------------------------------------------------------

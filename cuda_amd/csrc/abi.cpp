@@ -8,6 +8,7 @@
 // launching, e.g. flash_attention_v2_kernel.cuh:233-304).
 #include <hip/hip_runtime.h>
 
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <string>
@@ -202,6 +203,196 @@ ca_status ca_flash_attention_bwd(ca_dtype dtype, const void* q, const void* k, c
                                        num_q_heads, num_kv_heads, seq_len, head_dim,
                                        softmax_scale, is_causal != 0, workspace,
                                        (hipStream_t)stream),
+                  what);
+}
+
+// ---- cross attention and relative position bias ----
+
+// The shape of a call; false with a message if a size is out of range. Empty
+// calls (no sequence, query or key) are valid.
+static ca_status encdec_shape(const char* what, ca_dtype dtype, int batch, int hq, int hkv, int q_len, int kv_len,
+                              int head_dim, float scale, const int32_t* kv_lens, ca::EncDecShape* s) {
+  ca_status st;
+  if ((st = check_float_dtype(dtype, what)) != CA_OK) return st;
+  if ((st = check_heads(hq, hkv, what)) != CA_OK) return st;
+  if ((st = check_head_dim(head_dim, what)) != CA_OK) return st;
+  if (batch < 0 || q_len < 0 || kv_len < 0) return fail(CA_INVALID_ARGUMENT, "%s: negative size", what);
+  if (!std::isfinite(scale)) return fail(CA_INVALID_ARGUMENT, "%s: softmax_scale must be finite", what);
+  if (batch > 0) {
+    if ((st = check_sizes(batch, hq, q_len, head_dim, what)) != CA_OK) return st;
+    if ((st = check_sizes(batch, hkv, kv_len, head_dim, what)) != CA_OK) return st;
+    if ((long long)batch * hq > INT_MAX) return fail(CA_INVALID_ARGUMENT, "%s: too many heads", what);
+  }
+  *s = ca::EncDecShape{batch, hq, hkv, q_len, kv_len, head_dim, scale, kv_lens};
+  return CA_OK;
+}
+
+static ca_status bias_spec(const char* what, const float* table, const int32_t* starts, int num_buckets,
+                           bool one_sided, ca::BiasSpec* b) {
+  if (num_buckets < 1 || num_buckets > 256 || (!one_sided && num_buckets % 2))
+    return fail(CA_INVALID_ARGUMENT, "%s: num_buckets must be in [1, 256], and even when not causal (got %d)", what,
+                num_buckets);
+  if (!table || !starts) return fail(CA_INVALID_ARGUMENT, "%s: null bias table or bucket starts", what);
+  const int side = one_sided ? num_buckets : num_buckets / 2;
+  if (starts[0] != 0) return fail(CA_INVALID_ARGUMENT, "%s: bucket_starts must begin with 0", what);
+  for (int i = 1; i < side; ++i)
+    if (starts[i] < starts[i - 1] || starts[i] > 2048)
+      return fail(CA_INVALID_ARGUMENT, "%s: bucket_starts must not fall, and stay within 2048", what);
+  *b = ca::BiasSpec{table, side, one_sided, starts};
+  return CA_OK;
+}
+
+static ca_status check_pointers(const char* what, std::initializer_list<const void*> needed, bool required) {
+  for (const void* p : needed) {
+    if (!p && required) return fail(CA_INVALID_ARGUMENT, "%s: null pointer", what);
+    if (!aligned16(p)) return fail(CA_INVALID_ARGUMENT, "%s: pointers must be 16-byte aligned", what);
+  }
+  return CA_OK;
+}
+
+static ca_status check_workspace(const char* what, const void* ws, size_t given, size_t need) {
+  if (given < need || (need && !ws))
+    return fail(CA_INVALID_ARGUMENT, "%s: workspace of %zu bytes required, %zu given", what, need, given);
+  if (need && !aligned16(ws)) return fail(CA_INVALID_ARGUMENT, "%s: pointers must be 16-byte aligned", what);
+  return CA_OK;
+}
+
+// Sizes a workspace query takes; 0 bytes for others (the call itself says why).
+static bool encdec_sizes_ok(ca_dtype dtype, int batch, int hq, int hkv, int q_len, int kv_len, int head_dim) {
+  return (dtype == CA_BF16 || dtype == CA_F16 || dtype == CA_F32) && batch > 0 && hq > 0 && hkv > 0 && hq % hkv == 0 &&
+         q_len > 0 && kv_len > 0 && (head_dim == 64 || head_dim == 128) &&
+         product_at_most(1LL << 40, {batch, hq, q_len, head_dim}) &&
+         product_at_most(1LL << 40, {batch, hkv, kv_len, head_dim}) && (long long)batch * hq <= INT_MAX;
+}
+
+size_t ca_cross_attention_workspace_bytes(ca_dtype dtype, int batch, int num_q_heads, int num_kv_heads, int q_len,
+                                          int kv_len, int head_dim, int with_lse) {
+  if (!encdec_sizes_ok(dtype, batch, num_q_heads, num_kv_heads, q_len, kv_len, head_dim)) return 0;
+  const ca::EncDecShape s{batch, num_q_heads, num_kv_heads, q_len, kv_len, head_dim, 1.f, nullptr};
+  return ca::cross_workspace_bytes((int)dtype, s, false, false, with_lse != 0);
+}
+
+size_t ca_relative_bias_attention_workspace_bytes(ca_dtype dtype, int batch, int num_q_heads, int num_kv_heads,
+                                                  int q_len, int kv_len, int head_dim, int is_causal) {
+  if (!encdec_sizes_ok(dtype, batch, num_q_heads, num_kv_heads, q_len, kv_len, head_dim)) return 0;
+  const ca::EncDecShape s{batch, num_q_heads, num_kv_heads, q_len, kv_len, head_dim, 1.f, nullptr};
+  return ca::cross_workspace_bytes((int)dtype, s, true, is_causal != 0, true);
+}
+
+size_t ca_encoder_decoder_bwd_workspace_bytes(int batch, int num_q_heads, int q_len, int num_buckets) {
+  if (batch <= 0 || num_q_heads <= 0 || q_len <= 0 || num_buckets < 0 || num_buckets > 256 ||
+      !product_at_most(1LL << 40, {batch, num_q_heads, q_len}))
+    return 0;
+  return ca::cross_bwd_workspace_bytes(ca::EncDecShape{batch, num_q_heads, num_q_heads, q_len, 0, 64, 1.f, nullptr},
+                                       num_buckets);
+}
+
+static ca_status encdec_forward(const char* what, ca_dtype dtype, const void* q, const void* k, const void* v, void* o,
+                                float* lse, const ca::EncDecShape& s, const ca::BiasSpec* bias, bool causal,
+                                void* workspace, size_t workspace_bytes, void* stream) {
+  ca_status st;
+  if (s.B == 0 || s.Sq == 0) return CA_OK;
+  if ((st = check_pointers(what, {q, o}, true)) != CA_OK) return st;
+  if ((st = check_pointers(what, {k, v}, s.Skv > 0)) != CA_OK) return st;
+  const size_t need = s.Skv > 0 ? ca::cross_workspace_bytes((int)dtype, s, bias != nullptr, causal, lse != nullptr) : 0;
+  if ((st = check_workspace(what, workspace, workspace_bytes, need)) != CA_OK) return st;
+  return from_hip(ca::launch_cross((int)dtype, q, k, v, o, lse, s, bias, causal, workspace, need,
+                                   (hipStream_t)stream),
+                  what);
+}
+
+static ca_status encdec_backward(const char* what, ca_dtype dtype, const void* q, const void* k, const void* v,
+                                 const void* o, const void* dout, const float* lse, void* dq, void* dk, void* dv,
+                                 float* dtable, const ca::EncDecShape& s, const ca::BiasSpec* bias, bool causal,
+                                 void* workspace, size_t workspace_bytes, void* stream) {
+  ca_status st;
+  const bool rows = s.B > 0 && s.Sq > 0, keys = s.B > 0 && s.Skv > 0;
+  if ((st = check_pointers(what, {q, o, dout, dq}, rows)) != CA_OK) return st;
+  if (rows && !lse) return fail(CA_INVALID_ARGUMENT, "%s: null pointer", what);
+  if ((st = check_pointers(what, {k, v, dk, dv}, keys)) != CA_OK) return st;
+  if (bias && !dtable) return fail(CA_INVALID_ARGUMENT, "%s: null pointer", what);
+  const size_t need = rows ? ca::cross_bwd_workspace_bytes(s, bias ? bias->buckets() : 0) : 0;
+  if ((st = check_workspace(what, workspace, workspace_bytes, need)) != CA_OK) return st;
+  return from_hip(ca::launch_cross_bwd((int)dtype, q, k, v, o, dout, lse, dq, dk, dv, dtable, s, bias, causal,
+                                       workspace, (hipStream_t)stream),
+                  what);
+}
+
+ca_status ca_cross_attention(ca_dtype dtype, const void* q, const void* k, const void* v, const int32_t* kv_lens,
+                             void* o, float* lse, int batch, int num_q_heads, int num_kv_heads, int q_len, int kv_len,
+                             int head_dim, float softmax_scale, void* workspace, size_t workspace_bytes,
+                             void* stream) {
+  const char* what = "cross_attention";
+  ca::EncDecShape s;
+  ca_status st = encdec_shape(what, dtype, batch, num_q_heads, num_kv_heads, q_len, kv_len, head_dim, softmax_scale,
+                              kv_lens, &s);
+  if (st != CA_OK) return st;
+  return encdec_forward(what, dtype, q, k, v, o, lse, s, nullptr, false, workspace, workspace_bytes, stream);
+}
+
+ca_status ca_cross_attention_bwd(ca_dtype dtype, const void* q, const void* k, const void* v, const int32_t* kv_lens,
+                                 const void* o, const void* dout, const float* lse, void* dq, void* dk, void* dv,
+                                 int batch, int num_q_heads, int num_kv_heads, int q_len, int kv_len, int head_dim,
+                                 float softmax_scale, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "cross_attention_backward";
+  ca::EncDecShape s;
+  ca_status st = encdec_shape(what, dtype, batch, num_q_heads, num_kv_heads, q_len, kv_len, head_dim, softmax_scale,
+                              kv_lens, &s);
+  if (st != CA_OK) return st;
+  return encdec_backward(what, dtype, q, k, v, o, dout, lse, dq, dk, dv, nullptr, s, nullptr, false, workspace,
+                         workspace_bytes, stream);
+}
+
+ca_status ca_relative_bias_attention(ca_dtype dtype, const void* q, const void* k, const void* v,
+                                     const float* bias_table, const int32_t* bucket_starts, int num_buckets,
+                                     const int32_t* kv_lens, void* o, float* lse, int batch, int num_q_heads,
+                                     int num_kv_heads, int q_len, int kv_len, int head_dim, float softmax_scale,
+                                     int is_causal, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "relative_bias_attention";
+  ca::EncDecShape s;
+  ca::BiasSpec b;
+  ca_status st = encdec_shape(what, dtype, batch, num_q_heads, num_kv_heads, q_len, kv_len, head_dim, softmax_scale,
+                              kv_lens, &s);
+  if (st != CA_OK) return st;
+  if ((st = bias_spec(what, bias_table, bucket_starts, num_buckets, is_causal != 0, &b)) != CA_OK) return st;
+  return encdec_forward(what, dtype, q, k, v, o, lse, s, &b, is_causal != 0, workspace, workspace_bytes, stream);
+}
+
+ca_status ca_relative_bias_attention_bwd(ca_dtype dtype, const void* q, const void* k, const void* v,
+                                         const float* bias_table, const int32_t* bucket_starts, int num_buckets,
+                                         const int32_t* kv_lens, const void* o, const void* dout, const float* lse,
+                                         void* dq, void* dk, void* dv, float* dtable, int batch, int num_q_heads,
+                                         int num_kv_heads, int q_len, int kv_len, int head_dim, float softmax_scale,
+                                         int is_causal, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "relative_bias_attention_backward";
+  ca::EncDecShape s;
+  ca::BiasSpec b;
+  ca_status st = encdec_shape(what, dtype, batch, num_q_heads, num_kv_heads, q_len, kv_len, head_dim, softmax_scale,
+                              kv_lens, &s);
+  if (st != CA_OK) return st;
+  if ((st = bias_spec(what, bias_table, bucket_starts, num_buckets, is_causal != 0, &b)) != CA_OK) return st;
+  return encdec_backward(what, dtype, q, k, v, o, dout, lse, dq, dk, dv, dtable, s, &b, is_causal != 0, workspace,
+                         workspace_bytes, stream);
+}
+
+ca_status ca_relative_bias_decode(ca_dtype dtype, const void* q, const void* k, const void* v, const float* bias_table,
+                                  const int32_t* bucket_starts, int num_buckets, const int32_t* context_lens, void* o,
+                                  int batch, int num_q_heads, int num_kv_heads, int kv_len, int head_dim,
+                                  float softmax_scale, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "relative_bias_decode";
+  ca::EncDecShape s;
+  ca::BiasSpec b;
+  ca_status st = encdec_shape(what, dtype, batch, num_q_heads, num_kv_heads, 1, kv_len, head_dim, softmax_scale,
+                              context_lens, &s);
+  if (st != CA_OK) return st;
+  if ((st = bias_spec(what, bias_table, bucket_starts, num_buckets, true, &b)) != CA_OK) return st;
+  if (batch == 0) return CA_OK;
+  if ((st = check_pointers(what, {q, o}, true)) != CA_OK) return st;
+  if ((st = check_pointers(what, {k, v}, kv_len > 0)) != CA_OK) return st;
+  const size_t need = ca::decode_workspace_bytes(batch, num_q_heads, head_dim, kv_len);
+  if ((st = check_workspace(what, workspace, workspace_bytes, need)) != CA_OK) return st;
+  return from_hip(ca::launch_encdec_decode((int)dtype, q, k, v, o, s, &b, workspace, workspace_bytes,
+                                           (hipStream_t)stream),
                   what);
 }
 

@@ -32,9 +32,16 @@
 // the next product's k-steps, so P and dS go from accumulators to operands
 // without leaving registers. The transposed operands (K^T, Q^T, dO^T) come
 // from row-major LDS tiles through ds_read_b64_tr_b16.
+//
+// The same kernels, with an X of their own (encdec.h), are the backward of cross
+// attention (keys of another length; dK and dV of a sequence's padded keys are
+// 0) and of attention with a relative position bias: S starts as bias / scale in
+// the accumulators, and the dQ kernel, which has every dS, also sums them by
+// bucket (BiasGrad) for the gradient of the bias table.
 #include <algorithm>
 
 #include "common.h"
+#include "encdec.h"
 #include "launch.h"
 #include "lds_dma.h"
 
@@ -46,8 +53,9 @@ __device__ __forceinline__ int rho32(int i) { return (i & 0x13) | ((i & 4) << 1)
 // Per query row of B * Hq * S: the pair (LSE * log2(e), D) with D = sum_d
 // dO[row][d] * O[row][d] (flash_attention_bwd_kernel.cuh:96-108), so the
 // kernels below fetch both terms of a row with one 8-byte load. D / 8 lanes
-// per row, 8 elements each.
-template <typename Tr, int D>
+// per row, 8 elements each. X: rows without a key (LSE -inf) get +inf, with which
+// every P is 0.
+template <typename Tr, int D, class X>
 __global__ __launch_bounds__(256) void bwd_rowdot_kernel(const uint16_t* __restrict__ O,
                                                          const uint16_t* __restrict__ dO,
                                                          const float* __restrict__ LSE,
@@ -67,7 +75,8 @@ __global__ __launch_bounds__(256) void bwd_rowdot_kernel(const uint16_t* __restr
 #pragma unroll
   for (int m = L / 2; m >= 1; m >>= 1) acc += __shfl_xor(acc, m, 64);
   if (row < rows && c == 0) {
-    LD[2 * row] = LSE[row] * kLog2e;
+    const float l = LSE[row];
+    LD[2 * row] = X::kCross && l == kNegInf ? -kNegInf : l * kLog2e;
     LD[2 * row + 1] = acc;
   }
 }
@@ -246,14 +255,15 @@ __device__ __forceinline__ void reduce_parts(f32x16 (&acc)[NACC], unsigned char*
 // dQ of query tile qt (32 QG rows) of head bh: the keys [0, kv_end) in tiles of
 // 64, each computed as two halves of 32 keys. QG = 8: a wave per 32 rows; QG =
 // 4: two waves share 32 rows, each taking one half of every tile, and add up
-// at the end.
-template <typename Tr, int D, bool CAUSAL, int QG>
+// at the end. With a bias, the sums of dS by bucket go to part_table [buckets].
+template <typename Tr, int D, bool CAUSAL, int QG, class X>
 __device__ CA_INLINE void bwd_dq_dma_tile(const uint16_t* __restrict__ Q,
                                          const uint16_t* __restrict__ K,
                                          const uint16_t* __restrict__ V,
                                          const uint16_t* __restrict__ dO,
                                          const float* __restrict__ LD, uint16_t* __restrict__ dQ,
-                                         int S, int Hq, int Hkv, float scale, int bh, int qt) {
+                                         int S, int Hq, int Hkv, float scale, const X& x,
+                                         unsigned char* bias_mem, float* __restrict__ part_table, int bh, int qt) {
   using namespace bwdma;
   using Gm = Geom<D>;
   using vec8 = typename Tr::vec8;
@@ -267,6 +277,9 @@ __device__ CA_INLINE void bwd_dq_dma_tile(const uint16_t* __restrict__ Q,
   constexpr int kStageB = 2 * kTileB;          // K tile, then V tile
   constexpr int kDma = kTileB / 1024 / kNW;    // 1-KB loads per wave per K (and V) tile
   static_assert(kDma * 1024 * kNW == kTileB, "whole 1-KB loads per wave");
+  // (the bias and its totals take up to 30 KB of LDS)
+  constexpr int kStages = X::kBias && D == 128 ? bwdma::kStages - 1 : bwdma::kStages;
+  constexpr int kDist = kStages - 1;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[kStages * kStageB];
   // per wave: 32 dQ rows x 128 bytes, staging the dQ store
   __shared__ __attribute__((aligned(16))) unsigned char qstg[kNW * 32 * 128];
@@ -274,9 +287,14 @@ __device__ CA_INLINE void bwd_dq_dma_tile(const uint16_t* __restrict__ Q,
   const int b = bh / Hq, h = bh % Hq;
   const int hk = h / (Hq / Hkv);
   const int q0 = qt * BM;
+  int Skv = S, n_keys = S;
+  if constexpr (X::kCross) {
+    Skv = x.Skv;
+    n_keys = x.kv_len(b);
+  }
   const size_t qoff = (size_t)(b * Hq + h) * S;
-  const uint16_t* Kp = K + (size_t)(b * Hkv + hk) * S * D;
-  const uint16_t* Vp = V + (size_t)(b * Hkv + hk) * S * D;
+  const uint16_t* Kp = K + (size_t)(b * Hkv + hk) * Skv * D;
+  const uint16_t* Vp = V + (size_t)(b * Hkv + hk) * Skv * D;
   const int lane = __builtin_amdgcn_workitem_id_x() & 63;
   const int wave = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_workitem_id_x() >> 6);
   const int qg = KS == 1 ? wave : wave % QG, part = KS == 1 ? 0 : wave / QG;
@@ -284,7 +302,21 @@ __device__ CA_INLINE void bwd_dq_dma_tile(const uint16_t* __restrict__ Q,
   const int qw0 = q0 + 32 * qg;
   const int myq = qw0 + l32;
   const bool qvalid = myq < S;
-  const float c2 = scale * kLog2e;
+  float c2 = scale * kLog2e;
+  uint32_t bofs = 0, id_ofs = 0;  // LDS: the lane's bias of a block, its distances' bucket ids
+  BiasGrad grad;
+  float* totals = nullptr;        // [wave][buckets]
+  int n_buckets = 0;
+  if constexpr (X::kBias) {
+    c2 = x.scale_log2;
+    unsigned char* ids = bias_mem + bias_lds_bytes(x.reach);
+    totals = (float*)(ids + bias_id_bytes(x.reach));
+    n_buckets = x.one_sided ? x.side : 2 * x.side;
+    bofs = bias_fill(x, h, bias_mem, 64 * kNW) + 4 * (31 - l32 + 8 * hl);
+    id_ofs = bias_fill_ids(x, bias_mem, ids, 64 * kNW) + min(lane, 62);
+    grad.init(lds_off(qstg) + (uint32_t)(wave * BiasGrad::kScratchB), lds_off(totals + wave * n_buckets), n_buckets);
+    __syncthreads();
+  }
   float lse2 = -kNegInf, dd = 0.f;  // a query past S: P = 0
   vec8 qv[kNKS], gv[kNKS];          // Q and dO as B operands (column = this lane's query)
   if (qvalid) {
@@ -302,7 +334,7 @@ __device__ CA_INLINE void bwd_dq_dma_tile(const uint16_t* __restrict__ Q,
     }
   }
 
-  const int kv_end = CAUSAL ? min(S, q0 + BM) : S;
+  const int kv_end = CAUSAL ? min(n_keys, q0 + BM) : n_keys;
   const int n_tiles = (kv_end + BN - 1) / BN;
   // 32-key halves this wave computes; the last one holds the causal diagonal
   // or the end of the keys
@@ -345,12 +377,35 @@ __device__ CA_INLINE void bwd_dq_dma_tile(const uint16_t* __restrict__ Q,
     // S^T = K Q^T, dP^T = V dO^T: register r of half hl <-> key
     // k0 + 16 (r/8) + 8 hl + r%8, column = this lane's query
     f32x16 s, dp;
+    uint32_t id = 0;   // bucket of distance k0 - qw0 - 31 + min(lane, 62)
+    u32x2 br[X::kBias ? 8 : 1];
+    if constexpr (X::kBias) {
+      const int r0 = bias_block(x, k0 - qw0 - 31);
+      id = lds_read_u8<0>(id_ofs + (uint32_t)r0);
+      const uint32_t ba = bofs + 4 * (uint32_t)r0;
+      auto bread = [&](auto i) CA_INLINE {
+        constexpr int off = 16 * (decltype(i)::value >> 2) + 2 * (decltype(i)::value & 3);
+        br[decltype(i)::value] = lds_read2_b32<off, off + 1>(ba);
+      };
+      for_const<8>(bread);
+    }
 #pragma unroll
     for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
     const uint32_t ka = hb + rofs, va = ka + kTileB;
     u32x4 kr[2], vr[2];
     kr[0] = lds_read_b128<0>(ka);
     vr[0] = lds_read_b128<0>(va);
+    if constexpr (X::kBias) {
+      wait_lgkm<2>();
+      after_wait(id);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        after_wait(br[i]);
+        const uint32_t lo = br[i][0], hi = br[i][1];
+        s[2 * i] = __builtin_bit_cast(float, lo);
+        s[2 * i + 1] = __builtin_bit_cast(float, hi);
+      }
+    }
 #pragma unroll
     for (int ks = 0; ks < kNKS; ++ks) {
       const int cb = ks & 1;
@@ -368,6 +423,7 @@ __device__ CA_INLINE void bwd_dq_dma_tile(const uint16_t* __restrict__ Q,
     }
     // dS^T / scale = P (dP - D) as the B operand of dQ^T += K^T dS^T
     vec8 pb[2];
+    float dsv[X::kBias ? 16 : 1];
     auto softmax = [&](auto mask_tag) CA_INLINE {
     constexpr bool MASK = decltype(mask_tag)::value;
 #pragma unroll
@@ -381,9 +437,10 @@ __device__ CA_INLINE void bwd_dq_dma_tile(const uint16_t* __restrict__ Q,
           float p = fast_exp2(__builtin_fmaf(s[r], c2, -lse2));
           if (MASK) {
             const int key = k0 + 16 * kk + 8 * hl + 2 * j + e;
-            if (key >= S || (CAUSAL && key > myq)) p = 0.f;
+            if (key >= n_keys || (CAUSAL && key > myq)) p = 0.f;
           }
           ds[e] = p * (dp[r] - dd);
+          if constexpr (X::kBias) dsv[r] = ds[e];
         }
         const vec2 pk = Tr::pack2(ds[0], ds[1]);
         pb[kk][2 * j] = pk[0];
@@ -403,6 +460,7 @@ __device__ CA_INLINE void bwd_dq_dma_tile(const uint16_t* __restrict__ Q,
       acc[ob] = Tr::mfma32(x0, pb[0], acc[ob]);
       acc[ob] = Tr::mfma32(x1, pb[1], acc[ob]);
     }
+    if constexpr (X::kBias) grad.template block<8>(dsv, (int)id);
   };
 
 #pragma unroll
@@ -416,31 +474,48 @@ __device__ CA_INLINE void bwd_dq_dma_tile(const uint16_t* __restrict__ Q,
     for (int hh = 0; hh < 2; ++hh) {
       const int j = 2 * t + hh;
       if (j < w_halves && (KS == 1 || hh == part)) {
-        half(sb + hh * 32 * kRowB, 32 * j, CAUSAL ? (j == w_halves - 1) : (32 * j + 32 > S));
+        half(sb + hh * 32 * kRowB, 32 * j, CAUSAL ? (j == w_halves - 1) : (32 * j + 32 > n_keys));
       }
     }
   }
   wait_vmcnt<0>();  // no load may still target this workgroup's LDS when it exits
+  if constexpr (X::kBias) {
+    grad.flush();
+    wait_lgkm<0>();
+    __syncthreads();
+    for (int i = threadIdx.x; i < n_buckets; i += 64 * kNW) {
+      float t = 0.f;
+#pragma unroll
+      for (int w = 0; w < kNW; ++w) t += totals[w * n_buckets + i];
+      part_table[i] = t;
+    }
+  }
   if constexpr (KS > 1) reduce_parts<kNOB, QG, KS>(acc, lds, part, qg, lane);
   if (part == 0)
     store_rowsT_lds<Tr, kNOB, 128>(dQ + qoff * D, qw0, S, acc, scale,
                                    lds_off(qstg) + (uint32_t)(qg * 32 * 128), lane);
 }
 
-template <typename Tr, int D, bool CAUSAL, int QG>
+template <typename Tr, int D, bool CAUSAL, int QG, class X>
 __global__ __launch_bounds__(64 * bwdma::kNW) void bwd_dq_dma_kernel(
     const uint16_t* __restrict__ Q, const uint16_t* __restrict__ K,
     const uint16_t* __restrict__ V, const uint16_t* __restrict__ dO,
     const float* __restrict__ LD, uint16_t* __restrict__ dQ, int S, int Hq, int Hkv, float scale,
-    int n_qt, int n_bh, int n_work, int order) {
+    int n_qt, int n_bh, int n_work, int order, X x, float* __restrict__ part_table) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char bias_mem[];
   const QTileWork wk =
       prefill_item(__builtin_amdgcn_workgroup_id_x(), n_work, n_qt, n_bh, order);
   const int n_pass = wk.qt1 < 0 ? 1 : 2;
 #pragma clang loop unroll(disable)
   for (int pass = 0; pass < n_pass; ++pass) {
     if (pass) __builtin_amdgcn_s_barrier();  // every wave is done reading the ring
-    bwd_dq_dma_tile<Tr, D, CAUSAL, QG>(Q, K, V, dO, LD, dQ, S, Hq, Hkv, scale, pass ? wk.bh1 : wk.bh0,
-                               pass ? wk.qt1 : wk.qt0);
+    const int bh = pass ? wk.bh1 : wk.bh0, qt = pass ? wk.qt1 : wk.qt0;
+    float* pt = nullptr;
+    if constexpr (X::kBias) {
+      if (pass) __syncthreads();  // ... and the totals
+      pt = part_table + ((size_t)bh * n_qt + qt) * (x.one_sided ? x.side : 2 * x.side);
+    }
+    bwd_dq_dma_tile<Tr, D, CAUSAL, QG, X>(Q, K, V, dO, LD, dQ, S, Hq, Hkv, scale, x, bias_mem, pt, bh, qt);
   }
 }
 
@@ -450,14 +525,15 @@ __global__ __launch_bounds__(64 * bwdma::kNW) void bwd_dq_dma_kernel(
 // dO and the (LSE log2 e, D) pairs stream through the ring. KG = 8: a wave
 // per 32 keys. KG = 4 or 2: QS = 8 / KG waves share 32 keys, each taking every
 // QS-th query tile, and add up at the end.
-template <typename Tr, int D, bool CAUSAL, int KG>
+template <typename Tr, int D, bool CAUSAL, int KG, class X>
 __device__ CA_INLINE void bwd_dkv_dma_tile(const uint16_t* __restrict__ Q,
                                           const uint16_t* __restrict__ K,
                                           const uint16_t* __restrict__ V,
                                           const uint16_t* __restrict__ dO,
                                           const float* __restrict__ LD, uint16_t* __restrict__ dK,
                                           uint16_t* __restrict__ dV, int S, int Hq, int Hkv,
-                                          float scale, int bhk, int kt) {
+                                          float scale, const X& x, unsigned char* bias_mem, int bhk,
+                                          int kt) {
   using namespace bwdma;
   using Gm = Geom<D>;
   using vec8 = typename Tr::vec8;
@@ -485,7 +561,12 @@ __device__ CA_INLINE void bwd_dkv_dma_tile(const uint16_t* __restrict__ Q,
   const int b = bhk / Hkv, hk = bhk % Hkv;
   const int G = Hq / Hkv;
   const int K0 = kt * BK;
-  const size_t kvoff = (size_t)(b * Hkv + hk) * S;
+  int Skv = S, n_keys = S;
+  if constexpr (X::kCross) {
+    Skv = x.Skv;
+    n_keys = x.kv_len(b);
+  }
+  const size_t kvoff = (size_t)(b * Hkv + hk) * Skv;
   // The lane index is recomputed per call (lane_here): otherwise the
   // compiler hoists the lane-derived load offsets of both passes out of the
   // kernel's pass loop and keeps them live through the tile loop, which at
@@ -496,14 +577,18 @@ __device__ CA_INLINE void bwd_dkv_dma_tile(const uint16_t* __restrict__ Q,
   const int l32 = lane & 31, hl = lane >> 5;
   const int kw0 = K0 + 32 * kg;
   const int mykey = kw0 + l32;
-  const bool kvalid = mykey < S;
-  const float c2 = scale * kLog2e;
+  const bool kvalid = mykey < n_keys;
+  float c2 = scale * kLog2e;
+  // LDS: the lane's bias of a block that starts at distance r0; register r is
+  // 4 (l32 + 23 - 8 hl + 8 - off(r)) bytes past it, off = 16 (r / 8) + r % 8
+  uint32_t bofs = 0;
+  if constexpr (X::kBias) c2 = x.scale_log2;
 
   // the key group's V rows -> LDS (rows past S read as zero); its other parts
   // write the same bytes, so a wave's own loads cover its reads
   unsigned char* vw = lds + kg * kVB;
   {
-    const __amdgpu_buffer_rsrc_t rs = make_rsrc(V + kvoff * D, (uint32_t)S * kRowB);
+    const __amdgpu_buffer_rsrc_t rs = make_rsrc(V + kvoff * D, (uint32_t)n_keys * kRowB);
 #pragma unroll
     for (int i = 0; i < kVB / 1024; ++i)
       dma16_buf(rs, (CA_LDS void*)(vw + 1024 * i),
@@ -521,10 +606,14 @@ __device__ CA_INLINE void bwd_dkv_dma_tile(const uint16_t* __restrict__ Q,
   }
 
   const int t_begin = CAUSAL ? K0 / BQ : 0;
-  const int nt = max(0, (S + BQ - 1) / BQ - t_begin);  // query tiles per q head
-  const int n_u = G * nt;                         // tiles of all q heads
+  int nt = max(0, (S + BQ - 1) / BQ - t_begin);  // query tiles per q head
+  if constexpr (X::kCross)
+    if (K0 >= n_keys) nt = 0;
+  // with a bias, a stage's tiles are of one q head
+  const int ntp = X::kBias ? (nt + QS - 1) / QS * QS : nt;
+  const int n_u = G * ntp;                        // tiles of all q heads
   const int n_it = (n_u + QS - 1) / QS;
-  // tile u of the walk: head hk G + u / nt, queries from BQ (t_begin + u % nt)
+  // tile u of the walk: head hk G + u / ntp, queries from BQ (t_begin + u % ntp)
   const int wsub = kT == kNW ? wave : wave % kT;
   auto issue = [&](int it, int slot) CA_INLINE {
     unsigned char* st = lds + KG * kVB + slot * kStageB;
@@ -535,8 +624,8 @@ __device__ CA_INLINE void bwd_dkv_dma_tile(const uint16_t* __restrict__ Q,
       // past the walk (slots the loop never reads): offsets past the slice, zeros
       const bool past = u >= n_u;
       const int uc = past ? 0 : u;
-      q0 = past ? S : (t_begin + uc % max(nt, 1)) * BQ;
-      ho = (size_t)(b * Hq + hk * G + uc / max(nt, 1)) * S;
+      q0 = past ? S : (t_begin + uc % max(ntp, 1)) * BQ;
+      ho = (size_t)(b * Hq + hk * G + uc / max(ntp, 1)) * S;
     };
     const uint32_t sz = (uint32_t)S * kRowB;
 #pragma unroll
@@ -579,6 +668,15 @@ __device__ CA_INLINE void bwd_dkv_dma_tile(const uint16_t* __restrict__ Q,
     // S = Q K^T, dP = dO V^T: register r of half hl <-> query
     // q0 + 16 (r/8) + 8 hl + r%8, column = this lane's key
     f32x16 s, dp;
+    u32x2 br[X::kBias ? 8 : 1];
+    if constexpr (X::kBias) {
+      const uint32_t ba = bofs + 4 * (uint32_t)bias_block(x, kw0 - q0 - 31);
+      auto bread = [&](auto i) CA_INLINE {
+        constexpr int off = 23 - 16 * (decltype(i)::value >> 2) - 2 * (decltype(i)::value & 3);
+        br[decltype(i)::value] = lds_read2_b32<off, off - 1>(ba);
+      };
+      for_const<8>(bread);
+    }
 #pragma unroll
     for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
     const uint32_t qa = sb + rofs, ga = qa + kTileB;
@@ -586,6 +684,16 @@ __device__ CA_INLINE void bwd_dkv_dma_tile(const uint16_t* __restrict__ Q,
     qr[0] = lds_read_b128<0>(qa);
     gr[0] = lds_read_b128<0>(ga);
     vr[0] = lds_read_b128<0>(vofs);
+    if constexpr (X::kBias) {
+      wait_lgkm<3>();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        after_wait(br[i]);
+        const uint32_t lo = br[i][0], hi = br[i][1];
+        s[2 * i] = __builtin_bit_cast(float, lo);
+        s[2 * i + 1] = __builtin_bit_cast(float, hi);
+      }
+    }
 #pragma unroll
     for (int ks = 0; ks < kNKS; ++ks) {
       const int cb = ks & 1;
@@ -673,9 +781,15 @@ __device__ CA_INLINE void bwd_dkv_dma_tile(const uint16_t* __restrict__ Q,
     else wait_vmcnt<kLoads * (kDist - 1)>();
     __builtin_amdgcn_s_barrier();  // ... and every wave's; slot of it-1 is free
     issue(it + kDist, kPow2 ? (it + kDist) % kStages : slot == 0 ? kStages - 1 : slot - 1);
+    if constexpr (X::kBias) {
+      // the next q head's bias (every wave has read the one before: the barrier)
+      if (it * QS % ntp == 0)
+        bofs = bias_fill(x, hk * G + it * QS / ntp, bias_mem, 64 * kNW) + 4 * (l32 + 8 - 8 * hl);
+    }
     const int u = it * QS + part;
-    const int q0 = (t_begin + u % nt) * BQ;
-    if ((QS == 1 || u < n_u) && kw0 < S && (!CAUSAL || q0 >= kw0)) {  // causal: queries before every key of the wave
+    const int q0 = (t_begin + u % ntp) * BQ;
+    // (q0 < S: a head's tiles, filled up to whole stages)
+    if ((QS == 1 || (X::kBias ? q0 < S : u < n_u)) && kw0 < n_keys && (!CAUSAL || q0 >= kw0)) {  // causal: queries before every key of the wave
       const uint32_t sb = lds0 + KG * kVB + (uint32_t)(slot * kStageB + part * kSubB);
       tile(sb, q0, (CAUSAL && q0 == kw0) || q0 + BQ > S);
     }
@@ -683,21 +797,29 @@ __device__ CA_INLINE void bwd_dkv_dma_tile(const uint16_t* __restrict__ Q,
   }
   wait_vmcnt<0>();  // no load may still target this workgroup's LDS when it exits
   if constexpr (QS > 1) reduce_parts<2 * kNOB, KG, QS>(acc, lds, part, kg, lane_here());
+  if constexpr (X::kCross) {
+    // a padded key's gradients are 0, whatever its lane computed
+#pragma unroll
+    for (int i = 0; i < 2 * kNOB; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][r] = kvalid ? acc[i][r] : 0.f;
+  }
   // the key group's V rows are no longer read: their LDS block stages dK, then dV
   if (part == 0) {
-    store_rowsT_lds<Tr, kNOB, kRowB>(dK + kvoff * D, kw0, S, *(const f32x16(*)[kNOB])(acc), scale,
+    store_rowsT_lds<Tr, kNOB, kRowB>(dK + kvoff * D, kw0, Skv, *(const f32x16(*)[kNOB])(acc), scale,
                                      lds_off(vw), lane_here());
-    store_rowsT_lds<Tr, kNOB, kRowB>(dV + kvoff * D, kw0, S, *(const f32x16(*)[kNOB])(acc + kNOB), 1.f,
+    store_rowsT_lds<Tr, kNOB, kRowB>(dV + kvoff * D, kw0, Skv, *(const f32x16(*)[kNOB])(acc + kNOB), 1.f,
                                      lds_off(vw), lane_here());
   }
 }
 
-template <typename Tr, int D, bool CAUSAL, int KG>
+template <typename Tr, int D, bool CAUSAL, int KG, class X>
 __global__ __launch_bounds__(64 * bwdma::kNW) void bwd_dkv_dma_kernel(
     const uint16_t* __restrict__ Q, const uint16_t* __restrict__ K,
     const uint16_t* __restrict__ V, const uint16_t* __restrict__ dO,
     const float* __restrict__ LD, uint16_t* __restrict__ dK, uint16_t* __restrict__ dV, int S,
-    int Hq, int Hkv, float scale, int n_kt, int n_bh, int n_work, int order) {
+    int Hq, int Hkv, float scale, int n_kt, int n_bh, int n_work, int order, X x) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char bias_mem[];
   // key tile kt walks n_kt - kt query stretches: kt = n_kt - 1 - qt gives the
   // longest walks first (single) and pairs of equal total length
   const QTileWork wk =
@@ -706,7 +828,7 @@ __global__ __launch_bounds__(64 * bwdma::kNW) void bwd_dkv_dma_kernel(
 #pragma clang loop unroll(disable)
   for (int pass = 0; pass < n_pass; ++pass) {
     if (pass) __builtin_amdgcn_s_barrier();  // every wave is done reading the ring and V
-    bwd_dkv_dma_tile<Tr, D, CAUSAL, KG>(Q, K, V, dO, LD, dK, dV, S, Hq, Hkv, scale,
+    bwd_dkv_dma_tile<Tr, D, CAUSAL, KG, X>(Q, K, V, dO, LD, dK, dV, S, Hq, Hkv, scale, x, bias_mem,
                                 pass ? wk.bh1 : wk.bh0, n_kt - 1 - (pass ? wk.qt1 : wk.qt0));
   }
 }
@@ -750,41 +872,89 @@ BwdSplit bwd_split(int B, int heads, int S, bool causal, int cost4, int cost2) {
   return best;
 }
 
-template <typename Tr, int D, bool CAUSAL>
+// The X of a launch, what its kernels need beside it, and its table's gradient.
+template <class X>
+struct BwdX {
+  X x;
+  int Skv;
+  size_t dkv_lds = 0, dq_lds = 0;  // dynamic
+  float* part_table = nullptr;
+  float* dtable = nullptr;
+};
+
+template <typename Tr, int D, bool CAUSAL, class X>
 hipError_t launch_bwd_t(const void* q, const void* k, const void* v, const void* o,
                         const void* dout, const float* lse, void* dq, void* dk, void* dv, int B,
-                        int Hq, int Hkv, int S, float scale, float* ws, hipStream_t stream) {
+                        int Hq, int Hkv, int S, float scale, float* ws, const BwdX<X>& bx, hipStream_t stream) {
   const long long rows = (long long)B * Hq * S;
   const long long threads = rows * (D / 8);
   const long long g0 = (threads + 255) / 256;
   if (g0 > 0x7fffffffLL) return hipErrorInvalidValue;
-  const BwdSplit sk = bwd_split(B, Hkv, S, CAUSAL, D == 64 ? 122 : 109, D == 64 ? 168 : 142);
+  // (two waves to a key group's tiles only where LDS holds a bias beside them)
+  const BwdSplit sk = bwd_split(B, Hkv, bx.Skv, CAUSAL, D == 64 ? 122 : 109, X::kBias ? 0 : D == 64 ? 168 : 142);
   const BwdSplit sq = bwd_split(B, Hq, S, CAUSAL, 110, 0);
   if (sk.grid > 0x7fffffffLL || sq.grid > 0x7fffffffLL) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((bwd_rowdot_kernel<Tr, D>), dim3((unsigned)g0), dim3(256), 0, stream,
-                     (const uint16_t*)o, (const uint16_t*)dout, lse, ws, rows);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
+  hipError_t e = hipSuccess;
   const dim3 block(64 * bwdma::kNW);
-  const auto dkv = sk.groups == 8   ? &bwd_dkv_dma_kernel<Tr, D, CAUSAL, 8>
-                   : sk.groups == 4 ? &bwd_dkv_dma_kernel<Tr, D, CAUSAL, 4>
-                                    : &bwd_dkv_dma_kernel<Tr, D, CAUSAL, 2>;
-  hipLaunchKernelGGL(dkv, dim3((unsigned)sk.grid), block, 0, stream, (const uint16_t*)q,
-                     (const uint16_t*)k, (const uint16_t*)v, (const uint16_t*)dout, ws, (uint16_t*)dk,
-                     (uint16_t*)dv, S, Hq, Hkv, scale, sk.n_tiles, B * Hkv, (int)sk.grid, sk.order);
-  e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  const auto dqk = sq.groups == 8 ? &bwd_dq_dma_kernel<Tr, D, CAUSAL, 8>
-                                  : &bwd_dq_dma_kernel<Tr, D, CAUSAL, 4>;
-  hipLaunchKernelGGL(dqk, dim3((unsigned)sq.grid), block, 0, stream, (const uint16_t*)q,
-                     (const uint16_t*)k, (const uint16_t*)v, (const uint16_t*)dout, ws, (uint16_t*)dq,
-                     S, Hq, Hkv, scale, sq.n_tiles, B * Hq, (int)sq.grid, sq.order);
-  return hipGetLastError();
+  if (rows > 0) {
+    hipLaunchKernelGGL((bwd_rowdot_kernel<Tr, D, X>), dim3((unsigned)g0), dim3(256), 0, stream,
+                       (const uint16_t*)o, (const uint16_t*)dout, lse, ws, rows);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  if (sk.grid > 0) {
+    auto dkv = sk.groups == 8 ? &bwd_dkv_dma_kernel<Tr, D, CAUSAL, 8, X> : &bwd_dkv_dma_kernel<Tr, D, CAUSAL, 4, X>;
+    if constexpr (!X::kBias)
+      if (sk.groups == 2) dkv = &bwd_dkv_dma_kernel<Tr, D, CAUSAL, 2, X>;
+    hipLaunchKernelGGL(dkv, dim3((unsigned)sk.grid), block, bx.dkv_lds, stream, (const uint16_t*)q,
+                       (const uint16_t*)k, (const uint16_t*)v, (const uint16_t*)dout, ws, (uint16_t*)dk,
+                       (uint16_t*)dv, S, Hq, Hkv, scale, sk.n_tiles, B * Hkv, (int)sk.grid, sk.order, bx.x);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  if (sq.grid > 0) {
+    const auto dqk = sq.groups == 8 ? &bwd_dq_dma_kernel<Tr, D, CAUSAL, 8, X>
+                                    : &bwd_dq_dma_kernel<Tr, D, CAUSAL, 4, X>;
+    hipLaunchKernelGGL(dqk, dim3((unsigned)sq.grid), block, bx.dq_lds, stream, (const uint16_t*)q,
+                       (const uint16_t*)k, (const uint16_t*)v, (const uint16_t*)dout, ws, (uint16_t*)dq,
+                       S, Hq, Hkv, scale, sq.n_tiles, B * Hq, (int)sq.grid, sq.order, bx.x, bx.part_table);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  if constexpr (X::kBias)
+    return launch_bias_grad(bx.part_table, bx.dtable, B, Hq, sq.n_tiles, bx.x.one_sided ? bx.x.side : 2 * bx.x.side,
+                            stream);
+  return e;
+}
+
+// dtable[bucket][h] = the sum over sequences and tiles of part [B][Hq][n_qt]
+// [buckets]: a wave per entry, its lanes' terms in a fixed order, in 64 bits
+// (terms of both signs that nearly cancel).
+__global__ __launch_bounds__(64) void bias_grad_kernel(const float* __restrict__ part, float* __restrict__ dtable,
+                                                       int B, int Hq, int n_qt, int buckets) {
+  const int lane = threadIdx.x, bucket = blockIdx.x / Hq, h = blockIdx.x % Hq;
+  double t = 0.;
+  for (long long i = lane; i < (long long)B * n_qt; i += 64) {
+    const long long b = i / n_qt, qt = i % n_qt;
+    t += (double)part[((b * Hq + h) * n_qt + qt) * buckets + bucket];
+  }
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) t += __shfl_xor(t, m, 64);
+  if (lane == 0) dtable[blockIdx.x] = (float)t;
 }
 
 }  // namespace
 
 size_t bwd_workspace_bytes(int B, int Hq, int S) { return (size_t)B * Hq * S * 2 * sizeof(float); }
+
+hipError_t launch_bias_grad(const float* part, float* dtable, int B, int Hq, int n_qt, int buckets,
+                            hipStream_t stream) {
+  const long long grid = (long long)Hq * buckets;
+  if (grid > 0x7fffffffLL / 64) return hipErrorInvalidValue;
+  if (grid == 0) return hipSuccess;
+  hipLaunchKernelGGL(bias_grad_kernel, dim3((unsigned)grid), dim3(64), 0, stream, part, dtable, B, Hq, n_qt, buckets);
+  return hipGetLastError();
+}
 
 hipError_t launch_flash_bwd(int dtype, const void* q, const void* k, const void* v,
                             const void* o, const void* dout, const float* lse, void* dq, void* dk,
@@ -796,12 +966,14 @@ hipError_t launch_flash_bwd(int dtype, const void* q, const void* k, const void*
                                 (const float*)dout, lse, (float*)dq, (float*)dk, (float*)dv, B,
                                 Hq, Hkv, S, D, scale, causal, ws, stream);
   float* w = (float*)ws;
+  BwdX<SelfX> bx;
+  bx.Skv = S;
 #define CA_BWD_CASE(TR, DD)                                                                   \
   if (D == DD)                                                                                \
     return causal ? launch_bwd_t<TR, DD, true>(q, k, v, o, dout, lse, dq, dk, dv, B, Hq, Hkv, \
-                                               S, scale, w, stream)                           \
+                                               S, scale, w, bx, stream)                       \
                   : launch_bwd_t<TR, DD, false>(q, k, v, o, dout, lse, dq, dk, dv, B, Hq,     \
-                                                Hkv, S, scale, w, stream);
+                                                Hkv, S, scale, w, bx, stream);
   if (dtype == kDtypeBF16) {
     CA_BWD_CASE(BF16, 64)
     CA_BWD_CASE(BF16, 128)
@@ -809,6 +981,59 @@ hipError_t launch_flash_bwd(int dtype, const void* q, const void* k, const void*
     CA_BWD_CASE(F16, 64)
     CA_BWD_CASE(F16, 128)
   }
+#undef CA_BWD_CASE
+  return hipErrorInvalidValue;
+}
+
+// The row pairs, then (buckets > 0) a total per bucket and tile of 128 queries.
+size_t cross_bwd_workspace_bytes(const EncDecShape& s, int buckets) {
+  const size_t rows = (size_t)s.B * s.Hq * s.Sq;
+  const size_t tiles = (size_t)s.B * s.Hq * ((s.Sq + 127) / 128);
+  return (2 * rows + tiles * buckets) * sizeof(float);
+}
+
+hipError_t launch_cross_bwd(int dtype, const void* q, const void* k, const void* v, const void* o, const void* dout,
+                            const float* lse, void* dq, void* dk, void* dv, float* dtable, const EncDecShape& s,
+                            const BiasSpec* bias, bool causal, void* ws, hipStream_t stream) {
+  float* w = (float*)ws;
+  if (dtype == kDtypeF32)
+    return launch_cross_bwd_f32((const float*)q, (const float*)k, (const float*)v, (const float*)o,
+                                (const float*)dout, lse, (float*)dq, (float*)dk, (float*)dv, dtable, s, bias, causal,
+                                w, stream);
+#define CA_BWD_CASE(TR, DD, CAUSAL)                                                                            \
+  return launch_bwd_t<TR, DD, CAUSAL>(q, k, v, o, dout, lse, dq, dk, dv, s.B, s.Hq, s.Hkv, s.Sq, s.scale, w, bx, \
+                                      stream);
+#define CA_BWD_TYPES(CASE)                  \
+  if (dtype == kDtypeBF16) {                \
+    if (s.D == 64) { CASE(BF16, 64) }       \
+    if (s.D == 128) { CASE(BF16, 128) }     \
+  } else if (dtype == kDtypeF16) {          \
+    if (s.D == 64) { CASE(F16, 64) }        \
+    if (s.D == 128) { CASE(F16, 128) }      \
+  }
+  if (!bias) {
+    BwdX<CrossX> bx;
+    bx.x.kv_lens = s.kv_lens;
+    bx.x.Skv = bx.Skv = s.Skv;
+#define CA_CASE(TR, DD) CA_BWD_CASE(TR, DD, false)
+    CA_BWD_TYPES(CA_CASE)
+#undef CA_CASE
+    return hipErrorInvalidValue;
+  }
+  const float eff = bias_scale(s.scale);
+  BwdX<BiasX> bx;
+  bx.x = bias_x(s, *bias, eff, 1.f / eff);
+  bx.Skv = s.Skv;
+  bx.dkv_lds = bias_lds_bytes(bx.x.reach);
+  bx.dq_lds = bias_grad_lds_bytes(bx.x.reach, bias->buckets(), bwdma::kNW);
+  bx.part_table = w + 2 * (size_t)s.B * s.Hq * s.Sq;
+  bx.dtable = dtable;
+#define CA_CASE(TR, DD)                   \
+  if (causal) CA_BWD_CASE(TR, DD, true)   \
+  CA_BWD_CASE(TR, DD, false)
+  CA_BWD_TYPES(CA_CASE)
+#undef CA_CASE
+#undef CA_BWD_TYPES
 #undef CA_BWD_CASE
   return hipErrorInvalidValue;
 }

@@ -23,7 +23,12 @@
 //     S = Q K^T, dP = dO V^T, dV^T += dO^T P, dK^T += Q^T dS.
 // Rows are stored with stride D + 4 floats so the float4 row reads of a
 // 16-lane group fall on distinct 4-bank groups.
+//
+// With an X of their own (encdec.h) the same kernels are the backward of cross
+// attention and of attention with a relative position bias, which here is added
+// to the log2 logits; the dq kernel also sums dS by bucket.
 #include "common.h"
+#include "encdec.h"
 #include "launch.h"
 
 namespace ca {
@@ -36,8 +41,9 @@ __device__ __forceinline__ int krow32(int l32) {
   return 16 * ((l32 >> 2) & 1) + 4 * (l32 >> 3) + (l32 & 3);
 }
 
-// (LSE log2 e, rowsum(dO * O)) per query row; D / 4 lanes per row.
-template <int D>
+// (LSE log2 e, rowsum(dO * O)) per query row; D / 4 lanes per row. X: +inf for
+// the LSE of a row without a key, with which every P is 0.
+template <int D, class X>
 __global__ __launch_bounds__(256) void bwd_rowdot_f32_kernel(const float* __restrict__ O,
                                                              const float* __restrict__ dO,
                                                              const float* __restrict__ LSE,
@@ -56,7 +62,8 @@ __global__ __launch_bounds__(256) void bwd_rowdot_f32_kernel(const float* __rest
 #pragma unroll
   for (int m = L / 2; m >= 1; m >>= 1) acc += __shfl_xor(acc, m, 64);
   if (row < rows && c == 0) {
-    LD[2 * row] = LSE[row] * kLog2e;
+    const float l = LSE[row];
+    LD[2 * row] = X::kCross && l == kNegInf ? -kNegInf : l * kLog2e;
     LD[2 * row + 1] = acc;
   }
 }
@@ -110,12 +117,14 @@ __device__ __forceinline__ void store_rowT_f32(float* dst_row, const f32x16 (&ac
     }
 }
 
-// dQ: one workgroup = 128 queries of one (b, h).
-template <int D, bool CAUSAL>
+// dQ: one workgroup = 128 queries of one (b, h). With a bias, the sums of dS by
+// bucket go to part_table [b, h][tile][buckets].
+template <int D, bool CAUSAL, class X>
 __global__ __launch_bounds__(kF32Waves * 64) void bwd_dq_f32_kernel(
     const float* __restrict__ Q, const float* __restrict__ K, const float* __restrict__ V,
     const float* __restrict__ dO, const float* __restrict__ LD, float* __restrict__ dQ, int S,
-    int Hq, int Hkv, float scale, int n_qt, int n_work) {
+    int Hq, int Hkv, float scale, int n_qt, int n_work, X x, float* __restrict__ part_table) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char bias_mem[];
   constexpr int BM = 32 * kF32Waves;
   constexpr int HD = D / 2, NOB = D / 32;
   constexpr int KS = Stage2<D>::KS;
@@ -128,9 +137,14 @@ __global__ __launch_bounds__(kF32Waves * 64) void bwd_dq_f32_kernel(
   const int b = bh / Hq, h = bh % Hq;
   const int hk = h / (Hq / Hkv);
   const int q0 = qt * BM;
+  int Skv = S, n_keys = S;
+  if constexpr (X::kCross) {
+    Skv = x.Skv;
+    n_keys = x.kv_len(b);
+  }
   const size_t qoff = (size_t)(b * Hq + h) * S;
-  const float* Kp = K + (size_t)(b * Hkv + hk) * S * D;
-  const float* Vp = V + (size_t)(b * Hkv + hk) * S * D;
+  const float* Kp = K + (size_t)(b * Hkv + hk) * Skv * D;
+  const float* Vp = V + (size_t)(b * Hkv + hk) * Skv * D;
 
   const int tid = threadIdx.x;
   const int wave = tid >> 6, lane = tid & 63;
@@ -154,7 +168,24 @@ __global__ __launch_bounds__(kF32Waves * 64) void bwd_dq_f32_kernel(
     gv[k4] = y.x; gv[k4 + 1] = y.y; gv[k4 + 2] = y.z; gv[k4 + 3] = y.w;
   }
 
-  const int kv_end = CAUSAL ? min(S, q0 + BM) : S;
+  const float* be = nullptr;  // distance 0's bias, at the lane's query and its first key of a block
+  uint32_t id_ofs = 0;        // LDS: the bucket ids of a block's distances
+  BiasGrad grad;
+  float* totals = nullptr;    // [wave][buckets]
+  int n_buckets = 0;
+  if constexpr (X::kBias) {
+    unsigned char* ids = bias_mem + bias_lds_bytes(x.reach);
+    totals = (float*)(ids + bias_id_bytes(x.reach));
+    n_buckets = x.one_sided ? x.side : 2 * x.side;
+    unsigned char* scratch = (unsigned char*)totals + 4 * kF32Waves * n_buckets + wave * BiasGrad::kScratchB;
+    bias_fill(x, h, bias_mem, 64 * kF32Waves);
+    be = bias_zero(x, bias_mem) + 31 - l32 + 16 * hl;
+    id_ofs = bias_fill_ids(x, bias_mem, ids, 64 * kF32Waves) + min(lane, 62);
+    grad.init(lds_off(scratch), lds_off(totals + wave * n_buckets), n_buckets);
+    __syncthreads();
+  }
+
+  const int kv_end = CAUSAL ? min(n_keys, q0 + BM) : n_keys;
   const int n_tiles = (kv_end + kF32Tile - 1) / kF32Tile;
   Stage2<D> st;
   f32x16 acc[NOB];  // dQ^T
@@ -164,12 +195,12 @@ __global__ __launch_bounds__(kF32Waves * 64) void bwd_dq_f32_kernel(
     for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
   const int krow = krow32(l32);
 
-  if (n_tiles > 0) st.load(Kp, Vp, 0, S, tid);
+  if (n_tiles > 0) st.load(Kp, Vp, 0, n_keys, tid);
   for (int t = 0; t < n_tiles; ++t) {
     const int buf = t & 1;
     st.store(Ks[buf], Vs[buf], tid);
     __syncthreads();
-    if (t + 1 < n_tiles) st.load(Kp, Vp, (t + 1) * kF32Tile, S, tid);
+    if (t + 1 < n_tiles) st.load(Kp, Vp, (t + 1) * kF32Tile, n_keys, tid);
     const int k0 = t * kF32Tile;
     if (CAUSAL && k0 > qw0 + 31) continue;  // every key after every query of the wave
     // S^T = K Q^T, dP^T = V dO^T; register r of half hl <-> key k0 + 16 hl + r
@@ -191,14 +222,23 @@ __global__ __launch_bounds__(kF32Waves * 64) void bwd_dq_f32_kernel(
       s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, qv[k4 + 3], s, 0, 0, 0);
       dp = __builtin_amdgcn_mfma_f32_32x32x2f32(c.w, gv[k4 + 3], dp, 0, 0, 0);
     }
-    const bool need_mask = CAUSAL ? (k0 + kF32Tile - 1 > qw0) : (k0 + kF32Tile > S);
+    const bool need_mask =
+        CAUSAL ? (k0 + kF32Tile - 1 > qw0 || (X::kCross && k0 + kF32Tile > n_keys)) : (k0 + kF32Tile > n_keys);
     float ds[16];  // dS^T / scale
+    const float* bb = be;
+    int r0 = 0;
+    if constexpr (X::kBias) {
+      r0 = bias_block(x, k0 - qw0 - 31);
+      bb += r0;
+    }
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      float p = fast_exp2(__builtin_fmaf(s[r], c2, -lse2));
+      float e = __builtin_fmaf(s[r], c2, -lse2);
+      if constexpr (X::kBias) e += bb[r];
+      float p = fast_exp2(e);
       if (need_mask) {
         const int key = k0 + 16 * hl + r;
-        if (key >= S || (CAUSAL && key > myq)) p = 0.f;
+        if (key >= n_keys || (CAUSAL && key > myq)) p = 0.f;
       }
       ds[r] = p * (dp[r] - dd);
     }
@@ -210,17 +250,35 @@ __global__ __launch_bounds__(kF32Waves * 64) void bwd_dq_f32_kernel(
       for (int r = 0; r < 16; ++r)
         acc[ob] = __builtin_amdgcn_mfma_f32_32x32x2f32(kt[r * KS], ds[r], acc[ob], 0, 0, 0);
     }
+    if constexpr (X::kBias) {
+      uint32_t id = lds_read_u8<0>(id_ofs + (uint32_t)r0);
+      wait_lgkm<0>();
+      after_wait(id);
+      grad.template block<16>(ds, (int)id);
+    }
+  }
+  if constexpr (X::kBias) {
+    grad.flush();
+    wait_lgkm<0>();
+    __syncthreads();
+    for (int i = tid; i < n_buckets; i += 64 * kF32Waves) {
+      float t = 0.f;
+#pragma unroll
+      for (int w = 0; w < kF32Waves; ++w) t += totals[w * n_buckets + i];
+      part_table[((size_t)bh * n_qt + qt) * n_buckets + i] = t;
+    }
   }
   if (qvalid) store_rowT_f32<NOB>(dQ + (qoff + myq) * D, acc, hl, scale);
 }
 
 // dK, dV: one workgroup = 128 keys of one (b, kv head); 32-query tiles of
 // every q head of the kv head.
-template <int D, bool CAUSAL>
+template <int D, bool CAUSAL, class X>
 __global__ __launch_bounds__(kF32Waves * 64) void bwd_dkv_f32_kernel(
     const float* __restrict__ Q, const float* __restrict__ K, const float* __restrict__ V,
     const float* __restrict__ dO, const float* __restrict__ LD, float* __restrict__ dK,
-    float* __restrict__ dV, int S, int Hq, int Hkv, float scale, int n_kt, int n_work) {
+    float* __restrict__ dV, int S, int Hq, int Hkv, float scale, int n_kt, int n_work, X x) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char bias_mem[];
   constexpr int BK = 32 * kF32Waves;
   constexpr int HD = D / 2, NOB = D / 32;
   constexpr int KS = Stage2<D>::KS;
@@ -234,14 +292,19 @@ __global__ __launch_bounds__(kF32Waves * 64) void bwd_dkv_f32_kernel(
   const int b = bhk / Hkv, hk = bhk % Hkv;
   const int G = Hq / Hkv;
   const int K0 = kt * BK;
-  const size_t kvoff = (size_t)(b * Hkv + hk) * S;
+  int Skv = S, n_keys = S;
+  if constexpr (X::kCross) {
+    Skv = x.Skv;
+    n_keys = x.kv_len(b);
+  }
+  const size_t kvoff = (size_t)(b * Hkv + hk) * Skv;
 
   const int tid = threadIdx.x;
   const int wave = tid >> 6, lane = tid & 63;
   const int l32 = lane & 31, hl = lane >> 5;
   const int kw0 = K0 + 32 * wave;
   const int mykey = kw0 + l32;
-  const bool kvalid = mykey < S;
+  const bool kvalid = mykey < n_keys;
   const float c2 = scale * kLog2e;
 
   float kv[HD], vv[HD];  // K^T and V^T as B operands: element HD * hl + k of this lane's key
@@ -257,7 +320,9 @@ __global__ __launch_bounds__(kF32Waves * 64) void bwd_dkv_f32_kernel(
   }
 
   const int t_begin = CAUSAL ? K0 / kF32Tile : 0;
-  const int nt = max(0, (S + kF32Tile - 1) / kF32Tile - t_begin);
+  int nt = max(0, (S + kF32Tile - 1) / kF32Tile - t_begin);
+  if constexpr (X::kCross)
+    if (K0 >= n_keys) nt = 0;
   const int n_it = G * nt;
   Stage2<D> st;
   float lreg = 0.f;
@@ -282,6 +347,12 @@ __global__ __launch_bounds__(kF32Waves * 64) void bwd_dkv_f32_kernel(
   if (n_it > 0) gload(0);
   for (int it = 0; it < n_it; ++it) {
     const int buf = it & 1;
+    if constexpr (X::kBias) {
+      if (it % nt == 0) {
+        __syncthreads();  // every wave has read the last q head's bias
+        bias_fill(x, hk * G + it / nt, bias_mem, 64 * kF32Waves);
+      }
+    }
     st.store(Qs[buf], Gs[buf], tid);
     if (tid < 2 * kF32Tile) Ls[buf][tid] = lreg;
     __syncthreads();
@@ -309,10 +380,15 @@ __global__ __launch_bounds__(kF32Waves * 64) void bwd_dkv_f32_kernel(
     }
     const bool need_mask = !kvalid || (CAUSAL && q0 < kw0 + 31) || q0 + kF32Tile > S;
     float p[16], ds[16];
+    // register r: distance kw0 + l32 - (q0 + 16 hl + r)
+    const float* bb = nullptr;
+    if constexpr (X::kBias) bb = bias_zero(x, bias_mem) + bias_block(x, kw0 - q0 - 31) + 31 + l32 - 16 * hl;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int qi = 16 * hl + r;
-      p[r] = fast_exp2(__builtin_fmaf(s[r], c2, -Ls[buf][2 * qi]));
+      float e = __builtin_fmaf(s[r], c2, -Ls[buf][2 * qi]);
+      if constexpr (X::kBias) e += bb[-r];
+      p[r] = fast_exp2(e);
       if (need_mask) {
         const int query = q0 + qi;
         if (!kvalid || query >= S || (CAUSAL && mykey > query)) p[r] = 0.f;
@@ -332,34 +408,51 @@ __global__ __launch_bounds__(kF32Waves * 64) void bwd_dkv_f32_kernel(
       }
     }
   }
-  if (kvalid) {
+  if constexpr (X::kCross) {
+    if (!kvalid) {  // a padded key: 0
+#pragma unroll
+      for (int i = 0; i < NOB; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) { dk[i][r] = 0.f; dv[i][r] = 0.f; }
+    }
+  }
+  if (mykey < Skv) {
     store_rowT_f32<NOB>(dK + (kvoff + mykey) * D, dk, hl, scale);
     store_rowT_f32<NOB>(dV + (kvoff + mykey) * D, dv, hl, 1.f);
   }
 }
 
-template <int D, bool CAUSAL>
+template <int D, bool CAUSAL, class X>
 hipError_t launch_bwd_f32_t(const float* q, const float* k, const float* v, const float* o,
                             const float* dout, const float* lse, float* dq, float* dk, float* dv,
-                            int B, int Hq, int Hkv, int S, float scale, float* ws,
-                            hipStream_t stream) {
+                            int B, int Hq, int Hkv, int S, int Skv, float scale, float* ws, const X& x,
+                            size_t dkv_lds, size_t dq_lds, float* part_table, hipStream_t stream) {
   const long long rows = (long long)B * Hq * S;
   const long long g0 = (rows * (D / 4) + 255) / 256;
-  const int n_t = (S + 32 * kF32Waves - 1) / (32 * kF32Waves);
-  const long long gq = (long long)B * Hq * n_t;
-  const long long gk = (long long)B * Hkv * n_t;
+  const int n_qt = (S + 32 * kF32Waves - 1) / (32 * kF32Waves);
+  const int n_kt = (Skv + 32 * kF32Waves - 1) / (32 * kF32Waves);
+  const long long gq = (long long)B * Hq * n_qt;
+  const long long gk = (long long)B * Hkv * n_kt;
   if (g0 > 0x7fffffffLL || gq > 0x7fffffffLL || gk > 0x7fffffffLL) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((bwd_rowdot_f32_kernel<D>), dim3((unsigned)g0), dim3(256), 0, stream, o, dout,
-                     lse, ws, rows);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((bwd_dkv_f32_kernel<D, CAUSAL>), dim3((unsigned)gk), dim3(kF32Waves * 64), 0,
-                     stream, q, k, v, dout, ws, dk, dv, S, Hq, Hkv, scale, n_t, (int)gk);
-  e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((bwd_dq_f32_kernel<D, CAUSAL>), dim3((unsigned)gq), dim3(kF32Waves * 64), 0,
-                     stream, q, k, v, dout, ws, dq, S, Hq, Hkv, scale, n_t, (int)gq);
-  return hipGetLastError();
+  hipError_t e = hipSuccess;
+  if (g0 > 0) {
+    hipLaunchKernelGGL((bwd_rowdot_f32_kernel<D, X>), dim3((unsigned)g0), dim3(256), 0, stream, o, dout,
+                       lse, ws, rows);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  if (gk > 0) {
+    hipLaunchKernelGGL((bwd_dkv_f32_kernel<D, CAUSAL, X>), dim3((unsigned)gk), dim3(kF32Waves * 64), dkv_lds,
+                       stream, q, k, v, dout, ws, dk, dv, S, Hq, Hkv, scale, n_kt, (int)gk, x);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  if (gq > 0) {
+    hipLaunchKernelGGL((bwd_dq_f32_kernel<D, CAUSAL, X>), dim3((unsigned)gq), dim3(kF32Waves * 64), dq_lds,
+                       stream, q, k, v, dout, ws, dq, S, Hq, Hkv, scale, n_qt, (int)gq, x, part_table);
+    e = hipGetLastError();
+  }
+  return e;
 }
 
 }  // namespace
@@ -370,16 +463,42 @@ hipError_t launch_flash_bwd_f32(const float* q, const float* k, const float* v, 
                                 bool causal, void* ws, hipStream_t stream) {
   if ((long long)B * Hq * S == 0) return hipSuccess;
   float* w = (float*)ws;
-#define CA_BWD32(DD)                                                                          \
-  if (D == DD)                                                                                \
-    return causal ? launch_bwd_f32_t<DD, true>(q, k, v, o, dout, lse, dq, dk, dv, B, Hq, Hkv, \
-                                               S, scale, w, stream)                           \
-                  : launch_bwd_f32_t<DD, false>(q, k, v, o, dout, lse, dq, dk, dv, B, Hq,     \
-                                                Hkv, S, scale, w, stream);
-  CA_BWD32(64)
-  CA_BWD32(128)
+  const SelfX x;
+#define CA_BWD32(DD, CAUSAL)                                                                                      \
+  launch_bwd_f32_t<DD, CAUSAL>(q, k, v, o, dout, lse, dq, dk, dv, B, Hq, Hkv, S, S, scale, w, x, 0, 0, nullptr, \
+                               stream)
+  if (D == 64) return causal ? CA_BWD32(64, true) : CA_BWD32(64, false);
+  if (D == 128) return causal ? CA_BWD32(128, true) : CA_BWD32(128, false);
 #undef CA_BWD32
   return hipErrorInvalidValue;
+}
+
+hipError_t launch_cross_bwd_f32(const float* q, const float* k, const float* v, const float* o, const float* dout,
+                                const float* lse, float* dq, float* dk, float* dv, float* dtable,
+                                const EncDecShape& s, const BiasSpec* bias, bool causal, float* ws,
+                                hipStream_t stream) {
+#define CA_BWD32(DD, CAUSAL, X, DKV, DQ, PART)                                                               \
+  launch_bwd_f32_t<DD, CAUSAL>(q, k, v, o, dout, lse, dq, dk, dv, s.B, s.Hq, s.Hkv, s.Sq, s.Skv, s.scale, ws, \
+                               X, DKV, DQ, PART, stream)
+  if (!bias) {
+    CrossX x;
+    x.kv_lens = s.kv_lens;
+    x.Skv = s.Skv;
+    if (s.D == 64) return CA_BWD32(64, false, x, 0, 0, nullptr);
+    if (s.D == 128) return CA_BWD32(128, false, x, 0, 0, nullptr);
+    return hipErrorInvalidValue;
+  }
+  const BiasX x = bias_x(s, *bias, s.scale, kLog2e);
+  const size_t dkv = bias_lds_bytes(x.reach);
+  const size_t dqb = bias_grad_lds_bytes(x.reach, bias->buckets(), kF32Waves) + kF32Waves * BiasGrad::kScratchB;
+  float* part = ws + 2 * (size_t)s.B * s.Hq * s.Sq;
+  hipError_t e = hipErrorInvalidValue;
+  if (s.D == 64) e = causal ? CA_BWD32(64, true, x, dkv, dqb, part) : CA_BWD32(64, false, x, dkv, dqb, part);
+  if (s.D == 128) e = causal ? CA_BWD32(128, true, x, dkv, dqb, part) : CA_BWD32(128, false, x, dkv, dqb, part);
+#undef CA_BWD32
+  if (e != hipSuccess) return e;
+  return launch_bias_grad(part, dtable, s.B, s.Hq, (s.Sq + 32 * kF32Waves - 1) / (32 * kF32Waves), bias->buckets(),
+                          stream);
 }
 
 }  // namespace ca

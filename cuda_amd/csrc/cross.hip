@@ -1,0 +1,535 @@
+// Attention of encoder-decoder models, forward, 16-bit: cross attention (keys of
+// another length, padded per sequence) and self-attention with a learned
+// relative position bias (encdec.h).
+//
+// Computes O = softmax(Q K^T * scale [+ bias(key - query)] [+ causal mask]) V
+// over the first kv_len keys of each sequence, and the natural-log LSE; a row
+// with no key gives 0 and -inf. Math, tiles and register layouts are those of
+// prefill_rows.hip: a workgroup takes 32 QG query rows, QG row groups of KS =
+// 8 / QG waves ("parts"), each part walking every KS-th key tile with an online
+// softmax of its own; the parts meet in LDS. S^T = K Q^T with the rho row
+// permutation, whose accumulators are the B operand of O^T += V^T P^T.
+//
+// Cross attention has no position, and the query rows of the G heads of a kv
+// head lie one after the other, so a tile's rows run over all of them: G Sq
+// rows of a kv head make as few tiles as they can.
+//
+// The bias enters as the accumulators' start: S^T begins as bias / scale, so it
+// costs LDS reads (two dwords a lane for two logits) and no VALU work.
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "common.h"
+#include "encdec.h"
+#include "launch.h"
+#include "lds_dma.h"
+#include "prefill_common.h"
+
+namespace ca {
+namespace {
+
+constexpr int kWaves = 8;
+
+struct CrossArgs {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  uint16_t* o;
+  float* lse;
+  float* part_o;    // [rows of all groups][n_split][D], o / l, where n_split > 1
+  float* part_lse;  // ... log2 of the sum of 2^x
+  int rows;         // query rows of a group (a head, or a kv head's heads)
+  int per_b;        // groups per sequence
+  int ratio;        // groups per kv head
+  float scale_log2; // |scale| log2 e
+  uint32_t q_sign;  // flips q's signs for a negative scale
+  int n_qt, n_bh, n_work, order, n_split;
+};
+
+// Split `split` of the key walk of query tile qt of group bh.
+template <typename Tr, int D, class X, bool CAUSAL, int QG>
+__device__ CA_INLINE void cross_tile(const CrossArgs& a, const X& x, unsigned char* bias_mem, int bh, int qt,
+                                     int split) {
+  using Gm = PfGeom<D>;
+  using vec8 = typename Tr::vec8;
+  using vec4 = typename Tr::vec4;
+  using vec2 = typename Tr::vec2;
+  constexpr bool BIAS = X::kBias;
+  constexpr int kNW = kWaves, KS = kNW / QG;
+  // 64 keys per tile; 32 where four 64-key tiles would fill the ring
+  constexpr int kBN = D == 128 && KS == 4 ? 32 : 64;
+  constexpr int kMB = kBN / 32;                  // 32-key blocks per tile
+  constexpr int kKK = kBN / 16;                  // PV k-steps per tile
+  constexpr int kRowB = Gm::kRowB, kNKS = Gm::kNKS, kNOB = Gm::kNOB;
+  constexpr int kTileB = kBN * kRowB;            // K (or V) tile
+  constexpr int kGroupB = KS * 2 * kTileB;       // one K and one V tile per part
+  constexpr int kGroups = 128 * 1024 / kGroupB;  // ring, groups
+  static_assert(kGroups >= 2, "a group loads while another is read");
+  constexpr int kT = kTileB / 1024;              // 1-KB loads per tile
+  constexpr int kLoads = KS * 2 * kT / kNW;      // loads per wave per group
+  static_assert(kT % kNW == 0, "a tile's loads are dealt to all waves");
+  constexpr int NR = 16 * kNOB / KS;             // O^T registers a part combines
+  constexpr int kMeetB = QG * KS * (KS - 1) * NR * 256;  // the others' registers
+  constexpr int kRowsB = QG * 32 * kRowB;        // output rows, packed
+  static_assert(kMeetB + kRowsB <= kGroups * kGroupB, "the meeting fits the ring");
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[kGroups * kGroupB];
+  __shared__ float red_m[QG][KS][32], red_l[QG][KS][32];
+
+  const int rows = a.rows;
+  const int lane = lane_here();  // (not hoisted out of the pair's loop: registers)
+  const int wave = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_workitem_id_x() >> 6);
+  const int qg = wave % QG, part = wave / QG;
+  const int l32 = lane & 31, hl = lane >> 5;
+  const int q0 = qt * 32 * QG, qw0 = q0 + 32 * qg, myq = qw0 + l32;
+  const bool q_in = myq < rows;
+  const int b = bh / a.per_b, g_in_b = bh % a.per_b;
+  const size_t khead = ((size_t)b * (a.per_b / a.ratio) + g_in_b / a.ratio) * x.Skv;
+  const uint16_t* Kp = a.k + khead * D;
+  const uint16_t* Vp = a.v + khead * D;
+  const int n_keys = x.kv_len(b);
+
+  const int kv_end = CAUSAL ? min(n_keys, q0 + 32 * QG) : n_keys;
+  const int n_all = (kv_end + kBN - 1) / kBN;
+  // this split's tiles [t0, t0 + n_tiles)
+  const int t0 = (int)((long long)n_all * split / a.n_split);
+  const int n_tiles = (int)((long long)n_all * (split + 1) / a.n_split) - t0;
+  const int n_groups = (n_tiles + KS - 1) / KS;
+  // tiles this row group computes; the last of the whole walk holds the
+  // diagonal or the end
+  const int w_end = CAUSAL ? min(kv_end, qw0 + 32) : kv_end;
+  const int w_last = (w_end + kBN - 1) / kBN - 1 - t0;
+  const int w_tiles = qw0 < rows ? min(w_last + 1, n_tiles) : 0;
+
+  // load j of this wave: 1 KB of tile `sub` of the group, K or V, rows from
+  // kRpk * piece (rows past kv_end read as zero)
+  uint32_t off0;
+  {
+    const int row = Gm::kRpk * wave + lane / Gm::kLpr;
+    off0 = row * kRowB + 16 * ((lane % Gm::kLpr) ^ Gm::swz(row));
+  }
+  auto issue = [&](int g) CA_INLINE {
+    unsigned char* st = lds + (g % kGroups) * kGroupB;
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      constexpr int kPer = kT / kNW;  // loads of a wave per tile
+      const int sub = j / (2 * kPer), is_v = (j / kPer) % 2, p = j % kPer;
+      const uint32_t t = (uint32_t)(t0 + g * KS + sub);
+      dma16_buf(make_rsrc_at(is_v ? Vp : Kp, t * kTileB, (uint32_t)kv_end * kRowB),
+                (CA_LDS void*)(st + (2 * sub + is_v) * kTileB + 1024 * (kNW * p + wave)),
+                off0 + 1024u * kNW * p);  // swz repeats every 16 rows
+    }
+  };
+#pragma unroll
+  for (int g = 0; g < kGroups - 1; ++g) issue(g);
+
+  // Q as the B operand of S^T = K Q^T: k-step ks holds d = 16 ks + 8 hl + [0, 8).
+  // Lanes past the rows take the last one.
+  vec8 qv[kNKS];
+  {
+    const uint16_t* Qr = a.q + ((size_t)bh * rows + min(myq, rows - 1)) * D;
+#pragma unroll
+    for (int ks = 0; ks < kNKS; ++ks) {
+      u32x4 w = *(const u32x4*)(Qr + 16 * ks + 8 * hl);
+      w ^= a.q_sign;
+      qv[ks] = __builtin_bit_cast(vec8, w);
+    }
+  }
+
+  // LDS read offsets (prefill.hip): K row rho(l32), chunk hl (^ 32 ks bytes);
+  // V^T source rows tr_row and tr_row + 4, chunks c0 (^ 64 ob bytes)
+  const int krow = (l32 & 0x13) | ((l32 & 4) << 1) | ((l32 & 8) >> 1);
+  const uint32_t kofs = krow * kRowB + 16 * (hl ^ Gm::swz(krow));
+  const int g16 = lane >> 4, s16 = lane & 15;
+  const int tr_row = 8 * (g16 >> 1) + (s16 >> 2), c0 = 2 * (g16 & 1) + ((s16 & 3) >> 1);
+  const uint32_t vofs1 = kTileB + tr_row * kRowB + 16 * (c0 ^ Gm::swz(tr_row)) + 8 * (s16 & 1);
+  const uint32_t vofs2 =
+      kTileB + (tr_row + 4) * kRowB + 16 * (c0 ^ Gm::swz(tr_row + 4)) + 8 * (s16 & 1);
+  const uint32_t lds0 = lds_off(lds);
+  // the bias of the lane's query and its first key of a block that starts at
+  // distance r0: register i is 4 (31 - l32 + 8 hl + off(i)) bytes past entry r0
+  uint32_t bofs = 0;
+  if constexpr (BIAS) bofs = bias_fill(x, g_in_b, bias_mem, 64 * kNW) + 4 * (31 - l32 + 8 * hl);
+
+  f32x16 o[kNOB];
+#pragma unroll
+  for (int i = 0; i < kNOB; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
+  float m_run = kNegInf, l_run = 0.f;
+  constexpr float kStaleMax = std::is_same<Tr, BF16>::value ? 0x1p48f : 0x1p15f;
+
+  // One key tile at LDS byte `st`, keys from k0. FIRST: the part's first tile,
+  // which takes the row max before its exponentials; later ones take theirs
+  // against the running max as it stands, and again with their own only when a
+  // lane's sum passes what P's type and O hold (stale_softmax in prefill.hip), or
+  // a row has met no finite logit yet (a bias of -inf).
+  // MASK: the row group's last tile (diagonal, end of the keys).
+  auto tile = [&](uint32_t st, int k0, auto first_tag, auto mask_tag) CA_INLINE {
+    constexpr bool FIRST = decltype(first_tag)::value, MASK = decltype(mask_tag)::value;
+    // bias reads: pair i of the lane's kBN / 4 (logits 2 i, 2 i + 1)
+    constexpr int NB2 = BIAS ? 8 * kMB : 1;
+    u32x2 br[NB2];
+    if constexpr (BIAS) {
+      const uint32_t ba = bofs + 4 * (uint32_t)bias_block(x, k0 - qw0 - 31);
+      auto bread = [&](auto i) CA_INLINE {
+        constexpr int p = 2 * decltype(i)::value;
+        constexpr int off = 32 * (p >> 4) + 16 * ((p >> 3) & 1) + (p & 7);
+        br[decltype(i)::value] = lds_read2_b32<off, off + 1>(ba);
+      };
+      for_const<NB2>(bread);
+    }
+    const uint32_t ka = st + kofs;
+    u32x4 kr[kNKS][kMB];
+    auto kread = [&](int ks) CA_INLINE {
+      kr[ks][0] = lds_read_b128<0>(ka ^ (32 * ks));
+      if constexpr (kMB == 2) kr[ks][kMB - 1] = lds_read_b128<32 * kRowB>(ka ^ (32 * ks));
+    };
+    constexpr int KD = 2;  // k-steps read ahead
+#pragma unroll
+    for (int ks = 0; ks < KD; ++ks) kread(ks);
+    f32x16 s[kMB];
+    if constexpr (BIAS) {
+      wait_lgkm<kMB * KD>();
+#pragma unroll
+      for (int i = 0; i < NB2; ++i) {
+        after_wait(br[i]);
+        const uint32_t lo = br[i][0], hi = br[i][1];
+        s[i >> 3][(2 * i) & 15] = __builtin_bit_cast(float, lo);
+        s[i >> 3][(2 * i + 1) & 15] = __builtin_bit_cast(float, hi);
+      }
+    } else {
+#pragma unroll
+      for (int mb = 0; mb < kMB; ++mb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[mb][r] = 0.f;
+    }
+#pragma unroll
+    for (int ks = 0; ks < kNKS; ++ks) {
+      if (ks + KD < kNKS) kread(ks + KD);
+      wait_lgkm_n(kMB * (KD < kNKS - 1 - ks ? KD : kNKS - 1 - ks));
+#pragma unroll
+      for (int mb = 0; mb < kMB; ++mb) {
+        after_wait(kr[ks][mb]);
+        s[mb] = Tr::mfma32(__builtin_bit_cast(vec8, kr[ks][mb]), qv[ks], s[mb]);
+      }
+    }
+    // the first V^T fragments land under the softmax
+    constexpr int NST = kNOB * kKK, VD = 2;  // PV steps: O^T block st / kKK, k-step st % kKK
+    u32x2 vr[NST][2];
+    auto vread = [&](auto i) CA_INLINE {
+      constexpr int st_ = decltype(i)::value, ob = st_ / kKK, kk = st_ % kKK;
+      vr[st_][0] = lds_read_tr16<16 * kRowB * kk>((st + vofs1) ^ (64 * ob));
+      vr[st_][1] = lds_read_tr16<16 * kRowB * kk>((st + vofs2) ^ (64 * ob));
+    };
+    for_const<VD>(vread);
+
+    // a masked tile scales its logits before the mask, so that a masked one's
+    // weight is 0 for scale 0 too
+    vec8 pb[kKK];
+    float sv[16 * kMB];
+    // register i is key k0 + 8 hl + off
+    const int last = (CAUSAL ? min(n_keys - 1, myq) : n_keys - 1) - k0 - 8 * hl;
+#pragma unroll
+    for (int i = 0; i < 16 * kMB; ++i) {
+      sv[i] = s[i >> 4][i & 15];
+      if (MASK) {
+        const int off = 32 * (i >> 4) + 16 * ((i >> 3) & 1) + (i & 7);
+        sv[i] = off > last ? kNegInf : sv[i] * a.scale_log2;
+      }
+    }
+    auto settle_max = [&]() CA_INLINE {
+      float t0_ = kNegInf, t1_ = kNegInf;
+#pragma unroll
+      for (int i = 0; i < 16 * kMB; i += 4) {
+        t0_ = max3(t0_, sv[i], sv[i + 1]);
+        t1_ = max3(t1_, sv[i + 2], sv[i + 3]);
+      }
+      const float t2 = __builtin_fmaxf(t0_, t1_);
+      const float m_new = __builtin_fmaxf(m_run, pair32_max(MASK ? t2 : t2 * a.scale_log2));
+      if (!FIRST) {
+        const float alpha = m_new == kNegInf ? 1.f : fast_exp2(m_run - m_new);
+#pragma unroll
+        for (int i = 0; i < kNOB; ++i) o[i] *= alpha;
+        l_run *= alpha;
+      }
+      m_run = m_new;
+    };
+    float sum[2];
+    auto exp_all = [&]() CA_INLINE {
+      const float msub = m_run == kNegInf ? 0.f : m_run;
+#pragma unroll
+      for (int i = 0; i < 16 * kMB; i += 2) {
+        const float p0 = fast_exp2(MASK ? sv[i] - msub : __builtin_fmaf(sv[i], a.scale_log2, -msub));
+        const float p1 = fast_exp2(MASK ? sv[i + 1] - msub : __builtin_fmaf(sv[i + 1], a.scale_log2, -msub));
+        const vec2 pk = Tr::pack2(p0, p1);
+        pb[i / 8][i % 8] = pk[0];
+        pb[i / 8][i % 8 + 1] = pk[1];
+        sum[(i / 2) & 1] = i < 4 ? p0 + p1 : sum[(i / 2) & 1] + (p0 + p1);
+      }
+    };
+    if (FIRST) settle_max();
+    exp_all();
+    if (!FIRST &&
+        __builtin_expect(wave_any(!(sum[0] + sum[1] <= kStaleMax) || (BIAS && m_run == kNegInf)), 0)) {
+      settle_max();
+      exp_all();
+    }
+    l_run += sum[0] + sum[1];
+
+    // O^T += V^T P^T
+    auto step = [&](auto i) CA_INLINE {
+      constexpr int st_ = decltype(i)::value;
+      if constexpr (st_ + VD < NST) vread(std::integral_constant<int, st_ + VD>{});
+      wait_lgkm<2 * (VD < NST - 1 - st_ ? VD : NST - 1 - st_)>();
+      after_wait(vr[st_][0]);
+      after_wait(vr[st_][1]);
+      const u32x4 w = {vr[st_][0][0], vr[st_][0][1], vr[st_][1][0], vr[st_][1][1]};
+      o[st_ / kKK] = Tr::mfma32(__builtin_bit_cast(vec8, w), pb[st_ % kKK], o[st_ / kKK]);
+    };
+    for_const<NST>(step);
+  };
+
+  // one iteration per group: the part's tile of group g is t0 + g KS + part
+  auto sync = [&](int g) CA_INLINE {
+    wait_vmcnt<kLoads * (kGroups - 2)>();  // this wave's loads of group g landed
+    __builtin_amdgcn_s_barrier();          // ... and every wave's; group g - 1 is read
+    issue(g + kGroups - 1);
+    return lds0 + (uint32_t)((g % kGroups) * kGroupB + part * 2 * kTileB);
+  };
+  using T_ = std::true_type;
+  using F_ = std::false_type;
+  int g = 0;
+  const int w_full = min(w_tiles, w_last);  // tiles before the masked one
+  if (part < w_full) {
+    tile(sync(0), (t0 + part) * kBN, T_{}, F_{});
+#pragma clang loop unroll(disable)
+    for (g = 1; g * KS + part < w_full; ++g) tile(sync(g), (t0 + g * KS + part) * kBN, F_{}, F_{});
+  }
+  if (w_full < w_tiles && g * KS + part == w_full) {
+    const uint32_t st = sync(g);
+    if (g == 0) tile(st, (t0 + g * KS + part) * kBN, T_{}, T_{});
+    else tile(st, (t0 + g * KS + part) * kBN, F_{}, T_{});
+    ++g;
+  }
+  for (; g < n_groups; ++g) sync(g);
+  wait_vmcnt<0>();
+  const float l_part = pair32_sum(l_run);
+  if (hl == 0) {
+    red_m[qg][part][l32] = m_run;
+    red_l[qg][part][l32] = l_part;
+  }
+  __syncthreads();  // the ring is read: the parts' registers and the rows go there
+  // Register r of 16 kNOB goes to part r / NR. Block (qg, dst, j), j counting
+  // the other parts: [NR / 4][64 lanes] x 4 floats.
+  auto block = [&](int dst, int j) CA_INLINE {
+    return (f32x4*)lds + ((qg * KS + dst) * (KS - 1) + j) * (NR * 16) + lane;
+  };
+  f32x4 own[NR / 4];
+#pragma unroll
+  for (int dst = 0; dst < KS; ++dst) {
+    f32x4 y[NR / 4];
+#pragma unroll
+    for (int j = 0; j < NR / 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = dst * NR + 4 * j + e;
+        y[j][e] = o[i / 16][i % 16];
+      }
+    if (KS == 1 || dst == part) {
+#pragma unroll
+      for (int j = 0; j < NR / 4; ++j) own[j] = y[j];
+    } else {
+      f32x4* blk = block(dst, part < dst ? part : part - 1);
+#pragma unroll
+      for (int j = 0; j < NR / 4; ++j) blk[64 * j] = y[j];
+    }
+  }
+  if constexpr (KS > 1) __syncthreads();
+  float M = kNegInf, L = 0.f;
+#pragma unroll
+  for (int s = 0; s < KS; ++s) M = __builtin_fmaxf(M, red_m[qg][s][l32]);
+  auto weight = [&](int s) CA_INLINE { return M == kNegInf ? 0.f : fast_exp2(red_m[qg][s][l32] - M); };
+#pragma unroll
+  for (int s = 0; s < KS; ++s) L += weight(s) * red_l[qg][s][l32];
+  const float inv = L > 0.f ? 1.f / L : 0.f;
+  const float w_own = weight(part);
+#pragma unroll
+  for (int j = 0; j < NR / 4; ++j) own[j] *= w_own;
+#pragma unroll
+  for (int p = 0; p < KS - 1; ++p) {
+    const float w = weight(p < part ? p : p + 1);
+    const f32x4* blk = block(part, p);
+#pragma unroll
+    for (int j = 0; j < NR / 4; ++j) own[j] += blk[64 * j] * w;
+  }
+  // register r of a 32-d block is d = 8 (r / 4) + 4 hl + r % 4
+  if (a.n_split > 1) {
+    const size_t pr = ((size_t)bh * rows + myq) * a.n_split + split;
+    if (q_in) {
+      if (part == 0 && hl == 0) a.part_lse[pr] = L > 0.f ? M + __builtin_amdgcn_logf(L) : kNegInf;
+#pragma unroll
+      for (int j = 0; j < NR / 4; ++j)
+        *(f32x4*)(a.part_o + pr * D + 8 * (part * (NR / 4) + j) + 4 * hl) = own[j] * inv;
+    }
+    return;
+  }
+  if (a.lse && part == 0 && hl == 0 && q_in) a.lse[(size_t)bh * rows + myq] = row_lse(M, L);
+  // packed into the group's rows
+  unsigned char* orows = lds + kMeetB + qg * 32 * kRowB;
+#pragma unroll
+  for (int j = 0; j < NR / 4; ++j) {
+    const vec2 lo = Tr::pack2(own[j][0] * inv, own[j][1] * inv), hi = Tr::pack2(own[j][2] * inv, own[j][3] * inv);
+    vec4 y;
+    y[0] = lo[0]; y[1] = lo[1]; y[2] = hi[0]; y[3] = hi[1];
+    const int c = part * (NR / 4) + j;  // 16-byte chunk: d = 8 c + 4 hl
+    *(u32x2*)(orows + l32 * kRowB + 16 * (c ^ (l32 % Gm::kLpr)) + 8 * hl) = __builtin_bit_cast(u32x2, y);
+  }
+  __syncthreads();
+  // the group's KS waves store its 32 rows, 16 bytes a lane
+#pragma unroll
+  for (int j = 0; j < 32 * kRowB / 1024 / KS; ++j) {
+    const int p = 64 * (j * KS + part) + lane, r = p / Gm::kLpr, c = p % Gm::kLpr;
+    const int row = qw0 + r;
+    if (row < rows)
+      *(u32x4*)(a.o + ((size_t)bh * rows + row) * D + 8 * c) =
+          *(const u32x4*)(orows + r * kRowB + 16 * (c ^ (r % Gm::kLpr)));
+  }
+}
+
+template <typename Tr, int D, class X, bool CAUSAL, int QG>
+__global__ __launch_bounds__(64 * kWaves) void cross_kernel(CrossArgs a, X x) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char bias_mem[];
+  // the splits of a tile are a launch's outermost index
+  const int per_split = a.n_work;
+  const int wg = (int)__builtin_amdgcn_workgroup_id_x() % per_split;
+  const int split = (int)__builtin_amdgcn_workgroup_id_x() / per_split;
+  const QTileWork wk = prefill_item(wg, a.n_work, a.n_qt, a.n_bh, a.order);
+  const int n_pass = wk.qt1 < 0 ? 1 : 2;
+#pragma clang loop unroll(disable)
+  for (int pass = 0; pass < n_pass; ++pass) {
+    if (pass) __syncthreads();  // every wave has stored its rows from LDS
+    cross_tile<Tr, D, X, CAUSAL, QG>(a, x, bias_mem, pass ? wk.bh1 : wk.bh0, pass ? wk.qt1 : wk.qt0, split);
+  }
+}
+
+// Joins the splits' partials: one wave per row, D / 64 values a lane.
+template <typename Tr, int D>
+__global__ __launch_bounds__(256) void cross_merge_kernel(const float* __restrict__ part_o,
+                                                          const float* __restrict__ part_lse,
+                                                          uint16_t* __restrict__ o, float* __restrict__ lse,
+                                                          long long n_rows, int n_split) {
+  constexpr int PER = D / 64;
+  const int lane = threadIdx.x & 63;
+  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= n_rows) return;
+  const float* pl = part_lse + row * n_split;
+  float M = kNegInf;
+  for (int s = 0; s < n_split; ++s) M = __builtin_fmaxf(M, pl[s]);
+  float W = 0.f, acc[PER] = {};
+  for (int s = 0; s < n_split; ++s) {
+    const float w = M == kNegInf ? 0.f : fast_exp2(pl[s] - M);
+    W += w;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) acc[i] += w * part_o[(row * n_split + s) * D + PER * lane + i];
+  }
+  const float inv = W > 0.f ? 1.f / W : 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) Tr::store(o, row * D + PER * lane + i, acc[i] * inv);
+  if (lse && lane == 0) lse[row] = row_lse(M, W);
+}
+
+struct CrossPlan {
+  int groups = 8, n_qt = 0, order = 0, n_split = 1;
+  long long grid = 0;  // without the splits
+};
+
+CrossPlan cross_plan(long long n_bh, int rows, int Skv, bool causal) {
+  CrossPlan p;
+  const long long cus = std::max(device_cus(), 1);
+  for (p.groups = 8; p.groups > 2; p.groups /= 2)
+    if (n_bh * ((rows + 32 * p.groups - 1) / (32 * p.groups)) >= cus) break;
+  p.n_qt = (rows + 32 * p.groups - 1) / (32 * p.groups);
+  p.grid = prefill_grid(1, (int)n_bh, p.n_qt, causal, 1, &p.order);
+  return p;
+}
+
+template <typename Tr, int D, class X, bool CAUSAL>
+hipError_t launch_t(CrossArgs a, const X& x, const CrossPlan& p, size_t lds, hipStream_t stream) {
+  const auto kernel = p.groups == 8   ? &cross_kernel<Tr, D, X, CAUSAL, 8>
+                      : p.groups == 4 ? &cross_kernel<Tr, D, X, CAUSAL, 4>
+                                      : &cross_kernel<Tr, D, X, CAUSAL, 2>;
+  const long long grid = p.grid * p.n_split;
+  if (grid > 0x7fffffffLL / (64 * kWaves)) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * kWaves), lds, stream, a, x);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || p.n_split <= 1) return e;
+  const long long n_rows = (long long)a.n_bh * a.rows, wgs = (n_rows + 3) / 4;
+  if (wgs > 0x7fffffffLL / 256) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((cross_merge_kernel<Tr, D>), dim3((unsigned)wgs), dim3(256), 0, stream, a.part_o, a.part_lse,
+                     a.o, a.lse, n_rows, p.n_split);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+// Whether a launch goes to decode's split walk: few enough query rows of a kv
+// head to be its heads, and no LSE, which that walk does not keep.
+static bool few_rows(const EncDecShape& s, bool bias, bool lse) {
+  return !bias && !lse && (long long)(s.Hq / s.Hkv) * s.Sq <= 16;
+}
+
+size_t cross_workspace_bytes(int dtype, const EncDecShape& s, bool bias, bool, bool lse) {
+  if (few_rows(s, bias, lse))
+    return std::max(decode_workspace_bytes(s.B, s.Hq * s.Sq, s.D, s.Skv),
+                    flash_decode_partials_bytes(dtype, s.B, s.Hq * s.Sq, s.Hkv, s.D, s.Skv));
+  return 0;
+}
+
+hipError_t launch_cross(int dtype, const void* q, const void* k, const void* v, void* o, float* lse,
+                        const EncDecShape& s, const BiasSpec* bias, bool causal, void* ws, size_t ws_bytes,
+                        hipStream_t stream) {
+  if ((long long)s.B * s.Hq * s.Sq == 0) return hipSuccess;
+  if (few_rows(s, bias, lse)) return launch_encdec_decode(dtype, q, k, v, o, s, nullptr, ws, ws_bytes, stream);
+  if (dtype == kDtypeF32) return launch_cross_f32(q, k, v, o, lse, s, bias, causal, stream);
+  const int G = s.Hq / s.Hkv;
+  // without positions a kv head's query heads are one run of rows
+  const bool packed = !bias && (long long)G * s.Sq <= 0x3fffffff;
+  CrossArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (uint16_t*)o, lse};
+  a.rows = packed ? G * s.Sq : s.Sq;
+  a.per_b = packed ? s.Hkv : s.Hq;
+  a.ratio = packed ? 1 : G;
+  const float eff = bias ? bias_scale(s.scale) : s.scale;
+  a.scale_log2 = __builtin_fabsf(eff) * kLog2e;
+  a.q_sign = __builtin_signbit(eff) ? 0x80008000u : 0u;
+  if ((long long)s.B * a.per_b > 0x7fffffffLL) return hipErrorInvalidValue;
+  a.n_bh = s.B * a.per_b;
+  const CrossPlan p = cross_plan(a.n_bh, a.rows, s.Skv, causal);
+  if (p.grid > 0x7fffffffLL) return hipErrorInvalidValue;
+  a.n_qt = p.n_qt;
+  a.n_work = (int)p.grid;
+  a.order = p.order;
+  a.n_split = p.n_split;
+  CrossX cx;
+  cx.kv_lens = s.kv_lens;
+  cx.Skv = s.Skv;
+#define CA_CROSS_CASE(TR, DD)                                                                              \
+  if (s.D == DD) {                                                                                         \
+    if (!bias) return launch_t<TR, DD, CrossX, false>(a, cx, p, 0, stream);                                \
+    const BiasX bx = bias_x(s, *bias, eff, 1.f / __builtin_fabsf(eff));                                         \
+    const size_t lds = bias_lds_bytes(bx.reach);                                                           \
+    return causal ? launch_t<TR, DD, BiasX, true>(a, bx, p, lds, stream)                                   \
+                  : launch_t<TR, DD, BiasX, false>(a, bx, p, lds, stream);                                 \
+  }
+  if (dtype == kDtypeBF16) {
+    CA_CROSS_CASE(BF16, 64)
+    CA_CROSS_CASE(BF16, 128)
+  } else if (dtype == kDtypeF16) {
+    CA_CROSS_CASE(F16, 64)
+    CA_CROSS_CASE(F16, 128)
+  }
+#undef CA_CROSS_CASE
+  return hipErrorInvalidValue;
+}
+
+}  // namespace ca

@@ -31,6 +31,10 @@
 // A sequence that fits one split writes its output directly; otherwise each
 // split writes (o / l, log2-sum-exp) to the workspace and a merge kernel
 // combines them.
+//
+// The contiguous cache's kernels also take a key length per sequence (the
+// single-token form of cross attention; CrossX of encdec.h) and a relative
+// position bias of a query at the end of its keys (BiasX).
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -38,6 +42,7 @@
 #include <mutex>
 
 #include "common.h"
+#include "encdec.h"
 #include "launch.h"
 #include "lds_dma.h"
 
@@ -142,7 +147,7 @@ __device__ __forceinline__ void dma_load_q(const uint16_t* __restrict__ qrow, in
 // each call. A step takes two pages: its instructions form one dependent
 // chain (LDS reads, K^T Q, max, exponentials, P V), about 0.5 us whether it
 // carries 16 tokens or 32, which is what a wave alone on its SIMD waits for.
-template <typename Tr, int D, int KIND, int RING, int PAGES>
+template <typename Tr, int D, int KIND, int RING, int PAGES, bool BIAS = false>
 __device__ __forceinline__ void dma_walk(const typename Tr::vec8 (&qv)[D / 32], f32x4 (&o)[D / 16],
                                          float& m_run, float& l_run, unsigned char* ring,
                                          const void* __restrict__ Kc, const void* __restrict__ Vc,
@@ -150,7 +155,8 @@ __device__ __forceinline__ void dma_walk(const typename Tr::vec8 (&qv)[D / 32], 
                                          const float* __restrict__ v_scale, int per_block,
                                          const int32_t* __restrict__ bt_row, int Hkv, int hk,
                                          int num_blocks, int p_begin, int p_end, int Lctx,
-                                         float scale_log2, const unsigned char* dummy) {
+                                         float scale_log2, const unsigned char* dummy,
+                                         const DecodeBias& bias = {}) {
   using vec8 = typename Tr::vec8;
   constexpr int NKS = D / 32, NB = D / 16;
   constexpr bool FP8 = KIND == kKindPagedFp8, CONTIG = KIND == kKindContig16;
@@ -365,6 +371,18 @@ __device__ __forceinline__ void dma_walk(const typename Tr::vec8 (&qv)[D / 32], 
         slot_ok[4 * pp + r] = (page0 + pp) * 16 + 4 * grp + r < tok_end;
       }
     }
+    if constexpr (BIAS) {
+      // the step's first token lies Lctx - 1 - 16 page0 before the query
+      if (Lctx - 32 - 16 * page0 >= bias.reach) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] += bias.far;
+      } else {
+        float e[8];
+        decode_bias(bias, Lctx - 1 - 16 * page0 - 4 * grp, e);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] += e[i];
+      }
+    }
     if (partial) {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -486,14 +504,15 @@ struct MwCfg {
   static constexpr int kPages = 128;      // pages per call of dma_walk (two page-id registers)
 };
 
-template <typename Tr, int D, int KIND, int NW>
+template <typename Tr, int D, int KIND, int NW, class X = SelfX>
 __global__ __launch_bounds__(64 * NW) void decode_mw_kernel(
     const uint16_t* __restrict__ Q, const void* __restrict__ Kc, const void* __restrict__ Vc,
     const float* __restrict__ k_scale, const float* __restrict__ v_scale, int per_block,
     const int32_t* __restrict__ block_tables, const int32_t* __restrict__ context_lens,
     uint16_t* __restrict__ O, float* __restrict__ ws_o, float* __restrict__ ws_lse, int Hq,
     int Hkv, int max_blocks, int S_contig, int num_blocks, int max_splits, int pages_per_split,
-    int n_hc, float scale_log2) {
+    int n_hc, float scale_log2, X x) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char bias_mem[];
   using Cfg = MwCfg<KIND, D, NW>;
   constexpr bool CONTIG = KIND == kKindContig16;
   constexpr int NKS = D / 32, NB = D / 16;
@@ -518,7 +537,8 @@ __global__ __launch_bounds__(64 * NW) void decode_mw_kernel(
   const int Gq = Hq / Hkv;
   const int hq0 = hk * Gq + hc * 16;
   const int Gc = min(16, Gq - hc * 16);
-  const int Lctx = CONTIG ? S_contig : min(max(0, context_lens[n]), max_blocks * kDecodePage);
+  int Lctx = CONTIG ? S_contig : min(max(0, context_lens[n]), max_blocks * kDecodePage);
+  if constexpr (X::kCross) Lctx = x.kv_len(n);
   const int n_pages = (Lctx + kDecodePage - 1) / kDecodePage;
   const int n_splits = max(1, (n_pages + pages_per_split - 1) / pages_per_split);
   const int split = n_splits - 1 - from_end;
@@ -531,16 +551,18 @@ __global__ __launch_bounds__(64 * NW) void decode_mw_kernel(
 #pragma unroll
   for (int i = 0; i < NB; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m_run = kNegInf, l_run = 0.f;
+  DecodeBias bias{};
+  if constexpr (X::kBias) bias = decode_bias_fill(x, hq0, Gc, bias_mem, 64 * NW, l16);
   if (p_begin < p_end) {
     typename Tr::vec8 qv[NKS];
     dma_load_q<Tr, D>(Q + ((size_t)n * Hq + hq0) * D, Gc, qv);
     const size_t head = CONTIG ? ((size_t)n * Hkv + hk) * (size_t)S_contig * (2 * D) : 0;
     for (int p = p_begin; p < p_end; p += Cfg::kPages)
-      dma_walk<Tr, D, KIND, Cfg::kRing, Cfg::kPages>(
+      dma_walk<Tr, D, KIND, Cfg::kRing, Cfg::kPages, X::kBias>(
           qv, o, m_run, l_run, lds + wave * kRingB, (const unsigned char*)Kc + head,
           (const unsigned char*)Vc + head, k_scale, v_scale, per_block,
           CONTIG ? nullptr : block_tables + (size_t)n * max_blocks, Hkv, hk, num_blocks, p,
-          min(p + Cfg::kPages, p_end), Lctx, scale_log2, (const unsigned char*)Q);
+          min(p + Cfg::kPages, p_end), Lctx, scale_log2, (const unsigned char*)Q, bias);
   }
 
   if constexpr (NW == 1) {
@@ -985,11 +1007,11 @@ static int mw_waves(long long grid, int pages) {
   if (pages <= 16) return grid <= 2 * cus ? 8 : 1;
   return 4;
 }
-template <typename Tr, int D, int KIND>
+template <typename Tr, int D, int KIND, class X = SelfX>
 static auto mw_kernel(int nw) {
-  return nw == 8   ? &decode_mw_kernel<Tr, D, KIND, 8>
-         : nw == 4 ? &decode_mw_kernel<Tr, D, KIND, 4>
-                   : &decode_mw_kernel<Tr, D, KIND, 1>;
+  return nw == 8   ? &decode_mw_kernel<Tr, D, KIND, 8, X>
+         : nw == 4 ? &decode_mw_kernel<Tr, D, KIND, 4, X>
+                   : &decode_mw_kernel<Tr, D, KIND, 1, X>;
 }
 
 template <typename Tr, int D, int KIND>
@@ -1029,7 +1051,7 @@ static hipError_t launch_paged_decode_t(const void* q, const void* kc, const voi
   hipLaunchKernelGGL((mw_kernel<Tr, D, KIND>(nw)), dim3((unsigned)grid), dim3(64 * nw), 0, stream,
                      (const uint16_t*)q, kc, vc, k_scale, v_scale, per_block, bt, lens,
                      (uint16_t*)out, ws_o, ws_lse, Hq, Hkv, max_blocks, 0, num_blocks, max_splits,
-                     pages_per_split, n_hc, scale * kLog2e);
+                     pages_per_split, n_hc, scale * kLog2e, SelfX{});
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || max_splits <= 1) return e;
   hipLaunchKernelGGL((decode_merge_kernel<Tr, D>), dim3((unsigned)(N * Hq)), dim3(64), 0, stream,
@@ -1066,10 +1088,10 @@ static SplitGrid contig_grid(int N, int Hq, int Hkv, int D, int S, size_t ws_byt
   return g;
 }
 
-template <typename Tr, int D>
+template <typename Tr, int D, class X>
 static hipError_t launch_contig_decode_t(const void* q, const void* k, const void* v, void* out,
                                          int N, int Hq, int Hkv, int S, float scale, void* ws,
-                                         size_t ws_bytes, hipStream_t stream) {
+                                         size_t ws_bytes, const X& x, size_t lds, hipStream_t stream) {
   constexpr int KIND = kKindContig16;
   const int Gq = Hq / Hkv;
   const int n_hc = (Gq + 15) / 16;
@@ -1082,13 +1104,15 @@ static hipError_t launch_contig_decode_t(const void* q, const void* k, const voi
   if (grid == 0) return hipSuccess;
   if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
   const int nw = mw_waves(grid, plan.pages);
-  hipLaunchKernelGGL((mw_kernel<Tr, D, KIND>(nw)), dim3((unsigned)grid), dim3(64 * nw), 0, stream,
+  const int32_t* lens = nullptr;
+  if constexpr (X::kCross) lens = x.kv_lens;
+  hipLaunchKernelGGL((mw_kernel<Tr, D, KIND, X>(nw)), dim3((unsigned)grid), dim3(64 * nw), lds, stream,
                      (const uint16_t*)q, k, v, nullptr, nullptr, 0, nullptr, nullptr, (uint16_t*)out,
-                     ws_o, ws_lse, Hq, Hkv, 0, S, 1, max_splits, plan.pages, n_hc, scale * kLog2e);
+                     ws_o, ws_lse, Hq, Hkv, 0, S, 1, max_splits, plan.pages, n_hc, scale * kLog2e, x);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || max_splits <= 1) return e;
   hipLaunchKernelGGL((decode_merge_kernel<Tr, D>), dim3((unsigned)(N * Hq)), dim3(64), 0, stream,
-                     nullptr, S, ws_o, ws_lse, out, Hq, max_splits, plan.pages);
+                     lens, S, ws_o, ws_lse, out, Hq, max_splits, plan.pages);
   return hipGetLastError();
 }
 
@@ -1133,14 +1157,14 @@ __device__ __forceinline__ float e4m3_to_f32(uint32_t w, int b) {
   return b == 0 ? lo[0] : b == 1 ? lo[1] : b == 2 ? hi[0] : hi[1];
 }
 
-template <int D, int SRC, int G>
+template <int D, int SRC, int G, class X = SelfX>
 __global__ __launch_bounds__(64) void decode_f32_kernel(
     const float* __restrict__ Q, const void* __restrict__ Kc, const void* __restrict__ Vc,
     const float* __restrict__ k_scale, const float* __restrict__ v_scale, int per_block,
     const int32_t* __restrict__ block_tables, const int32_t* __restrict__ context_lens,
     float* __restrict__ O, float* __restrict__ ws_o, float* __restrict__ ws_lse, int Hq,
     int Hkv, int S_contig, int max_blocks, int num_blocks, int max_splits, int n_hc,
-    float scale_log2) {
+    float scale_log2, X x) {
   constexpr bool PAGED = SRC != kSrcF32Contig;
   constexpr bool FP8 = SRC == kSrcFp8Paged;
   constexpr int PER = D / 64;
@@ -1160,7 +1184,8 @@ __global__ __launch_bounds__(64) void decode_f32_kernel(
   const int Gq = Hq / Hkv;
   const int hq0 = hk * Gq + hc * G;
   const int Gc = min(G, Gq - hc * G);
-  const int L = PAGED ? min(max(0, context_lens[n]), max_blocks * kDecodePage) : S_contig;
+  int L = PAGED ? min(max(0, context_lens[n]), max_blocks * kDecodePage) : S_contig;
+  if constexpr (X::kCross) L = x.kv_len(n);
   // (no sum past L: contexts go up to 2^31 - 16 tokens)
   const int n_splits = max(1, L / kSplitTokens + (L % kSplitTokens != 0));
   if (split >= n_splits) return;
@@ -1170,6 +1195,9 @@ __global__ __launch_bounds__(64) void decode_f32_kernel(
     const int g = i / D, d = i % D;
     qs[g][d] = (g < Gc) ? Q[((size_t)n * Hq + hq0 + g) * D + d] * scale_log2 : 0.f;
   }
+  __shared__ uint16_t first[X::kBias ? kMaxBuckets : 1];
+  if constexpr (X::kBias)
+    for (int i = lane; i < x.side; i += 64) first[i] = x.first[i];
   __syncthreads();
 
   float m_run[G], l_run[G], o[G][PER];
@@ -1235,6 +1263,11 @@ __global__ __launch_bounds__(64) void decode_f32_kernel(
           s[g] = __builtin_fmaf(qs[g][d + 2], kv.z, s[g]);
           s[g] = __builtin_fmaf(qs[g][d + 3], kv.w, s[g]);
         }
+      }
+      if constexpr (X::kBias) {
+        const float* col = x.table + (size_t)bias_bucket(x, first, tc - (L - 1)) * x.Hq + hq0;
+#pragma unroll
+        for (int g = 0; g < G; ++g) s[g] += bias_clamp(col[min(g, Gc - 1)]) * x.mul;
       }
     }
 #pragma unroll
@@ -1334,8 +1367,8 @@ struct F32DecodeArgs {
   size_t ws_bytes;
 };
 
-template <int D, int SRC, int G>
-static hipError_t launch_decode_f32_t(const F32DecodeArgs& a, hipStream_t stream) {
+template <int D, int SRC, int G, class X>
+static hipError_t launch_decode_f32_t(const F32DecodeArgs& a, const X& x, hipStream_t stream) {
   constexpr bool PAGED = SRC != kSrcF32Contig;
   const int max_tokens = PAGED ? a.max_blocks * kDecodePage : a.S_contig;
   const int pages = (max_tokens + kDecodePage - 1) / kDecodePage;
@@ -1349,24 +1382,24 @@ static hipError_t launch_decode_f32_t(const F32DecodeArgs& a, hipStream_t stream
   const long long grid = (long long)a.N * a.Hkv * n_hc * max_splits;
   if (grid == 0) return hipSuccess;
   if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((decode_f32_kernel<D, SRC, G>), dim3((unsigned)grid), dim3(64), 0, stream,
+  hipLaunchKernelGGL((decode_f32_kernel<D, SRC, G, X>), dim3((unsigned)grid), dim3(64), 0, stream,
                      (const float*)a.q, a.kc, a.vc, a.k_scale, a.v_scale, a.per_block, a.bt, a.lens,
                      (float*)a.out, ws_o, ws_lse, a.Hq, a.Hkv, a.S_contig, a.max_blocks,
-                     a.num_blocks, max_splits, n_hc, a.scale * kLog2e);
+                     a.num_blocks, max_splits, n_hc, a.scale * kLog2e, x);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || max_splits <= 1) return e;
   hipLaunchKernelGGL((decode_merge_kernel<F32, D>), dim3((unsigned)(a.N * a.Hq)), dim3(64), 0,
-                     stream, PAGED ? a.lens : nullptr, max_tokens, ws_o, ws_lse, a.out, a.Hq,
+                     stream, a.lens, max_tokens, ws_o, ws_lse, a.out, a.Hq,
                      max_splits, kPagesPerWave);
   return hipGetLastError();
 }
 
 // Query heads per wave for the fp32 kernel: the group size rounded up to a
 // power of two, at most 8 (larger groups take several waves).
-template <int SRC>
-static hipError_t launch_decode_f32(int D, const F32DecodeArgs& a, hipStream_t stream) {
+template <int SRC, class X = SelfX>
+static hipError_t launch_decode_f32(int D, const F32DecodeArgs& a, hipStream_t stream, const X& x = {}) {
   const int Gq = a.Hq / a.Hkv;
-#define CA_F32D(DD, GG) return launch_decode_f32_t<DD, SRC, GG>(a, stream);
+#define CA_F32D(DD, GG) return launch_decode_f32_t<DD, SRC, GG>(a, x, stream);
 #define CA_F32G(DD)                  \
   if (Gq <= 1) { CA_F32D(DD, 1) }    \
   if (Gq <= 2) { CA_F32D(DD, 2) }    \
@@ -1494,7 +1527,8 @@ hipError_t launch_flash_decode(int dtype, const void* q, const void* k, const vo
                                int B, int Hq, int Hkv, int S, int D, float scale, void* ws,
                                size_t ws_bytes, hipStream_t stream) {
 #define CA_FD(TR, DD) \
-  if (D == DD) return launch_contig_decode_t<TR, DD>(q, k, v, o, B, Hq, Hkv, S, scale, ws, ws_bytes, stream);
+  if (D == DD)        \
+    return launch_contig_decode_t<TR, DD>(q, k, v, o, B, Hq, Hkv, S, scale, ws, ws_bytes, SelfX{}, 0, stream);
   if (dtype == kDtypeBF16) { CA_FD(BF16, 64) CA_FD(BF16, 128) }
   if (dtype == kDtypeF16) { CA_FD(F16, 64) CA_FD(F16, 128) }
 #undef CA_FD
@@ -1503,6 +1537,35 @@ hipError_t launch_flash_decode(int dtype, const void* q, const void* k, const vo
                           scale, ws, ws_bytes};
     return launch_decode_f32<kSrcF32Contig>(D, a, stream);
   }
+  return hipErrorInvalidValue;
+}
+
+hipError_t launch_encdec_decode(int dtype, const void* q, const void* k, const void* v, void* o,
+                                const EncDecShape& s, const BiasSpec* bias, void* ws, size_t ws_bytes,
+                                hipStream_t stream) {
+  CrossX cx;
+  cx.kv_lens = s.kv_lens;
+  cx.Skv = s.Skv;
+  // query rows of a kv head are its heads' one after the other, as decode's heads are
+  const int Hq = s.Hq * s.Sq;
+  if (dtype == kDtypeF32) {
+    const F32DecodeArgs a{q, k, v, nullptr, nullptr, 0, nullptr, s.kv_lens, o, s.B, Hq, s.Hkv, 0, 1, s.Skv,
+                          s.scale, ws, ws_bytes};
+    if (!bias) return launch_decode_f32<kSrcF32Contig>(s.D, a, stream, cx);
+    return launch_decode_f32<kSrcF32Contig>(s.D, a, stream, bias_x(s, *bias, s.scale, kLog2e));
+  }
+#define CA_FD(TR, DD)                                                                                              \
+  if (s.D == DD) {                                                                                                 \
+    if (!bias)                                                                                                     \
+      return launch_contig_decode_t<TR, DD>(q, k, v, o, s.B, Hq, s.Hkv, s.Skv, s.scale, ws, ws_bytes, cx, 0,       \
+                                            stream);                                                               \
+    const BiasX bx = bias_x(s, *bias, s.scale, kLog2e);                                                            \
+    return launch_contig_decode_t<TR, DD>(q, k, v, o, s.B, Hq, s.Hkv, s.Skv, s.scale, ws, ws_bytes, bx,            \
+                                          decode_bias_lds_bytes(bx.side, bx.reach), stream);                       \
+  }
+  if (dtype == kDtypeBF16) { CA_FD(BF16, 64) CA_FD(BF16, 128) }
+  if (dtype == kDtypeF16) { CA_FD(F16, 64) CA_FD(F16, 128) }
+#undef CA_FD
   return hipErrorInvalidValue;
 }
 

@@ -26,17 +26,22 @@
 // LDS (prefill_f32_kernel): K row-major with row stride D + 4 floats, V
 // transposed ([D][32 keys]) with row stride 36 floats; both make the float4
 // operand reads of a 16-lane group hit 16 distinct 4-bank groups.
+//
+// With an X of their own (encdec.h) the same kernels serve cross attention and
+// attention with a relative position bias, which here is added to the log2 logits.
 #include "common.h"
+#include "encdec.h"
 #include "launch.h"
 
 namespace ca {
 
 // One query tile (BM rows of head bh): the key walk and the output store.
 // Other waves may still read the LDS tiles when a wave returns.
-template <int D, bool CAUSAL>
+template <int D, bool CAUSAL, class X>
 __device__ CA_INLINE void prefill_f32_qtile(
     const float* __restrict__ Q, const float* __restrict__ K, const float* __restrict__ V,
-    float* __restrict__ O, float* __restrict__ Lse, int S, int Hq, int Hkv, float scale_log2, int bh, int qt) {
+    float* __restrict__ O, float* __restrict__ Lse, int S, int Hq, int Hkv, float scale_log2, int bh, int qt,
+    const X& x_, unsigned char* bias_mem) {
   constexpr int NW = 4;
   constexpr int BM = 32 * NW;
   constexpr int BN = 32;
@@ -55,10 +60,15 @@ __device__ CA_INLINE void prefill_f32_qtile(
   const int b = bh / Hq, h = bh % Hq;
   const int hk = h / (Hq / Hkv);
   const int q0 = qt * BM;
+  int Skv = S, n_keys = S;
+  if constexpr (X::kCross) {
+    Skv = x_.Skv;
+    n_keys = x_.kv_len(b);
+  }
   const float* Qp = Q + (size_t)(b * Hq + h) * S * D;
   float* Op = O + (size_t)(b * Hq + h) * S * D;
-  const float* Kp = K + (size_t)(b * Hkv + hk) * S * D;
-  const float* Vp = V + (size_t)(b * Hkv + hk) * S * D;
+  const float* Kp = K + (size_t)(b * Hkv + hk) * Skv * D;
+  const float* Vp = V + (size_t)(b * Hkv + hk) * Skv * D;
 
   // lane recomputed per query tile (lane_here): hoisted out of the kernel's
   // pass loop, its offsets spilled at D = 128
@@ -78,8 +88,14 @@ __device__ CA_INLINE void prefill_f32_qtile(
     qv[k4] = x.x; qv[k4 + 1] = x.y; qv[k4 + 2] = x.z; qv[k4 + 3] = x.w;
   }
 
-  const int kv_end = CAUSAL ? min(S, q0 + BM) : S;
+  const int kv_end = CAUSAL ? min(n_keys, q0 + BM) : n_keys;
   const int n_tiles = (kv_end + BN - 1) / BN;
+  // distance 0's bias, at the lane's query and its first key of a block
+  const float* be = nullptr;
+  if constexpr (X::kBias) {
+    bias_fill(x_, h, bias_mem, NW * 64);
+    be = bias_zero(x_, bias_mem) + 31 - l32 + 16 * hl;
+  }
 
   float4 kreg[F4_PER_THREAD], vreg[F4_PER_THREAD];
   auto gload = [&](int t) {
@@ -88,7 +104,7 @@ __device__ CA_INLINE void prefill_f32_qtile(
       const int idx = tid + NW * 64 * it;
       const int row = idx / F4_ROW, c4 = idx % F4_ROW;
       const int key = t * BN + row;
-      if (key < S) {
+      if (key < n_keys) {
         kreg[it] = *(const float4*)(Kp + (size_t)key * D + 4 * c4);
         vreg[it] = *(const float4*)(Vp + (size_t)key * D + 4 * c4);
       } else {
@@ -144,13 +160,17 @@ __device__ CA_INLINE void prefill_f32_qtile(
     // online softmax in the log2 domain; register r holds key k0 + 16 hl + r
     float x[16];
     float tm = kNegInf;
-    const bool need_mask = CAUSAL ? (k0 + BN - 1 > qw0) : (k0 + BN > S);
+    const bool need_mask =
+        CAUSAL ? (k0 + BN - 1 > qw0 || (X::kCross && k0 + BN > n_keys)) : (k0 + BN > n_keys);
+    const float* bb = be;
+    if constexpr (X::kBias) bb += bias_block(x_, k0 - qw0 - 31);
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       x[r] = s[r] * scale_log2;
+      if constexpr (X::kBias) x[r] = __builtin_fmaf(s[r], scale_log2, bb[r]);
       if (need_mask) {
         const int key = k0 + 16 * hl + r;
-        if (key >= S || (CAUSAL && key > myq)) x[r] = kNegInf;
+        if (key >= n_keys || (CAUSAL && key > myq)) x[r] = kNegInf;
       }
       tm = __builtin_fmaxf(tm, x[r]);
     }
@@ -203,19 +223,20 @@ __device__ CA_INLINE void prefill_f32_qtile(
   }
 }
 
-template <int D, bool CAUSAL>
+template <int D, bool CAUSAL, class X>
 __global__ __launch_bounds__(256, 2) void prefill_f32_kernel(
     const float* __restrict__ Q, const float* __restrict__ K, const float* __restrict__ V,
     float* __restrict__ O, float* __restrict__ Lse, int S, int Hq, int Hkv, float scale_log2, int n_qt, int n_bh,
-    int n_work, int order) {
+    int n_work, int order, X x) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char bias_mem[];
   const QTileWork wk = prefill_item(blockIdx.x, n_work, n_qt, n_bh, order);
   const int n_pass = wk.qt1 < 0 ? 1 : 2;
 #pragma clang loop unroll(disable)
   for (int pass = 0; pass < n_pass; ++pass) {
     // the second tile restages the LDS buffers: every wave must be done reading them
     if (pass) __syncthreads();
-    prefill_f32_qtile<D, CAUSAL>(Q, K, V, O, Lse, S, Hq, Hkv, scale_log2, pass ? wk.bh1 : wk.bh0,
-                                 pass ? wk.qt1 : wk.qt0);
+    prefill_f32_qtile<D, CAUSAL, X>(Q, K, V, O, Lse, S, Hq, Hkv, scale_log2, pass ? wk.bh1 : wk.bh0,
+                                    pass ? wk.qt1 : wk.qt0, x, bias_mem);
   }
 }
 
@@ -270,10 +291,11 @@ struct SplitStage {
 // item's S MFMAs have read K, its V once the PV MFMAs have read V, and at the
 // switch from block qa to qb2 the new Q once the last S MFMAs of qa have read
 // Q, so the walk runs on from one block into the other.
-template <int D, bool CAUSAL>
+template <int D, bool CAUSAL, class X>
 __device__ CA_INLINE void prefill_f32_split_walk(
     const float* __restrict__ Q, const float* __restrict__ K, const float* __restrict__ V, int S,
-    int Hq, int Hkv, float scale_log2, int bh, int qa, int qb2, SplitStage<D>& stg) {
+    int Hq, int Hkv, float scale_log2, int bh, int qa, int qb2, SplitStage<D>& stg, const X& x,
+    unsigned char* bias_mem) {
   constexpr int HD = D / 2;
   constexpr int NOB = D / 32;
   constexpr int NW = SplitStage<D>::NW;
@@ -281,9 +303,14 @@ __device__ CA_INLINE void prefill_f32_split_walk(
 
   const int b = bh / Hq, h = bh % Hq;
   const int hk = h / (Hq / Hkv);
+  int Skv = S, n_keys = S;
+  if constexpr (X::kCross) {
+    Skv = x.Skv;
+    n_keys = x.kv_len(b);
+  }
   const float* Qp = Q + (size_t)(b * Hq + h) * S * D;
-  const float* Kp = K + (size_t)(b * Hkv + hk) * S * D;
-  const float* Vp = V + (size_t)(b * Hkv + hk) * S * D;
+  const float* Kp = K + (size_t)(b * Hkv + hk) * Skv * D;
+  const float* Vp = V + (size_t)(b * Hkv + hk) * Skv * D;
 
   const int tid = threadIdx.x;
   // wave index made scalar: the item loop and its branches are uniform
@@ -291,7 +318,16 @@ __device__ CA_INLINE void prefill_f32_split_walk(
   const int l32 = lane & 31, hl = lane >> 5;
   const int krow = 16 * ((l32 >> 2) & 1) + 4 * (l32 >> 3) + (l32 & 3);
 
-  auto n_tiles_of = [&](int qb) { return CAUSAL ? qb + 1 : (S + 31) / 32; };
+  auto n_tiles_of = [&](int qb) {
+    if constexpr (X::kCross && CAUSAL) return min(qb + 1, (n_keys + 31) / 32);
+    return CAUSAL ? qb + 1 : (n_keys + 31) / 32;
+  };
+  // distance 0's bias, at the lane's query and its first key of a block
+  const float* be = nullptr;
+  if constexpr (X::kBias) {
+    bias_fill(x, h, bias_mem, NW * 64);
+    be = bias_zero(x, bias_mem) + 31 - l32 + 16 * hl;
+  }
   const int na = n_tiles_of(qa);
   const int n_all = na + (qb2 >= 0 ? n_tiles_of(qb2) : 0);
   // item -> first key of its tile (items past the list clamp to valid rows)
@@ -349,17 +385,17 @@ __device__ CA_INLINE void prefill_f32_split_walk(
   };
   load_q(qv, g < na ? qa : qb2);
 
-  // key rows past S are clamped to S - 1 (finite data; their logits are masked)
+  // key rows past the last are clamped to it (finite data; their logits are masked)
   float4 kr[HD / 4];
   float vr[NOB][16];
   auto load_k = [&](int gi) {
-    const float* kp = Kp + (size_t)min(key0(gi) + krow, S - 1) * D + 4 * hl;
+    const float* kp = Kp + (size_t)min(key0(gi) + krow, n_keys - 1) * D + 4 * hl;
 #pragma unroll
     for (int j = 0; j < HD / 4; ++j) kr[j] = *(const float4*)(kp + 8 * j);
   };
   auto load_v = [&](int gi) {
     const int k0 = key0(gi);
-    if (k0 + 32 <= S) {  // whole tile: one address, immediate offsets
+    if (k0 + 32 <= n_keys) {  // whole tile: one address, immediate offsets
       const float* vp = Vp + (size_t)(k0 + 16 * hl) * D + l32;
 #pragma unroll
       for (int st = 0; st < 16; ++st)
@@ -368,15 +404,20 @@ __device__ CA_INLINE void prefill_f32_split_walk(
     } else {
 #pragma unroll
       for (int st = 0; st < 16; ++st) {
-        const float* vp = Vp + (size_t)min(k0 + 16 * hl + st, S - 1) * D + l32;
+        const float* vp = Vp + (size_t)min(k0 + 16 * hl + st, n_keys - 1) * D + l32;
 #pragma unroll
         for (int ob = 0; ob < NOB; ++ob) vr[ob][st] = vp[32 * ob];
       }
     }
   };
-  auto qk = [&](f32x16& s) {
+  auto qk = [&](f32x16& s, int gi) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = 0.f;
+    if constexpr (X::kBias) {
+      const float* bb = be + bias_block(x, key0(gi) - 32 * (gi < na ? qa : qb2) - 31);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = bb[r];
+    }
 #pragma unroll
     for (int j = 0; j < HD / 4; ++j) {
       s = __builtin_amdgcn_mfma_f32_32x32x2f32(kr[j].x, qv[4 * j], s, 0, 0, 0);
@@ -395,8 +436,8 @@ __device__ CA_INLINE void prefill_f32_split_walk(
   auto softmax = [&](f32x16& s, int gi) {
     const int q0 = (gi < na ? qa : qb2) * 32;
     const int k0 = key0(gi);
-    if ((CAUSAL && k0 == q0) || k0 + 32 > S) {
-      const int lim = CAUSAL ? min(q0 + l32, S - 1) : S - 1;  // last visible key of this row
+    if ((CAUSAL && k0 == q0) || k0 + 32 > n_keys) {
+      const int lim = CAUSAL ? min(q0 + l32, n_keys - 1) : n_keys - 1;  // last visible key of this row
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         if (k0 + 16 * hl + r > lim) s[r] = kNegInf;
@@ -447,7 +488,7 @@ __device__ CA_INLINE void prefill_f32_split_walk(
   for (;; g += NW) {
     const bool more = g + NW < n_all;
     const bool switch_blk = g < na && g + NW >= na && more;  // next item is in block qb2
-    qk(s);
+    qk(s, g);
     if (switch_blk) load_q(qv, qb2);
     if (more) load_k(g + NW);
     softmax(s, g);
@@ -516,17 +557,18 @@ __device__ CA_INLINE void prefill_f32_split_merge(float* __restrict__ O, float* 
 // p and n_qb-1-p (equal total walks); non-causal, when the launch has more
 // blocks than CUs, p and p + per_head (one round of workgroups instead of
 // two). per_head = work items per (b, h).
-template <int D, bool CAUSAL>
+template <int D, bool CAUSAL, class X>
 __global__ __launch_bounds__(64 * SplitStage<D>::NW, 1) void prefill_f32_split_kernel(
     const float* __restrict__ Q, const float* __restrict__ K, const float* __restrict__ V,
     float* __restrict__ O, float* __restrict__ Lse, int S, int Hq, int Hkv, float scale_log2, int n_qb,
-    int per_head, int n_work) {
+    int per_head, int n_work, X x) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char bias_mem[];
   __shared__ __attribute__((aligned(16))) SplitStage<D> stg;
   const int item = xcd_remap(blockIdx.x, n_work);
   const int bh = item / per_head, p = item % per_head;
   int p2 = CAUSAL ? n_qb - 1 - p : p + per_head;
   if (p2 == p || p2 >= n_qb) p2 = -1;
-  prefill_f32_split_walk<D, CAUSAL>(Q, K, V, S, Hq, Hkv, scale_log2, bh, p, p2, stg);
+  prefill_f32_split_walk<D, CAUSAL, X>(Q, K, V, S, Hq, Hkv, scale_log2, bh, p, p2, stg, x, bias_mem);
   __syncthreads();
   prefill_f32_split_merge<D>(O, Lse, S, bh, p, 0, stg);
   if (p2 >= 0) prefill_f32_split_merge<D>(O, Lse, S, bh, p2, 1, stg);
@@ -554,9 +596,9 @@ static bool f32_splits(long long grid, bool causal, int D, int S, long long n_qt
   return 10 * 2 * cus > 6 * n_bh * (n_qt + 1);
 }
 
-template <int D, bool CAUSAL>
+template <int D, bool CAUSAL, class X>
 static hipError_t launch_prefill_f32_t(const void* q, const void* k, const void* v, void* o, float* lse,
-                                       int B, int Hq, int Hkv, int S, float scale,
+                                       int B, int Hq, int Hkv, int S, float scale, const X& x, size_t lds,
                                        hipStream_t stream) {
   constexpr int BM = 128;
   const int n_qt = (S + BM - 1) / BM;
@@ -569,26 +611,47 @@ static hipError_t launch_prefill_f32_t(const void* q, const void* k, const void*
     const bool two = CAUSAL || (long long)B * Hq * n_qb > device_cus();
     const int per_head = two ? (n_qb + 1) / 2 : n_qb;
     const long long grid_s = (long long)B * Hq * per_head;
-    hipLaunchKernelGGL((prefill_f32_split_kernel<D, CAUSAL>), dim3((unsigned)grid_s),
-                       dim3(64 * SplitStage<D>::NW), 0, stream, (const float*)q, (const float*)k, (const float*)v, (float*)o, lse, S,
-                       Hq, Hkv, scale * kLog2e, n_qb, per_head, (int)grid_s);
+    hipLaunchKernelGGL((prefill_f32_split_kernel<D, CAUSAL, X>), dim3((unsigned)grid_s),
+                       dim3(64 * SplitStage<D>::NW), lds, stream, (const float*)q, (const float*)k, (const float*)v, (float*)o, lse, S,
+                       Hq, Hkv, scale * kLog2e, n_qb, per_head, (int)grid_s, x);
     return hipGetLastError();
   }
-  hipLaunchKernelGGL((prefill_f32_kernel<D, CAUSAL>), dim3((unsigned)grid), dim3(256), 0, stream,
+  hipLaunchKernelGGL((prefill_f32_kernel<D, CAUSAL, X>), dim3((unsigned)grid), dim3(256), lds, stream,
                      (const float*)q, (const float*)k, (const float*)v, (float*)o, lse, S, Hq, Hkv,
-                     scale * kLog2e, n_qt, B * Hq, (int)grid, order);
+                     scale * kLog2e, n_qt, B * Hq, (int)grid, order, x);
   return hipGetLastError();
 }
 
 hipError_t launch_prefill_f32(const void* q, const void* k, const void* v, void* o, float* lse, int B,
                               int Hq, int Hkv, int S, int D, float scale, bool causal,
                               hipStream_t stream) {
+  const SelfX x;
   if (D == 64)
-    return causal ? launch_prefill_f32_t<64, true>(q, k, v, o, lse, B, Hq, Hkv, S, scale, stream)
-                  : launch_prefill_f32_t<64, false>(q, k, v, o, lse, B, Hq, Hkv, S, scale, stream);
+    return causal ? launch_prefill_f32_t<64, true>(q, k, v, o, lse, B, Hq, Hkv, S, scale, x, 0, stream)
+                  : launch_prefill_f32_t<64, false>(q, k, v, o, lse, B, Hq, Hkv, S, scale, x, 0, stream);
   if (D == 128)
-    return causal ? launch_prefill_f32_t<128, true>(q, k, v, o, lse, B, Hq, Hkv, S, scale, stream)
-                  : launch_prefill_f32_t<128, false>(q, k, v, o, lse, B, Hq, Hkv, S, scale, stream);
+    return causal ? launch_prefill_f32_t<128, true>(q, k, v, o, lse, B, Hq, Hkv, S, scale, x, 0, stream)
+                  : launch_prefill_f32_t<128, false>(q, k, v, o, lse, B, Hq, Hkv, S, scale, x, 0, stream);
+  return hipErrorInvalidValue;
+}
+
+hipError_t launch_cross_f32(const void* q, const void* k, const void* v, void* o, float* lse, const EncDecShape& s,
+                            const BiasSpec* bias, bool causal, hipStream_t stream) {
+#define CA_F32_CASE(DD, CAUSAL, X, LDS) \
+  launch_prefill_f32_t<DD, CAUSAL>(q, k, v, o, lse, s.B, s.Hq, s.Hkv, s.Sq, s.scale, X, LDS, stream)
+  if (!bias) {
+    CrossX x;
+    x.kv_lens = s.kv_lens;
+    x.Skv = s.Skv;
+    if (s.D == 64) return CA_F32_CASE(64, false, x, 0);
+    if (s.D == 128) return CA_F32_CASE(128, false, x, 0);
+    return hipErrorInvalidValue;
+  }
+  const BiasX x = bias_x(s, *bias, s.scale, kLog2e);
+  const size_t lds = bias_lds_bytes(x.reach);
+  if (s.D == 64) return causal ? CA_F32_CASE(64, true, x, lds) : CA_F32_CASE(64, false, x, lds);
+  if (s.D == 128) return causal ? CA_F32_CASE(128, true, x, lds) : CA_F32_CASE(128, false, x, lds);
+#undef CA_F32_CASE
   return hipErrorInvalidValue;
 }
 

@@ -70,6 +70,49 @@ hipError_t launch_flash_bwd_f32(const float* q, const float* k, const float* v, 
                                 float* dv, int B, int Hq, int Hkv, int S, int D, float scale,
                                 bool causal, void* ws, hipStream_t stream);
 
+// Attention of encoder-decoder models: q [B, Hq, Sq, D], k and v [B, Hkv, Skv, D],
+// of which sequence b has its first kv_lens[b] keys (device; null: Skv).
+struct EncDecShape {
+  int B, Hq, Hkv, Sq, Skv, D;
+  float scale;
+  const int32_t* kv_lens;
+};
+// A relative position bias: table [buckets][Hq] on the device, and on the host
+// the first distance of each of a side's buckets (encdec.h).
+struct BiasSpec {
+  const float* table;
+  int side;
+  bool one_sided;
+  const int32_t* first;
+  int buckets() const { return one_sided ? side : 2 * side; }
+};
+// Forward (cross.hip; float32: f32.hip); bias may be null. ws holds
+// cross_workspace_bytes.
+size_t cross_workspace_bytes(int dtype, const EncDecShape& s, bool bias, bool causal, bool lse);
+hipError_t launch_cross(int dtype, const void* q, const void* k, const void* v, void* o, float* lse,
+                        const EncDecShape& s, const BiasSpec* bias, bool causal, void* ws, size_t ws_bytes,
+                        hipStream_t stream);
+hipError_t launch_cross_f32(const void* q, const void* k, const void* v, void* o, float* lse, const EncDecShape& s,
+                            const BiasSpec* bias, bool causal, hipStream_t stream);
+// Few query rows (decode.hip; without a bias Sq may pass 1; with one, Sq is 1 and
+// the query is at its last key): ws holds flash_decode_partials_bytes of Hq Sq heads.
+hipError_t launch_encdec_decode(int dtype, const void* q, const void* k, const void* v, void* o,
+                                const EncDecShape& s, const BiasSpec* bias, void* ws, size_t ws_bytes,
+                                hipStream_t stream);
+// Backward (backward.hip; float32: backward_f32.hip); dtable [buckets][Hq] with
+// a bias. ws holds cross_bwd_workspace_bytes.
+size_t cross_bwd_workspace_bytes(const EncDecShape& s, int buckets);
+hipError_t launch_cross_bwd(int dtype, const void* q, const void* k, const void* v, const void* o, const void* dout,
+                            const float* lse, void* dq, void* dk, void* dv, float* dtable, const EncDecShape& s,
+                            const BiasSpec* bias, bool causal, void* ws, hipStream_t stream);
+hipError_t launch_cross_bwd_f32(const float* q, const float* k, const float* v, const float* o, const float* dout,
+                                const float* lse, float* dq, float* dk, float* dv, float* dtable,
+                                const EncDecShape& s, const BiasSpec* bias, bool causal, float* ws,
+                                hipStream_t stream);
+// Sums the workgroups' totals part [B][Hq][n_qt][buckets] of a table's gradient.
+hipError_t launch_bias_grad(const float* part, float* dtable, int B, int Hq, int n_qt, int buckets,
+                            hipStream_t stream);
+
 // Compute units of the current device (cached per device; 0 if unknown).
 // Safe for concurrent first calls: each slot is an atomic, and every thread
 // that finds it empty stores the same attribute value.

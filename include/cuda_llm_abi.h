@@ -21,7 +21,7 @@
  *  - Element types: CA_BF16 and CA_F16 for 16-bit q/k/v/out everywhere;
  *    CA_F32 for prefill (with and without LSE), backward, RoPE prefill,
  *    flash_decode, paged and FP8 paged decode (the entry points the reference
- *    instantiates for float). paged_kv_append takes CA_BF16 / CA_F16 only, and
+ *    instantiates for float), cross attention and relative position bias. paged_kv_append takes CA_BF16 / CA_F16 only, and
  *    MXFP8 writes CA_BF16 / CA_F16 outputs.
  *  - head_dim must be 64 or 128 (fused_softmax_binding.cpp:65-67); the MXFP8
  *    entry point requires 128.
@@ -117,6 +117,86 @@ ca_status ca_fused_rope_flash_attention(ca_dtype dtype, const void* q, const voi
 /* Bytes of the ca_fused_rope_flash_attention workspace. */
 size_t ca_rope_workspace_bytes(ca_dtype dtype, int batch, int num_q_heads, int num_kv_heads,
                                int seq_len, int head_dim);
+
+/* Cross attention, no counterpart in the reference: attention of q [batch,
+ * num_q_heads, q_len, head_dim] to k, v [batch, num_kv_heads, kv_len, head_dim]
+ * of another length, as a decoder attends to an encoder's states. Sequence b
+ * has its first kv_lens[b] keys (int32 on the device, taken into [0, kv_len];
+ * NULL: kv_len each); what k and v hold past them (NaN and infinities included)
+ * is never used. A row without a key gives 0, and -inf in lse. lse (may be
+ * NULL): natural-log logsumexp [batch, num_q_heads, q_len]. Few query rows
+ * without lse go to the split walk of ca_flash_decode. softmax_scale must be
+ * finite. workspace: ca_cross_attention_workspace_bytes(...). */
+ca_status ca_cross_attention(ca_dtype dtype, const void* q, const void* k, const void* v,
+                             const int32_t* kv_lens, void* o, float* lse, int batch,
+                             int num_q_heads, int num_kv_heads, int q_len, int kv_len,
+                             int head_dim, float softmax_scale, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/* Bytes of the ca_cross_attention workspace (with_lse: lse is not NULL). */
+size_t ca_cross_attention_workspace_bytes(ca_dtype dtype, int batch, int num_q_heads,
+                                          int num_kv_heads, int q_len, int kv_len, int head_dim,
+                                          int with_lse);
+
+/* Its backward: dq, dk, dv from the forward's o and lse, as
+ * ca_flash_attention_bwd. dk and dv of the keys past kv_lens[b] are 0. */
+ca_status ca_cross_attention_bwd(ca_dtype dtype, const void* q, const void* k, const void* v,
+                                 const int32_t* kv_lens, const void* o, const void* dout,
+                                 const float* lse, void* dq, void* dk, void* dv, int batch,
+                                 int num_q_heads, int num_kv_heads, int q_len, int kv_len,
+                                 int head_dim, float softmax_scale, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+
+/* Attention with a learned relative position bias by buckets, no counterpart in
+ * the reference: as ca_cross_attention, with bias_table[bucket(j - i)][h] added
+ * to the scaled logit of query i and key j of q head h, and with is_causal the
+ * keys j > i masked. bias_table: float32 [num_buckets, num_q_heads] on the
+ * device; its finite values are taken into [-32768, 32768], -inf masks.
+ * A side has num_buckets buckets (is_causal) or num_buckets / 2, which must be
+ * even then (otherwise: keys after their query have the second half);
+ * bucket_starts, on the HOST, holds the first distance of each bucket of a
+ * side: bucket_starts[0] = 0, never falling, at most 2048; distance n = |j - i|
+ * is in the last bucket that starts at or before it. num_buckets <= 256.
+ * workspace: ca_relative_bias_attention_workspace_bytes(...). */
+ca_status ca_relative_bias_attention(ca_dtype dtype, const void* q, const void* k, const void* v,
+                                     const float* bias_table, const int32_t* bucket_starts,
+                                     int num_buckets, const int32_t* kv_lens, void* o, float* lse,
+                                     int batch, int num_q_heads, int num_kv_heads, int q_len,
+                                     int kv_len, int head_dim, float softmax_scale, int is_causal,
+                                     void* workspace, size_t workspace_bytes, void* stream);
+
+size_t ca_relative_bias_attention_workspace_bytes(ca_dtype dtype, int batch, int num_q_heads,
+                                                  int num_kv_heads, int q_len, int kv_len,
+                                                  int head_dim, int is_causal);
+
+/* Its backward; dtable: float32 [num_buckets, num_q_heads], the sums over the
+ * batch, queries and keys of each bucket's dS = P (dP - rowsum(dout o)). */
+ca_status ca_relative_bias_attention_bwd(ca_dtype dtype, const void* q, const void* k,
+                                         const void* v, const float* bias_table,
+                                         const int32_t* bucket_starts, int num_buckets,
+                                         const int32_t* kv_lens, const void* o, const void* dout,
+                                         const float* lse, void* dq, void* dk, void* dv,
+                                         float* dtable, int batch, int num_q_heads,
+                                         int num_kv_heads, int q_len, int kv_len, int head_dim,
+                                         float softmax_scale, int is_causal, void* workspace,
+                                         size_t workspace_bytes, void* stream);
+
+/* Bytes of the workspace of either backward (num_buckets 0: cross attention's):
+ * per query row the pair of ca_flash_attention_bwd, and per bucket and tile of
+ * 128 query rows a float. */
+size_t ca_encoder_decoder_bwd_workspace_bytes(int batch, int num_q_heads, int q_len,
+                                              int num_buckets);
+
+/* Its single-token form: q [batch, num_q_heads, 1, head_dim] at the position of
+ * the last of its sequence's first context_lens[b] keys (NULL: kv_len each) of a
+ * contiguous cache; buckets as with is_causal. workspace:
+ * ca_flash_decode_workspace_bytes(...). */
+ca_status ca_relative_bias_decode(ca_dtype dtype, const void* q, const void* k, const void* v,
+                                  const float* bias_table, const int32_t* bucket_starts,
+                                  int num_buckets, const int32_t* context_lens, void* o, int batch,
+                                  int num_q_heads, int num_kv_heads, int kv_len, int head_dim,
+                                  float softmax_scale, void* workspace, size_t workspace_bytes,
+                                  void* stream);
 
 /* Measurement helper, no counterpart in the reference: reads `bytes` bytes
  * (a multiple of 16, 16-byte aligned) from device memory at `p` with

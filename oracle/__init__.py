@@ -34,6 +34,13 @@ Pinning (what checks each function; see ``tests/test_oracle.py``):
                                      central finite differences of
                                      ``attention`` (fp64), the one-key closed
                                      form (dq = dk = 0, dv = dout)
+  encdec_attention / encdec_backward attention / attention_backward of the same
+                                     library at equal lengths, torch autograd
+                                     (CPU, fp64) of the written-out formula,
+                                     central differences
+  relative_bucket                    the closed form's logarithms away from
+                                     its borders, monotony, the borders that
+                                     are whole numbers
 No function is left "parity unpinned" except the MXFP8 *semantics* as a whole:
 the reference declares ``dispatch_fused_microscaled_attention``
 (kernels_api.h:103-108) but ships no kernel, binding or test for it, so the
@@ -41,6 +48,7 @@ oracle follows the OCP MX v1.0 definition instead of a reference vector.
 """
 from .attention import (apply_rope, attention, attention_backward, attention_lse,
                         attention_tiled, decode, default_scale, rope_attention, split_merge)
+from .encdec import bucket_matrix, encdec_attention, encdec_backward, relative_bucket
 from .fp8 import (E4M3_MAX, e4m3_decode, e4m3_encode, e8m0_decode,
                   mx_dequantize, mx_quantize, quantize_per_page_fp8)
 from .paged import gather_paged, make_paged_cache, paged_append, paged_decode
@@ -50,4 +58,5 @@ __all__ = [
     "split_merge", "E4M3_MAX", "e4m3_decode", "e4m3_encode", "e8m0_decode",
     "mx_dequantize", "mx_quantize", "quantize_per_page_fp8", "gather_paged",
     "make_paged_cache", "paged_append", "paged_decode",
+    "bucket_matrix", "encdec_attention", "encdec_backward", "relative_bucket",
 ]
