@@ -34,13 +34,13 @@ SIGNATURES = {
     "ca_cross_attention_workspace_bytes": (_Z, [_I, _I, _I, _I, _I, _I, _I, _I]),
     "ca_cross_attention_bwd": (_I, [_I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P,
                                     _Z, _P]),
-    "ca_relative_bias_attention": (_I, [_I, _P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I,
+    "ca_relative_bias_attention": (_I, [_I, _P, _P, _P, _P, _I, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I,
                                         _P, _Z, _P]),
     "ca_relative_bias_attention_workspace_bytes": (_Z, [_I, _I, _I, _I, _I, _I, _I, _I]),
-    "ca_relative_bias_attention_bwd": (_I, [_I, _P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I,
+    "ca_relative_bias_attention_bwd": (_I, [_I, _P, _P, _P, _P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I,
                                             _I, _I, _I, _I, _F, _I, _P, _Z, _P]),
     "ca_encoder_decoder_bwd_workspace_bytes": (_Z, [_I, _I, _I, _I]),
-    "ca_relative_bias_decode": (_I, [_I, _P, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _F, _P, _Z, _P]),
+    "ca_relative_bias_decode": (_I, [_I, _P, _P, _P, _P, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _F, _P, _Z, _P]),
     "ca_stream_read": (_I, [_P, _Z, _P, _P]),
     "ca_paged_kv_append": (_I, [_I, _I, _P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I,
                                 _I, _P]),
@@ -115,7 +115,10 @@ NATIVE_FUNCTIONS = (
     "ca_flash_attention_bwd_workspace_bytes", "ca_fused_rope_flash_attention", "ca_rope_workspace_bytes",
     "ca_flash_decode", "ca_flash_decode_workspace_bytes", "ca_paged_attention", "ca_fp8_paged_attention",
     "ca_paged_decode_workspace_bytes",
-    "ca_paged_kv_append", "ca_fused_microscaled_attention", "ca_mx_workspace_bytes")
+    "ca_paged_kv_append", "ca_fused_microscaled_attention", "ca_mx_workspace_bytes", "ca_cross_attention",
+    "ca_cross_attention_workspace_bytes", "ca_cross_attention_bwd", "ca_relative_bias_attention",
+    "ca_relative_bias_attention_workspace_bytes", "ca_relative_bias_attention_bwd",
+    "ca_encoder_decoder_bwd_workspace_bytes", "ca_relative_bias_decode")
 
 
 def native():

@@ -317,7 +317,8 @@ def _encdec_checks(q, k, v, kv_lens):
 
 @functools.lru_cache(maxsize=64)
 def _bucket_starts(num_buckets, is_causal, max_distance):
-    """First distance of each bucket of a side, as the C ABI takes them: the
+    """First distance of each bucket of a side, as the C ABI takes them, and its
+    address: the
     first half of the side's buckets hold one distance each, the others
     distances that grow as a power up to max_distance: bucket e + j starts at
     the first n with (n / e) ** span >= (max_distance / e) ** j, e buckets
@@ -339,7 +340,8 @@ def _bucket_starts(num_buckets, is_causal, max_distance):
             else:
                 lo = mid + 1
         starts.append(lo)
-    return (ctypes.c_int32 * side)(*starts)
+    starts = (ctypes.c_int32 * side)(*starts)
+    return starts, ctypes.addressof(starts)
 
 
 def _bias_checks(q, bias_table, is_causal, max_distance):
@@ -347,8 +349,16 @@ def _bias_checks(q, bias_table, is_causal, max_distance):
     _check(bias_table.dim() == 2 and bias_table.shape[1] == q.shape[1], "bias_table must be [num_buckets, num_heads]")
     _check(bias_table.dtype in _DT, "Unsupported scalar type for bias_table. Supported: Float, Float16, BFloat16.")
     _check(isinstance(max_distance, int), "max_distance must be an integer")
-    starts = _bucket_starts(bias_table.shape[0], bool(is_causal), max_distance)
-    return bias_table.detach().to(torch.float32).contiguous(), starts
+    starts, _ = _bucket_starts(bias_table.shape[0], bool(is_causal), max_distance)
+    return bias_table.detach().contiguous(), starts
+
+
+def _starts_address(bias_table, is_causal, max_distance):
+    """What the extension module takes of a bias's buckets (0: nothing, as for
+    arguments that the checks above are to refuse)."""
+    if not torch.is_tensor(bias_table) or bias_table.dim() != 2 or type(max_distance) is not int:
+        return 0
+    return _bucket_starts(bias_table.shape[0], bool(is_causal), max_distance)[1]
 
 
 def _encdec_forward(q, k, v, kv_lens, softmax_scale, want_lse, bias=None, is_causal=False):
@@ -371,8 +381,8 @@ def _encdec_forward(q, k, v, kv_lens, softmax_scale, want_lse, bias=None, is_cau
         else:
             nbytes = lib.ca_relative_bias_attention_workspace_bytes(dt, b, hq, hkv, sq, skv, d, int(bool(is_causal)))
             ws, nbytes = _workspace(nbytes, q.device)
-            _lib.call("ca_relative_bias_attention", dt, _ptr(q), _ptr(k), _ptr(v), _ptr(table), starts,
-                      table.shape[0], _ptr(lens), _ptr(out), _ptr(lse), b, hq, hkv, sq, skv, d,
+            _lib.call("ca_relative_bias_attention", dt, _ptr(q), _ptr(k), _ptr(v), _ptr(table),
+                      _DT[table.dtype], starts, table.shape[0], _ptr(lens), _ptr(out), _ptr(lse), b, hq, hkv, sq, skv, d,
                       _scale(softmax_scale, d), int(bool(is_causal)), _ptr(ws), nbytes, _stream())
     return out, lse
 
@@ -401,10 +411,11 @@ def _encdec_backward(dout, q, k, v, out, lse, kv_lens, softmax_scale, bias=None,
                       _ptr(ws), nbytes, _stream())
             return [dq, dk, dv]
         dtable = torch.empty_like(table)
-        _lib.call("ca_relative_bias_attention_bwd", dt, _ptr(q), _ptr(k), _ptr(v), _ptr(table), starts, n_buckets,
+        _lib.call("ca_relative_bias_attention_bwd", dt, _ptr(q), _ptr(k), _ptr(v), _ptr(table),
+                  _DT[table.dtype], starts, n_buckets,
                   _ptr(lens), _ptr(out), _ptr(dout), _ptr(lse), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dtable), b, hq,
                   hkv, sq, skv, d, _scale(softmax_scale, d), int(bool(is_causal)), _ptr(ws), nbytes, _stream())
-    return [dq, dk, dv, dtable.to(bias[0].dtype)]
+    return [dq, dk, dv, dtable]
 
 
 def cross_attention_forward(q, k, v, kv_lens=None, softmax_scale=None):
@@ -414,12 +425,18 @@ def cross_attention_forward(q, k, v, kv_lens=None, softmax_scale=None):
     [B] on the device, taken into [0, Skv]; None: all). What k and v hold past
     them is never used; a sequence without a key gives zeros. Any Sq from a
     single token on; fp16 / bf16 / float32. No reference counterpart."""
+    out = _native().cross_attention_forward(q, k, v, kv_lens, softmax_scale)
+    if out is not None:
+        return out
     return _encdec_forward(q, k, v, kv_lens, softmax_scale, False)[0]
 
 
 def cross_attention_forward_lse(q, k, v, kv_lens=None, softmax_scale=None):
     """(O, LSE): cross_attention_forward and the natural-log logsumexp of every
     row's scaled logits, [B, Hq, Sq] float32 (-inf for a row without a key)."""
+    res = _native().cross_attention_forward_lse(q, k, v, kv_lens, softmax_scale)
+    if res is not None:
+        return res
     return _encdec_forward(q, k, v, kv_lens, softmax_scale, True)
 
 
@@ -427,6 +444,9 @@ def cross_attention_backward(dout, q, k, v, out, lse, kv_lens=None, softmax_scal
     """[dq, dk, dv] of cross_attention_forward, given its output, the gradient of
     it and its LSE (as flash_attention_backward). dk and dv of a sequence's keys
     past kv_lens are zeros."""
+    res = _native().cross_attention_backward(dout, q, k, v, out, lse, kv_lens, softmax_scale)
+    if res is not None:
+        return res
     return _encdec_backward(dout, q, k, v, out, lse, kv_lens, softmax_scale)
 
 
@@ -469,6 +489,10 @@ def relative_bias_attention_forward(q, k, v, bias_table, kv_lens=None, is_causal
     (from 0 on), the other half distances that grow as a power up to
     max_distance (at most 2048); what lies beyond is in the last one. No
     reference counterpart."""
+    out = _native().relative_bias_attention_forward(q, k, v, bias_table, kv_lens, is_causal, softmax_scale,
+                                                    _starts_address(bias_table, is_causal, max_distance))
+    if out is not None:
+        return out
     return _encdec_forward(q, k, v, kv_lens, softmax_scale, False, (bias_table, max_distance), is_causal)[0]
 
 
@@ -476,6 +500,10 @@ def relative_bias_attention_forward_lse(q, k, v, bias_table, kv_lens=None, is_ca
                                         max_distance=128):
     """(O, LSE): relative_bias_attention_forward and the natural-log logsumexp of
     every row's biased logits, [B, Hq, Sq] float32."""
+    res = _native().relative_bias_attention_forward_lse(q, k, v, bias_table, kv_lens, is_causal, softmax_scale,
+                                                        _starts_address(bias_table, is_causal, max_distance))
+    if res is not None:
+        return res
     return _encdec_forward(q, k, v, kv_lens, softmax_scale, True, (bias_table, max_distance), is_causal)
 
 
@@ -484,6 +512,11 @@ def relative_bias_attention_backward(dout, q, k, v, out, lse, bias_table, kv_len
     """[dq, dk, dv, dtable] of relative_bias_attention_forward, given its output,
     the gradient of it and its LSE. dtable, of bias_table's type, is summed over
     the batch in an order that does not depend on timing."""
+    res = _native().relative_bias_attention_backward(dout, q, k, v, out, lse, bias_table, kv_lens, is_causal,
+                                                     softmax_scale,
+                                                     _starts_address(bias_table, is_causal, max_distance))
+    if res is not None:
+        return res
     return _encdec_backward(dout, q, k, v, out, lse, kv_lens, softmax_scale, (bias_table, max_distance), is_causal)
 
 
@@ -518,6 +551,10 @@ def relative_bias_decode(q, k, v, bias_table, context_lens=None, softmax_scale=N
     against a contiguous cache k, v [B, Hkv, S, D], the token of sequence b at
     the position of the last of its first ``context_lens[b]`` keys (None: S), its
     own among them. What the cache holds past them is never used."""
+    out = _native().relative_bias_decode(q, k, v, bias_table, context_lens, softmax_scale,
+                                         _starts_address(bias_table, True, max_distance))
+    if out is not None:
+        return out
     b, hq, hkv, sq, skv, d, lens = _encdec_checks(q, k, v, context_lens)
     _check(sq == 1, "Query sequence length must be 1 for relative_bias_decode")
     dt = _dtype_code(q, "Relative Bias Decode")
@@ -526,7 +563,7 @@ def relative_bias_decode(q, k, v, bias_table, context_lens=None, softmax_scale=N
         q, k, v = _aligned(q), _aligned(k), _aligned(v)
         out = torch.empty_like(q)
         ws, nbytes = _workspace(_lib.load().ca_flash_decode_workspace_bytes(dt, b, hq, hkv, skv, d), q.device)
-        _lib.call("ca_relative_bias_decode", dt, _ptr(q), _ptr(k), _ptr(v), _ptr(table), starts, table.shape[0],
+        _lib.call("ca_relative_bias_decode", dt, _ptr(q), _ptr(k), _ptr(v), _ptr(table), _DT[table.dtype], starts, table.shape[0],
                   _ptr(lens), _ptr(out), b, hq, hkv, skv, d, _scale(softmax_scale, d), _ptr(ws), nbytes, _stream())
     return out
 

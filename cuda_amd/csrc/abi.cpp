@@ -227,18 +227,20 @@ static ca_status encdec_shape(const char* what, ca_dtype dtype, int batch, int h
   return CA_OK;
 }
 
-static ca_status bias_spec(const char* what, const float* table, const int32_t* starts, int num_buckets,
+static ca_status bias_spec(const char* what, const void* table, ca_dtype table_dtype, const int32_t* starts, int num_buckets,
                            bool one_sided, ca::BiasSpec* b) {
   if (num_buckets < 1 || num_buckets > 256 || (!one_sided && num_buckets % 2))
     return fail(CA_INVALID_ARGUMENT, "%s: num_buckets must be in [1, 256], and even when not causal (got %d)", what,
                 num_buckets);
+  if (table_dtype != CA_F32 && table_dtype != CA_F16 && table_dtype != CA_BF16)
+    return fail(CA_INVALID_ARGUMENT, "%s: unknown dtype %d of the bias table", what, (int)table_dtype);
   if (!table || !starts) return fail(CA_INVALID_ARGUMENT, "%s: null bias table or bucket starts", what);
   const int side = one_sided ? num_buckets : num_buckets / 2;
   if (starts[0] != 0) return fail(CA_INVALID_ARGUMENT, "%s: bucket_starts must begin with 0", what);
   for (int i = 1; i < side; ++i)
     if (starts[i] < starts[i - 1] || starts[i] > 2048)
       return fail(CA_INVALID_ARGUMENT, "%s: bucket_starts must not fall, and stay within 2048", what);
-  *b = ca::BiasSpec{table, side, one_sided, starts};
+  *b = ca::BiasSpec{table, (int)table_dtype, side, one_sided, starts};
   return CA_OK;
 }
 
@@ -303,7 +305,7 @@ static ca_status encdec_forward(const char* what, ca_dtype dtype, const void* q,
 
 static ca_status encdec_backward(const char* what, ca_dtype dtype, const void* q, const void* k, const void* v,
                                  const void* o, const void* dout, const float* lse, void* dq, void* dk, void* dv,
-                                 float* dtable, const ca::EncDecShape& s, const ca::BiasSpec* bias, bool causal,
+                                 void* dtable, const ca::EncDecShape& s, const ca::BiasSpec* bias, bool causal,
                                  void* workspace, size_t workspace_bytes, void* stream) {
   ca_status st;
   const bool rows = s.B > 0 && s.Sq > 0, keys = s.B > 0 && s.Skv > 0;
@@ -344,7 +346,7 @@ ca_status ca_cross_attention_bwd(ca_dtype dtype, const void* q, const void* k, c
 }
 
 ca_status ca_relative_bias_attention(ca_dtype dtype, const void* q, const void* k, const void* v,
-                                     const float* bias_table, const int32_t* bucket_starts, int num_buckets,
+                                     const void* bias_table, ca_dtype table_dtype, const int32_t* bucket_starts, int num_buckets,
                                      const int32_t* kv_lens, void* o, float* lse, int batch, int num_q_heads,
                                      int num_kv_heads, int q_len, int kv_len, int head_dim, float softmax_scale,
                                      int is_causal, void* workspace, size_t workspace_bytes, void* stream) {
@@ -354,14 +356,14 @@ ca_status ca_relative_bias_attention(ca_dtype dtype, const void* q, const void* 
   ca_status st = encdec_shape(what, dtype, batch, num_q_heads, num_kv_heads, q_len, kv_len, head_dim, softmax_scale,
                               kv_lens, &s);
   if (st != CA_OK) return st;
-  if ((st = bias_spec(what, bias_table, bucket_starts, num_buckets, is_causal != 0, &b)) != CA_OK) return st;
+  if ((st = bias_spec(what, bias_table, table_dtype, bucket_starts, num_buckets, is_causal != 0, &b)) != CA_OK) return st;
   return encdec_forward(what, dtype, q, k, v, o, lse, s, &b, is_causal != 0, workspace, workspace_bytes, stream);
 }
 
 ca_status ca_relative_bias_attention_bwd(ca_dtype dtype, const void* q, const void* k, const void* v,
-                                         const float* bias_table, const int32_t* bucket_starts, int num_buckets,
+                                         const void* bias_table, ca_dtype table_dtype, const int32_t* bucket_starts, int num_buckets,
                                          const int32_t* kv_lens, const void* o, const void* dout, const float* lse,
-                                         void* dq, void* dk, void* dv, float* dtable, int batch, int num_q_heads,
+                                         void* dq, void* dk, void* dv, void* dtable, int batch, int num_q_heads,
                                          int num_kv_heads, int q_len, int kv_len, int head_dim, float softmax_scale,
                                          int is_causal, void* workspace, size_t workspace_bytes, void* stream) {
   const char* what = "relative_bias_attention_backward";
@@ -370,12 +372,13 @@ ca_status ca_relative_bias_attention_bwd(ca_dtype dtype, const void* q, const vo
   ca_status st = encdec_shape(what, dtype, batch, num_q_heads, num_kv_heads, q_len, kv_len, head_dim, softmax_scale,
                               kv_lens, &s);
   if (st != CA_OK) return st;
-  if ((st = bias_spec(what, bias_table, bucket_starts, num_buckets, is_causal != 0, &b)) != CA_OK) return st;
+  if ((st = bias_spec(what, bias_table, table_dtype, bucket_starts, num_buckets, is_causal != 0, &b)) != CA_OK) return st;
   return encdec_backward(what, dtype, q, k, v, o, dout, lse, dq, dk, dv, dtable, s, &b, is_causal != 0, workspace,
                          workspace_bytes, stream);
 }
 
-ca_status ca_relative_bias_decode(ca_dtype dtype, const void* q, const void* k, const void* v, const float* bias_table,
+ca_status ca_relative_bias_decode(ca_dtype dtype, const void* q, const void* k, const void* v, const void* bias_table,
+                                  ca_dtype table_dtype,
                                   const int32_t* bucket_starts, int num_buckets, const int32_t* context_lens, void* o,
                                   int batch, int num_q_heads, int num_kv_heads, int kv_len, int head_dim,
                                   float softmax_scale, void* workspace, size_t workspace_bytes, void* stream) {
@@ -385,7 +388,7 @@ ca_status ca_relative_bias_decode(ca_dtype dtype, const void* q, const void* k, 
   ca_status st = encdec_shape(what, dtype, batch, num_q_heads, num_kv_heads, 1, kv_len, head_dim, softmax_scale,
                               context_lens, &s);
   if (st != CA_OK) return st;
-  if ((st = bias_spec(what, bias_table, bucket_starts, num_buckets, true, &b)) != CA_OK) return st;
+  if ((st = bias_spec(what, bias_table, table_dtype, bucket_starts, num_buckets, true, &b)) != CA_OK) return st;
   if (batch == 0) return CA_OK;
   if ((st = check_pointers(what, {q, o}, true)) != CA_OK) return st;
   if ((st = check_pointers(what, {k, v}, kv_len > 0)) != CA_OK) return st;

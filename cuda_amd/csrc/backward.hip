@@ -879,7 +879,7 @@ struct BwdX {
   int Skv;
   size_t dkv_lds = 0, dq_lds = 0;  // dynamic
   float* part_table = nullptr;
-  float* dtable = nullptr;
+  void* dtable = nullptr;
 };
 
 template <typename Tr, int D, bool CAUSAL, class X>
@@ -922,15 +922,16 @@ hipError_t launch_bwd_t(const void* q, const void* k, const void* v, const void*
     if (e != hipSuccess) return e;
   }
   if constexpr (X::kBias)
-    return launch_bias_grad(bx.part_table, bx.dtable, B, Hq, sq.n_tiles, bx.x.one_sided ? bx.x.side : 2 * bx.x.side,
+    return launch_bias_grad(bx.part_table, bx.dtable, bx.x.table_dtype, B, Hq, sq.n_tiles, bx.x.one_sided ? bx.x.side : 2 * bx.x.side,
                             stream);
   return e;
 }
 
 // dtable[bucket][h] = the sum over sequences and tiles of part [B][Hq][n_qt]
 // [buckets]: a wave per entry, its lanes' terms in a fixed order, in 64 bits
-// (terms of both signs that nearly cancel).
-__global__ __launch_bounds__(64) void bias_grad_kernel(const float* __restrict__ part, float* __restrict__ dtable,
+// (terms of both signs that nearly cancel), rounded once to the table's type.
+template <typename Tr>
+__global__ __launch_bounds__(64) void bias_grad_kernel(const float* __restrict__ part, void* __restrict__ dtable,
                                                        int B, int Hq, int n_qt, int buckets) {
   const int lane = threadIdx.x, bucket = blockIdx.x / Hq, h = blockIdx.x % Hq;
   double t = 0.;
@@ -940,19 +941,22 @@ __global__ __launch_bounds__(64) void bias_grad_kernel(const float* __restrict__
   }
 #pragma unroll
   for (int m = 32; m >= 1; m >>= 1) t += __shfl_xor(t, m, 64);
-  if (lane == 0) dtable[blockIdx.x] = (float)t;
+  if (lane == 0) Tr::store(dtable, blockIdx.x, (float)t);
 }
 
 }  // namespace
 
 size_t bwd_workspace_bytes(int B, int Hq, int S) { return (size_t)B * Hq * S * 2 * sizeof(float); }
 
-hipError_t launch_bias_grad(const float* part, float* dtable, int B, int Hq, int n_qt, int buckets,
+hipError_t launch_bias_grad(const float* part, void* dtable, int dtype, int B, int Hq, int n_qt, int buckets,
                             hipStream_t stream) {
   const long long grid = (long long)Hq * buckets;
   if (grid > 0x7fffffffLL / 64) return hipErrorInvalidValue;
   if (grid == 0) return hipSuccess;
-  hipLaunchKernelGGL(bias_grad_kernel, dim3((unsigned)grid), dim3(64), 0, stream, part, dtable, B, Hq, n_qt, buckets);
+  const auto kernel = dtype == kDtypeF32    ? &bias_grad_kernel<F32>
+                      : dtype == kDtypeBF16 ? &bias_grad_kernel<BF16>
+                                            : &bias_grad_kernel<F16>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64), 0, stream, part, dtable, B, Hq, n_qt, buckets);
   return hipGetLastError();
 }
 
@@ -993,7 +997,7 @@ size_t cross_bwd_workspace_bytes(const EncDecShape& s, int buckets) {
 }
 
 hipError_t launch_cross_bwd(int dtype, const void* q, const void* k, const void* v, const void* o, const void* dout,
-                            const float* lse, void* dq, void* dk, void* dv, float* dtable, const EncDecShape& s,
+                            const float* lse, void* dq, void* dk, void* dv, void* dtable, const EncDecShape& s,
                             const BiasSpec* bias, bool causal, void* ws, hipStream_t stream) {
   float* w = (float*)ws;
   if (dtype == kDtypeF32)

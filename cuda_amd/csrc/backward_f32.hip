@@ -474,7 +474,7 @@ hipError_t launch_flash_bwd_f32(const float* q, const float* k, const float* v, 
 }
 
 hipError_t launch_cross_bwd_f32(const float* q, const float* k, const float* v, const float* o, const float* dout,
-                                const float* lse, float* dq, float* dk, float* dv, float* dtable,
+                                const float* lse, float* dq, float* dk, float* dv, void* dtable,
                                 const EncDecShape& s, const BiasSpec* bias, bool causal, float* ws,
                                 hipStream_t stream) {
 #define CA_BWD32(DD, CAUSAL, X, DKV, DQ, PART)                                                               \
@@ -497,7 +497,7 @@ hipError_t launch_cross_bwd_f32(const float* q, const float* k, const float* v, 
   if (s.D == 128) e = causal ? CA_BWD32(128, true, x, dkv, dqb, part) : CA_BWD32(128, false, x, dkv, dqb, part);
 #undef CA_BWD32
   if (e != hipSuccess) return e;
-  return launch_bias_grad(part, dtable, s.B, s.Hq, (s.Sq + 32 * kF32Waves - 1) / (32 * kF32Waves), bias->buckets(),
+  return launch_bias_grad(part, dtable, bias->table_dtype, s.B, s.Hq, (s.Sq + 32 * kF32Waves - 1) / (32 * kF32Waves), bias->buckets(),
                           stream);
 }
 

@@ -1265,9 +1265,9 @@ __global__ __launch_bounds__(64) void decode_f32_kernel(
         }
       }
       if constexpr (X::kBias) {
-        const float* col = x.table + (size_t)bias_bucket(x, first, tc - (L - 1)) * x.Hq + hq0;
+        const int bucket = bias_bucket(x, first, tc - (L - 1));
 #pragma unroll
-        for (int g = 0; g < G; ++g) s[g] += bias_clamp(col[min(g, Gc - 1)]) * x.mul;
+        for (int g = 0; g < G; ++g) s[g] += x.value(bucket, hq0 + min(g, Gc - 1));
       }
     }
 #pragma unroll

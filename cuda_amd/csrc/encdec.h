@@ -48,7 +48,8 @@ struct CrossX {
 
 struct BiasX : CrossX {
   static constexpr bool kBias = true;
-  const float* table;  // [buckets][Hq]
+  const void* table;   // [buckets][Hq] of table_dtype
+  int table_dtype;     // kDtypeF32, ...
   float mul;           // table values times this are the kernel's
   float scale_log2;    // ... which, times this, are log2 logits
   int side;            // buckets of a side
@@ -56,6 +57,7 @@ struct BiasX : CrossX {
   int reach;           // distances from here on are in a side's last bucket
   int Hq;
   uint16_t first[kMaxBuckets];  // first distance of a side's bucket
+  __device__ __forceinline__ float value(int bucket, int h) const;
 };
 
 // ---------------------------------------------------------------------------
@@ -81,6 +83,16 @@ __device__ __forceinline__ float bias_clamp(float v) {
   return v < -kMaxBias && v != kNegInf ? -kMaxBias : v;
 }
 
+// The kernel's bias of a bucket: clamped, times mul.
+__device__ __forceinline__ float BiasX::value(int bucket, int h) const {
+  const size_t i = (size_t)bucket * Hq + h;
+  float v;
+  if (table_dtype == kDtypeF32) v = ((const float*)table)[i];
+  else if (table_dtype == kDtypeBF16) v = BF16::to_float(((const uint16_t*)table)[i]);
+  else v = F16::to_float(((const uint16_t*)table)[i]);
+  return bias_clamp(v) * mul;
+}
+
 // Fills the workgroup's bias of head h at `mem` (all threads; ends with a
 // barrier). Returns the LDS byte offset of distance 0's entry.
 __device__ __forceinline__ uint32_t bias_fill(const BiasX& x, int h, unsigned char* mem, int threads) {
@@ -91,7 +103,7 @@ __device__ __forceinline__ uint32_t bias_fill(const BiasX& x, int h, unsigned ch
   __syncthreads();
   const int zero = x.reach + kBiasMargin;
   for (int i = tid; i < bias_entries(x.reach); i += threads)
-    e[i] = bias_clamp(x.table[(size_t)bias_bucket(x, first, i - zero) * x.Hq + h]) * x.mul;
+    e[i] = x.value(bias_bucket(x, first, i - zero), h);
   __syncthreads();
   return lds_off(e + zero);
 }
@@ -154,7 +166,7 @@ __device__ __forceinline__ DecodeBias decode_bias_fill(const BiasX& x, int h0, i
   const int tid = threadIdx.x;
   for (int i = tid; i < x.side; i += threads) first[i] = x.first[i];
   for (int i = tid; i < 16 * x.side; i += threads)
-    col[i] = (i & 15) < n_heads ? bias_clamp(x.table[(size_t)(i >> 4) * x.Hq + h0 + (i & 15)]) * x.mul : 0.f;
+    col[i] = (i & 15) < n_heads ? x.value(i >> 4, h0 + (i & 15)) : 0.f;
   __syncthreads();
   for (int i = tid; i <= x.reach; i += threads) ids[i] = (unsigned char)bias_bucket(x, first, -i);
   __syncthreads();
@@ -293,6 +305,7 @@ inline BiasX bias_x(const EncDecShape& s, const BiasSpec& spec, float eff, float
   x.kv_lens = s.kv_lens;
   x.Skv = s.Skv;
   x.table = spec.table;
+  x.table_dtype = spec.table_dtype;
   x.mul = mul;
   x.scale_log2 = eff * kLog2e;
   x.side = spec.side;

@@ -77,10 +77,11 @@ struct EncDecShape {
   float scale;
   const int32_t* kv_lens;
 };
-// A relative position bias: table [buckets][Hq] on the device, and on the host
-// the first distance of each of a side's buckets (encdec.h).
+// A relative position bias: table [buckets][Hq] on the device, of table_dtype, and
+// on the host the first distance of each of a side's buckets (encdec.h).
 struct BiasSpec {
-  const float* table;
+  const void* table;
+  int table_dtype;
   int side;
   bool one_sided;
   const int32_t* first;
@@ -99,18 +100,18 @@ hipError_t launch_cross_f32(const void* q, const void* k, const void* v, void* o
 hipError_t launch_encdec_decode(int dtype, const void* q, const void* k, const void* v, void* o,
                                 const EncDecShape& s, const BiasSpec* bias, void* ws, size_t ws_bytes,
                                 hipStream_t stream);
-// Backward (backward.hip; float32: backward_f32.hip); dtable [buckets][Hq] with
-// a bias. ws holds cross_bwd_workspace_bytes.
+// Backward (backward.hip; float32: backward_f32.hip); with a bias dtable [buckets]
+// [Hq] of the table's type. ws holds cross_bwd_workspace_bytes.
 size_t cross_bwd_workspace_bytes(const EncDecShape& s, int buckets);
 hipError_t launch_cross_bwd(int dtype, const void* q, const void* k, const void* v, const void* o, const void* dout,
-                            const float* lse, void* dq, void* dk, void* dv, float* dtable, const EncDecShape& s,
+                            const float* lse, void* dq, void* dk, void* dv, void* dtable, const EncDecShape& s,
                             const BiasSpec* bias, bool causal, void* ws, hipStream_t stream);
 hipError_t launch_cross_bwd_f32(const float* q, const float* k, const float* v, const float* o, const float* dout,
-                                const float* lse, float* dq, float* dk, float* dv, float* dtable,
+                                const float* lse, float* dq, float* dk, float* dv, void* dtable,
                                 const EncDecShape& s, const BiasSpec* bias, bool causal, float* ws,
                                 hipStream_t stream);
 // Sums the workgroups' totals part [B][Hq][n_qt][buckets] of a table's gradient.
-hipError_t launch_bias_grad(const float* part, float* dtable, int B, int Hq, int n_qt, int buckets,
+hipError_t launch_bias_grad(const float* part, void* dtable, int dtype, int B, int Hq, int n_qt, int buckets,
                             hipStream_t stream);
 
 // Compute units of the current device (cached per device; 0 if unknown).

@@ -43,6 +43,14 @@ struct Abi {
   decltype(&ca_paged_kv_append) paged_kv_append;
   decltype(&ca_fused_microscaled_attention) fused_microscaled_attention;
   decltype(&ca_mx_workspace_bytes) mx_workspace_bytes;
+  decltype(&ca_cross_attention) cross_attention;
+  decltype(&ca_cross_attention_workspace_bytes) cross_attention_workspace_bytes;
+  decltype(&ca_cross_attention_bwd) cross_attention_bwd;
+  decltype(&ca_relative_bias_attention) relative_bias_attention;
+  decltype(&ca_relative_bias_attention_workspace_bytes) relative_bias_attention_workspace_bytes;
+  decltype(&ca_relative_bias_attention_bwd) relative_bias_attention_bwd;
+  decltype(&ca_encoder_decoder_bwd_workspace_bytes) encoder_decoder_bwd_workspace_bytes;
+  decltype(&ca_relative_bias_decode) relative_bias_decode;
 } abi;
 
 bool type_code(at::ScalarType t, ca_dtype* out) {
@@ -345,6 +353,153 @@ PyObject* fused_microscaled_attention(PyObject* const* a) {
   return THPVariable_Wrap(o);
 }
 
+// q, k, v and the lengths of an encoder-decoder call, on the current device
+struct EncDec {
+  const at::Tensor *q, *k, *v, *lens;
+  ca_dtype dt;
+  float scale;
+  bool take(PyObject* qo, PyObject* ko, PyObject* vo, PyObject* lo, PyObject* so) {
+    lens = nullptr;
+    if (!(q = plain(qo, 4)) || !(k = plain(ko, 4)) || !(v = plain(vo, 4)) || k->sizes() != v->sizes() ||
+        q->scalar_type() != k->scalar_type() || q->scalar_type() != v->scalar_type() ||
+        !type_code(q->scalar_type(), &dt) || !fits(*q) || !fits(*k) || k->size(0) != q->size(0) ||
+        k->size(3) != q->size(3) || k->size(1) < 1 || q->size(1) < 1 || q->size(1) % k->size(1) ||
+        (q->size(3) != 64 && q->size(3) != 128) || !scale_of(so, n(*q, 3), &scale) || !here(*q) || !here(*k) ||
+        !here(*v))
+      return false;
+    if (lo == Py_None) return true;
+    lens = plain(lo, 1, 4);
+    return lens && lens->scalar_type() == at::kInt && lens->size(0) == q->size(0) && here(*lens);
+  }
+  static bool here(const at::Tensor& t) { return t.device().index() == c10::hip::current_device(); }
+  const int32_t* kv_lens() const { return lens ? (const int32_t*)in(*lens) : nullptr; }
+  at::Tensor lse() const {
+    return at::empty({q->size(0), q->size(1), q->size(2)}, q->options().dtype(at::kFloat).requires_grad(false));
+  }
+  // dout, out, lse of a backward call
+  bool backward(PyObject* go, PyObject* oo, PyObject* lo, const at::Tensor*& g, const at::Tensor*& o,
+                const at::Tensor*& l) const {
+    return (g = plain(go, 4)) && (o = plain(oo, 4)) && (l = plain(lo, 3, 4)) && g->sizes() == q->sizes() &&
+           o->sizes() == q->sizes() && g->scalar_type() == q->scalar_type() && o->scalar_type() == q->scalar_type() &&
+           l->scalar_type() == at::kFloat && l->sizes() == q->sizes().slice(0, 3) && here(*g) && here(*o) && here(*l);
+  }
+};
+
+PyObject* cross_forward(PyObject* const* a, bool want_lse) {
+  EncDec x;
+  if (!x.take(a[0], a[1], a[2], a[3], a[4])) return nullptr;
+  const at::Tensor &q = *x.q, &k = *x.k, o = like(q);
+  at::Tensor lse;
+  if (want_lse) lse = x.lse();
+  const Workspace ws(abi.cross_attention_workspace_bytes(x.dt, n(q, 0), n(q, 1), n(k, 1), n(q, 2), n(k, 2), n(q, 3),
+                                                         want_lse), q);
+  if (!ok([&] {
+        return abi.cross_attention(x.dt, in(q), in(k), in(*x.v), x.kv_lens(), out(o), want_lse ? (float*)out(lse) : nullptr,
+                                   n(q, 0), n(q, 1), n(k, 1), n(q, 2), n(k, 2), n(q, 3), x.scale, ws.ptr(), ws.bytes,
+                                   stream());
+      }))
+    return nullptr;
+  if (!want_lse) return THPVariable_Wrap(o);
+  return Py_BuildValue("(NN)", THPVariable_Wrap(o), THPVariable_Wrap(lse));
+}
+// (q, k, v, kv_lens, softmax_scale) -> out or (out, lse)
+PyObject* cross_attention_forward(PyObject* const* a) { return cross_forward(a, false); }
+PyObject* cross_attention_forward_lse(PyObject* const* a) { return cross_forward(a, true); }
+
+// (dout, q, k, v, out, lse, kv_lens, softmax_scale) -> [dq, dk, dv]
+PyObject* cross_attention_backward(PyObject* const* a) {
+  EncDec x;
+  const at::Tensor *g, *o, *l;
+  if (!x.take(a[1], a[2], a[3], a[6], a[7]) || !x.backward(a[0], a[4], a[5], g, o, l)) return nullptr;
+  const at::Tensor &q = *x.q, &k = *x.k, dq = like(q), dk = like(k), dv = like(*x.v);
+  const Workspace ws(abi.encoder_decoder_bwd_workspace_bytes(n(q, 0), n(q, 1), n(q, 2), 0), q);
+  if (!ok([&] {
+        return abi.cross_attention_bwd(x.dt, in(q), in(k), in(*x.v), x.kv_lens(), in(*o), in(*g), (const float*)in(*l),
+                                       out(dq), out(dk), out(dv), n(q, 0), n(q, 1), n(k, 1), n(q, 2), n(k, 2), n(q, 3),
+                                       x.scale, ws.ptr(), ws.bytes, stream());
+      }))
+    return nullptr;
+  return Py_BuildValue("[NNN]", THPVariable_Wrap(dq), THPVariable_Wrap(dk), THPVariable_Wrap(dv));
+}
+
+// a bias table for q's heads and the address of its bucket starts
+bool bias_of(PyObject* to, PyObject* address, const at::Tensor& q, const at::Tensor*& t, ca_dtype* dt,
+             const int32_t** starts) {
+  if (!(t = plain(to, 2, 4)) || t->size(1) != q.size(1) || t->size(0) < 1 || t->size(0) > 256 ||
+      !type_code(t->scalar_type(), dt) || !EncDec::here(*t) || !PyLong_CheckExact(address))
+    return false;
+  *starts = (const int32_t*)PyLong_AsVoidPtr(address);
+  return *starts != nullptr;
+}
+
+PyObject* bias_forward(PyObject* const* a, bool want_lse) {
+  EncDec x;
+  const at::Tensor* t;
+  ca_dtype tdt;
+  const int32_t* starts;
+  int causal;
+  if (!x.take(a[0], a[1], a[2], a[4], a[6]) || !bias_of(a[3], a[7], *x.q, t, &tdt, &starts) || !flag_of(a[5], &causal))
+    return nullptr;
+  const at::Tensor &q = *x.q, &k = *x.k, o = like(q);
+  at::Tensor lse;
+  if (want_lse) lse = x.lse();
+  const Workspace ws(abi.relative_bias_attention_workspace_bytes(x.dt, n(q, 0), n(q, 1), n(k, 1), n(q, 2), n(k, 2),
+                                                                 n(q, 3), causal), q);
+  if (!ok([&] {
+        return abi.relative_bias_attention(x.dt, in(q), in(k), in(*x.v), in(*t), tdt, starts, n(*t, 0), x.kv_lens(),
+                                           out(o), want_lse ? (float*)out(lse) : nullptr, n(q, 0), n(q, 1), n(k, 1),
+                                           n(q, 2), n(k, 2), n(q, 3), x.scale, causal, ws.ptr(), ws.bytes, stream());
+      }))
+    return nullptr;
+  if (!want_lse) return THPVariable_Wrap(o);
+  return Py_BuildValue("(NN)", THPVariable_Wrap(o), THPVariable_Wrap(lse));
+}
+// (q, k, v, bias_table, kv_lens, is_causal, softmax_scale, address of the bucket starts) -> out or (out, lse)
+PyObject* relative_bias_attention_forward(PyObject* const* a) { return bias_forward(a, false); }
+PyObject* relative_bias_attention_forward_lse(PyObject* const* a) { return bias_forward(a, true); }
+
+// (dout, q, k, v, out, lse, bias_table, kv_lens, is_causal, softmax_scale, address) -> [dq, dk, dv, dtable]
+PyObject* relative_bias_attention_backward(PyObject* const* a) {
+  EncDec x;
+  const at::Tensor *g, *o, *l, *t;
+  ca_dtype tdt;
+  const int32_t* starts;
+  int causal;
+  if (!x.take(a[1], a[2], a[3], a[7], a[9]) || !x.backward(a[0], a[4], a[5], g, o, l) ||
+      !bias_of(a[6], a[10], *x.q, t, &tdt, &starts) || !flag_of(a[8], &causal))
+    return nullptr;
+  const at::Tensor &q = *x.q, &k = *x.k, dq = like(q), dk = like(k), dv = like(*x.v), dt = like(*t);
+  const Workspace ws(abi.encoder_decoder_bwd_workspace_bytes(n(q, 0), n(q, 1), n(q, 2), n(*t, 0)), q);
+  if (!ok([&] {
+        return abi.relative_bias_attention_bwd(x.dt, in(q), in(k), in(*x.v), in(*t), tdt, starts, n(*t, 0), x.kv_lens(),
+                                               in(*o), in(*g), (const float*)in(*l), out(dq), out(dk), out(dv), out(dt),
+                                               n(q, 0), n(q, 1), n(k, 1), n(q, 2), n(k, 2), n(q, 3), x.scale, causal,
+                                               ws.ptr(), ws.bytes, stream());
+      }))
+    return nullptr;
+  return Py_BuildValue("[NNNN]", THPVariable_Wrap(dq), THPVariable_Wrap(dk), THPVariable_Wrap(dv),
+                       THPVariable_Wrap(dt));
+}
+
+// (q, k, v, bias_table, context_lens, softmax_scale, address of the bucket starts) -> out
+PyObject* relative_bias_decode(PyObject* const* a) {
+  EncDec x;
+  const at::Tensor* t;
+  ca_dtype tdt;
+  const int32_t* starts;
+  if (!x.take(a[0], a[1], a[2], a[4], a[5]) || x.q->size(2) != 1 || !bias_of(a[3], a[6], *x.q, t, &tdt, &starts))
+    return nullptr;
+  const at::Tensor &q = *x.q, &k = *x.k, o = like(q);
+  const Workspace ws(abi.flash_decode_workspace_bytes(x.dt, n(q, 0), n(q, 1), n(k, 1), n(k, 2), n(q, 3)), q);
+  if (!ok([&] {
+        return abi.relative_bias_decode(x.dt, in(q), in(k), in(*x.v), in(*t), tdt, starts, n(*t, 0), x.kv_lens(), out(o),
+                                        n(q, 0), n(q, 1), n(k, 1), n(k, 2), n(q, 3), x.scale, ws.ptr(), ws.bytes,
+                                        stream());
+      }))
+    return nullptr;
+  return THPVariable_Wrap(o);
+}
+
 // A function of exactly N arguments; anything it does not take, and any C++
 // exception (an allocation that fails, say), is None.
 template <PyObject* (*F)(PyObject* const*), int N>
@@ -387,6 +542,13 @@ PyMethodDef methods[] = {{"bind", (PyCFunction)(void (*)(void))bind, METH_FASTCA
                          CA_FAST(fp8_paged_attention_forward, 8),
                          CA_FAST(paged_kv_append, 9),
                          CA_FAST(fused_microscaled_attention, 9),
+                         CA_FAST(cross_attention_forward, 5),
+                         CA_FAST(cross_attention_forward_lse, 5),
+                         CA_FAST(cross_attention_backward, 8),
+                         CA_FAST(relative_bias_attention_forward, 8),
+                         CA_FAST(relative_bias_attention_forward_lse, 8),
+                         CA_FAST(relative_bias_attention_backward, 11),
+                         CA_FAST(relative_bias_decode, 7),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -150,8 +150,8 @@ ca_status ca_cross_attention_bwd(ca_dtype dtype, const void* q, const void* k, c
 /* Attention with a learned relative position bias by buckets, no counterpart in
  * the reference: as ca_cross_attention, with bias_table[bucket(j - i)][h] added
  * to the scaled logit of query i and key j of q head h, and with is_causal the
- * keys j > i masked. bias_table: float32 [num_buckets, num_q_heads] on the
- * device; its finite values are taken into [-32768, 32768], -inf masks.
+ * keys j > i masked. bias_table: [num_buckets, num_q_heads] of table_dtype
+ * (CA_F32, CA_F16 or CA_BF16, whatever dtype is) on the device; its finite values are taken into [-32768, 32768], -inf masks.
  * A side has num_buckets buckets (is_causal) or num_buckets / 2, which must be
  * even then (otherwise: keys after their query have the second half);
  * bucket_starts, on the HOST, holds the first distance of each bucket of a
@@ -159,7 +159,7 @@ ca_status ca_cross_attention_bwd(ca_dtype dtype, const void* q, const void* k, c
  * is in the last bucket that starts at or before it. num_buckets <= 256.
  * workspace: ca_relative_bias_attention_workspace_bytes(...). */
 ca_status ca_relative_bias_attention(ca_dtype dtype, const void* q, const void* k, const void* v,
-                                     const float* bias_table, const int32_t* bucket_starts,
+                                     const void* bias_table, ca_dtype table_dtype, const int32_t* bucket_starts,
                                      int num_buckets, const int32_t* kv_lens, void* o, float* lse,
                                      int batch, int num_q_heads, int num_kv_heads, int q_len,
                                      int kv_len, int head_dim, float softmax_scale, int is_causal,
@@ -169,14 +169,15 @@ size_t ca_relative_bias_attention_workspace_bytes(ca_dtype dtype, int batch, int
                                                   int num_kv_heads, int q_len, int kv_len,
                                                   int head_dim, int is_causal);
 
-/* Its backward; dtable: float32 [num_buckets, num_q_heads], the sums over the
- * batch, queries and keys of each bucket's dS = P (dP - rowsum(dout o)). */
+/* Its backward; dtable: [num_buckets, num_q_heads] of table_dtype, the sums over
+ * the batch, queries and keys of each bucket's dS = P (dP - rowsum(dout o)), in
+ * an order that does not depend on timing. */
 ca_status ca_relative_bias_attention_bwd(ca_dtype dtype, const void* q, const void* k,
-                                         const void* v, const float* bias_table,
+                                         const void* v, const void* bias_table, ca_dtype table_dtype,
                                          const int32_t* bucket_starts, int num_buckets,
                                          const int32_t* kv_lens, const void* o, const void* dout,
                                          const float* lse, void* dq, void* dk, void* dv,
-                                         float* dtable, int batch, int num_q_heads,
+                                         void* dtable, int batch, int num_q_heads,
                                          int num_kv_heads, int q_len, int kv_len, int head_dim,
                                          float softmax_scale, int is_causal, void* workspace,
                                          size_t workspace_bytes, void* stream);
@@ -192,7 +193,7 @@ size_t ca_encoder_decoder_bwd_workspace_bytes(int batch, int num_q_heads, int q_
  * contiguous cache; buckets as with is_causal. workspace:
  * ca_flash_decode_workspace_bytes(...). */
 ca_status ca_relative_bias_decode(ca_dtype dtype, const void* q, const void* k, const void* v,
-                                  const float* bias_table, const int32_t* bucket_starts,
+                                  const void* bias_table, ca_dtype table_dtype, const int32_t* bucket_starts,
                                   int num_buckets, const int32_t* context_lens, void* o, int batch,
                                   int num_q_heads, int num_kv_heads, int kv_len, int head_dim,
                                   float softmax_scale, void* workspace, size_t workspace_bytes,

@@ -82,7 +82,7 @@ def test_oracle_is_plain_attention_at_equal_lengths():
     (32, False, 128), (32, True, 128), (64, True, 500), (256, True, 2048), (10, False, 20), (4, False, 2),
     (2, True, 2), (8, False, 2048), (12, True, 7), (256, False, 65), (3, True, 2)])
 def test_bucket_starts(buckets, causal, distance):
-    starts = list(api._bucket_starts(buckets, causal, distance))
+    starts = list(api._bucket_starts(buckets, causal, distance)[0])
     side = buckets if causal else buckets // 2
     e, span = side // 2, side - side // 2
     assert len(starts) == side and starts[0] == 0 and starts == sorted(starts) and starts[-1] <= distance
@@ -128,8 +128,9 @@ def _starts(*x):
 GOOD = _starts(0, 1, 2, 5)
 
 
-def _bias(table=P, starts=GOOD, buckets=8, causal=0, sizes=SIZES, scale=0.1, dtype=L.CA_BF16, q=P):
-    return L.load().ca_relative_bias_attention(dtype, q, P, P, table, starts, buckets, None, P, None, *sizes, scale,
+def _bias(table=P, starts=GOOD, buckets=8, causal=0, sizes=SIZES, scale=0.1, dtype=L.CA_BF16, q=P,
+          table_dtype=L.CA_F32):
+    return L.load().ca_relative_bias_attention(dtype, q, P, P, table, table_dtype, starts, buckets, None, P, None, *sizes, scale,
                                                causal, P, 1 << 30, None)
 
 
@@ -156,7 +157,7 @@ def test_cross_refusals(kw, word):
     (dict(table=None), "null"), (dict(starts=None), "null"), (dict(starts=_starts(1, 2, 3, 4)), "begin"),
     (dict(starts=_starts(0, 3, 2, 4)), "fall"), (dict(starts=_starts(0, 1, 2, 2049)), "2048"),
     (dict(starts=_starts(0, -1, 2, 3)), "fall"), (dict(scale=math.nan), "finite"), (dict(dtype=9), "dtype"),
-    (dict(q=ODD), "aligned"),
+    (dict(q=ODD), "aligned"), (dict(table_dtype=5), "dtype"),
 ])
 def test_bias_refusals(kw, word):
     assert _bias(**kw) == L.CA_INVALID_ARGUMENT
@@ -168,7 +169,7 @@ def test_empty_calls_do_nothing():
     assert _cross(sizes=(2, 4, 2, 0, 9, 64), q=None, k=None, v=None, o=None) == L.CA_OK
     assert _bias(sizes=(0, 4, 2, 8, 9, 64)) == L.CA_OK
     lib = L.load()
-    assert lib.ca_relative_bias_decode(L.CA_F16, None, None, None, P, GOOD, 4, None, None, 0, 4, 2, 9, 64, 0.1, None,
+    assert lib.ca_relative_bias_decode(L.CA_F16, None, None, None, P, L.CA_F16, GOOD, 4, None, None, 0, 4, 2, 9, 64, 0.1, None,
                                        0, None) == L.CA_OK
 
 
@@ -177,7 +178,7 @@ def test_backward_refusals():
 
     def bwd(lse=P, dq=P, ws=P, nbytes=1 << 30, scale=0.1, dtable=P, bias=True):
         if bias:
-            return lib.ca_relative_bias_attention_bwd(L.CA_BF16, P, P, P, P, GOOD, 8, None, P, P, lse, dq, P, P,
+            return lib.ca_relative_bias_attention_bwd(L.CA_BF16, P, P, P, P, L.CA_F32, GOOD, 8, None, P, P, lse, dq, P, P,
                                                       dtable, *SIZES, scale, 0, ws, nbytes, None)
         return lib.ca_cross_attention_bwd(L.CA_BF16, P, P, P, None, P, P, lse, dq, P, P, *SIZES, scale, ws, nbytes,
                                           None)
