@@ -413,7 +413,9 @@ __global__ __launch_bounds__(64 * kWaves) void cross_kernel(CrossArgs a, X x) {
   }
 }
 
-// Joins the splits' partials: one wave per row, D / 64 values a lane.
+// Joins the splits' partials: one wave per row, D / 64 values a lane. Bound by
+// latency: everything is loaded before the first use.
+constexpr int kMaxSplits = 16;
 template <typename Tr, int D>
 __global__ __launch_bounds__(256) void cross_merge_kernel(const float* __restrict__ part_o,
                                                           const float* __restrict__ part_lse,
@@ -423,16 +425,28 @@ __global__ __launch_bounds__(256) void cross_merge_kernel(const float* __restric
   const int lane = threadIdx.x & 63;
   const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= n_rows) return;
-  const float* pl = part_lse + row * n_split;
-  float M = kNegInf;
-  for (int s = 0; s < n_split; ++s) M = __builtin_fmaxf(M, pl[s]);
-  float W = 0.f, acc[PER] = {};
-  for (int s = 0; s < n_split; ++s) {
-    const float w = M == kNegInf ? 0.f : fast_exp2(pl[s] - M);
-    W += w;
+  const float l = lane < n_split ? part_lse[row * n_split + lane] : kNegInf;
+  float part[kMaxSplits][PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) acc[i] += w * part_o[(row * n_split + s) * D + PER * lane + i];
-  }
+  for (int s = 0; s < kMaxSplits; ++s)
+    if (s < n_split) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) part[s][i] = part_o[(row * n_split + s) * D + PER * lane + i];
+    }
+  float M = l;
+#pragma unroll
+  for (int m = kMaxSplits / 2; m >= 1; m >>= 1) M = __builtin_fmaxf(M, __shfl_xor(M, m, 64));
+  M = __shfl(M, 0, 64);
+  const float w = M == kNegInf ? 0.f : fast_exp2(l - M);
+  float W = 0.f, acc[PER] = {};
+#pragma unroll
+  for (int s = 0; s < kMaxSplits; ++s)
+    if (s < n_split) {
+      const float ws = __shfl(w, s, 64);
+      W += ws;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) acc[i] += ws * part[s][i];
+    }
   const float inv = W > 0.f ? 1.f / W : 0.f;
 #pragma unroll
   for (int i = 0; i < PER; ++i) Tr::store(o, row * D + PER * lane + i, acc[i] * inv);
@@ -444,14 +458,48 @@ struct CrossPlan {
   long long grid = 0;  // without the splits
 };
 
-CrossPlan cross_plan(long long n_bh, int rows, int Skv, bool causal) {
-  CrossPlan p;
-  const long long cus = std::max(device_cus(), 1);
-  for (p.groups = 8; p.groups > 2; p.groups /= 2)
-    if (n_bh * ((rows + 32 * p.groups - 1) / (32 * p.groups)) >= cus) break;
-  p.n_qt = (rows + 32 * p.groups - 1) / (32 * p.groups);
-  p.grid = prefill_grid(1, (int)n_bh, p.n_qt, causal, 1, &p.order);
-  return p;
+// Row groups per workgroup (8, 4, 2) and, where those leave the chip idle,
+// splits of the key walk. Times in 0.1 us, as in prefill_rows.hip: a key step of
+// a workgroup (64 keys of 8 groups; 128 of 4; 128, at D = 64 256, of 2) and what
+// a tile costs beside its steps; a launch takes its busiest CU's. A split launch
+// also writes and reads its partials and launches the merge.
+CrossPlan cross_plan(long long n_bh, int rows, int Skv, int D, bool bias, bool causal) {
+  const double cus = std::max(device_cus(), 1);
+  const bool d64 = D == 64;
+  CrossPlan best;
+  double best_cost = 0;
+  for (int groups = 8; groups >= 2; groups /= 2) {
+    const int keys = groups == 8 ? 64 : groups == 4 || !d64 ? 128 : 256;
+    const double step = groups == 8 ? (d64 ? 9 : 11) : groups == 4 ? (d64 ? 12 : 17) : (d64 ? 10.5 : 13);
+    const double tile = (groups == 8 ? 30 : groups == 4 ? 28 : 39) + (bias ? 10 : 0);
+    CrossPlan p;
+    p.groups = groups;
+    p.n_qt = (rows + 32 * groups - 1) / (32 * groups);
+    p.grid = prefill_grid(1, (int)n_bh, p.n_qt, causal, 1, &p.order);
+    const int steps = (Skv + keys - 1) / keys;
+    double cost;
+    if (causal) {
+      // the mean of a causal tile's steps: half the longest's and a half step
+      const double mean = tile + step * (0.5 * steps + 0.5), longest = tile + step * steps;
+      cost = p.order == kOrderPairs ? std::ceil(p.grid / cus) * 2 * mean
+                                    : std::max(longest, 1.1 * n_bh * p.n_qt * mean / cus);
+    } else {
+      cost = std::ceil(p.grid / cus) * (tile + step * steps);
+      for (int n = 2; n <= std::min(kMaxSplits, steps); ++n) {
+        const double bytes = 2.0 * n_bh * rows * n * D * 4;
+        const double c = std::ceil(p.grid * n / cus) * (tile + step * ((steps + n - 1) / n)) + 45 + bytes / 4e5;
+        if (c < 0.9 * cost) {
+          cost = c;
+          p.n_split = n;
+        }
+      }
+    }
+    if (groups == 8 || cost < 0.9 * best_cost) {
+      best = p;
+      best_cost = cost;
+    }
+  }
+  return best;
 }
 
 template <typename Tr, int D, class X, bool CAUSAL>
@@ -479,11 +527,28 @@ static bool few_rows(const EncDecShape& s, bool bias, bool lse) {
   return !bias && !lse && (long long)(s.Hq / s.Hkv) * s.Sq <= 16;
 }
 
-size_t cross_workspace_bytes(int dtype, const EncDecShape& s, bool bias, bool, bool lse) {
+// A launch's rows: without positions a kv head's query heads are one run of rows.
+struct CrossRows {
+  long long n_bh;
+  int rows, per_b, ratio;
+  CrossRows(const EncDecShape& s, bool bias) {
+    const int G = s.Hq / s.Hkv;
+    const bool packed = !bias && (long long)G * s.Sq <= 0x3fffffff;
+    rows = packed ? G * s.Sq : s.Sq;
+    per_b = packed ? s.Hkv : s.Hq;
+    ratio = packed ? 1 : G;
+    n_bh = (long long)s.B * per_b;
+  }
+};
+
+size_t cross_workspace_bytes(int dtype, const EncDecShape& s, bool bias, bool causal, bool lse) {
   if (few_rows(s, bias, lse))
     return std::max(decode_workspace_bytes(s.B, s.Hq * s.Sq, s.D, s.Skv),
                     flash_decode_partials_bytes(dtype, s.B, s.Hq * s.Sq, s.Hkv, s.D, s.Skv));
-  return 0;
+  if (dtype == kDtypeF32) return 0;
+  const CrossRows r(s, bias);
+  const CrossPlan p = cross_plan(r.n_bh, r.rows, s.Skv, s.D, bias, causal);
+  return p.n_split > 1 ? (size_t)r.n_bh * r.rows * p.n_split * (s.D + 1) * sizeof(float) : 0;
 }
 
 hipError_t launch_cross(int dtype, const void* q, const void* k, const void* v, void* o, float* lse,
@@ -492,24 +557,28 @@ hipError_t launch_cross(int dtype, const void* q, const void* k, const void* v, 
   if ((long long)s.B * s.Hq * s.Sq == 0) return hipSuccess;
   if (few_rows(s, bias, lse)) return launch_encdec_decode(dtype, q, k, v, o, s, nullptr, ws, ws_bytes, stream);
   if (dtype == kDtypeF32) return launch_cross_f32(q, k, v, o, lse, s, bias, causal, stream);
-  const int G = s.Hq / s.Hkv;
-  // without positions a kv head's query heads are one run of rows
-  const bool packed = !bias && (long long)G * s.Sq <= 0x3fffffff;
   CrossArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (uint16_t*)o, lse};
-  a.rows = packed ? G * s.Sq : s.Sq;
-  a.per_b = packed ? s.Hkv : s.Hq;
-  a.ratio = packed ? 1 : G;
+  const CrossRows r(s, bias);
+  if (r.n_bh > 0x7fffffffLL) return hipErrorInvalidValue;
+  a.rows = r.rows;
+  a.per_b = r.per_b;
+  a.ratio = r.ratio;
+  a.n_bh = (int)r.n_bh;
   const float eff = bias ? bias_scale(s.scale) : s.scale;
   a.scale_log2 = __builtin_fabsf(eff) * kLog2e;
   a.q_sign = __builtin_signbit(eff) ? 0x80008000u : 0u;
-  if ((long long)s.B * a.per_b > 0x7fffffffLL) return hipErrorInvalidValue;
-  a.n_bh = s.B * a.per_b;
-  const CrossPlan p = cross_plan(a.n_bh, a.rows, s.Skv, causal);
+  const CrossPlan p = cross_plan(r.n_bh, r.rows, s.Skv, s.D, bias, causal);
   if (p.grid > 0x7fffffffLL) return hipErrorInvalidValue;
   a.n_qt = p.n_qt;
   a.n_work = (int)p.grid;
   a.order = p.order;
   a.n_split = p.n_split;
+  if (p.n_split > 1) {
+    const size_t n = (size_t)r.n_bh * r.rows * p.n_split;
+    if (ws_bytes < n * (s.D + 1) * sizeof(float)) return hipErrorInvalidValue;
+    a.part_o = (float*)ws;
+    a.part_lse = a.part_o + n * s.D;
+  }
   CrossX cx;
   cx.kv_lens = s.kv_lens;
   cx.Skv = s.Skv;
