@@ -989,10 +989,11 @@ hipError_t launch_flash_bwd(int dtype, const void* q, const void* k, const void*
   return hipErrorInvalidValue;
 }
 
-// The row pairs, then (buckets > 0) a total per bucket and tile of 128 queries.
+// The row pairs, then (buckets > 0) a total per bucket and tile of 32 queries (the
+// least that a workgroup has).
 size_t cross_bwd_workspace_bytes(const EncDecShape& s, int buckets) {
   const size_t rows = (size_t)s.B * s.Hq * s.Sq;
-  const size_t tiles = (size_t)s.B * s.Hq * ((s.Sq + 127) / 128);
+  const size_t tiles = (size_t)s.B * s.Hq * ((s.Sq + 31) / 32);
   return (2 * rows + tiles * buckets) * sizeof(float);
 }
 

@@ -26,7 +26,11 @@
 //
 // With an X of their own (encdec.h) the same kernels are the backward of cross
 // attention and of attention with a relative position bias, which here is added
-// to the log2 logits; the dq kernel also sums dS by bucket.
+// to the log2 logits; the dq kernel also sums dS by bucket. Launches of few tiles
+// take their SPLIT form: a workgroup has 32 rows (queries, or keys), each wave
+// every fourth tile of their walk, staged in LDS of its own (no barriers), and
+// the waves add up at the end (2 x 8 heads x 300 queries x 1024 keys x 64: dQ
+// 120 -> 38 us, dK/dV 58 -> 46).
 #include "common.h"
 #include "encdec.h"
 #include "launch.h"
@@ -70,17 +74,18 @@ __global__ __launch_bounds__(256) void bwd_rowdot_f32_kernel(const float* __rest
 
 // Stage 32 rows of two [.., D] fp32 tensors into registers (rows past S as
 // zeros), then into padded LDS tiles.
-template <int D>
+// (T threads: the workgroup's, or a wave's)
+template <int D, int T = kF32Waves * 64>
 struct Stage2 {
   static constexpr int KS = D + 4;
   static constexpr int F4_ROW = D / 4;
-  static constexpr int PER = kF32Tile * F4_ROW / (kF32Waves * 64);
-  static_assert(PER * kF32Waves * 64 == kF32Tile * F4_ROW, "staging must cover the tile");
+  static constexpr int PER = kF32Tile * F4_ROW / T;
+  static_assert(PER * T == kF32Tile * F4_ROW, "staging must cover the tile");
   float4 a[PER], b[PER];
   __device__ __forceinline__ void load(const float* A, const float* B, int r0, int S, int tid) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int idx = tid + kF32Waves * 64 * i;
+      const int idx = tid + T * i;
       const int row = idx / F4_ROW, c4 = idx % F4_ROW;
       if (r0 + row < S) {
         a[i] = *(const float4*)(A + (size_t)(r0 + row) * D + 4 * c4);
@@ -94,7 +99,7 @@ struct Stage2 {
   __device__ __forceinline__ void store(float* As, float* Bs, int tid) const {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int idx = tid + kF32Waves * 64 * i;
+      const int idx = tid + T * i;
       const int row = idx / F4_ROW, c4 = idx % F4_ROW;
       *(float4*)(As + row * KS + 4 * c4) = a[i];
       *(float4*)(Bs + row * KS + 4 * c4) = b[i];
@@ -117,19 +122,60 @@ __device__ __forceinline__ void store_rowT_f32(float* dst_row, const f32x16 (&ac
     }
 }
 
-// dQ: one workgroup = 128 queries of one (b, h). With a bias, the sums of dS by
-// bucket go to part_table [b, h][tile][buckets].
-template <int D, bool CAUSAL, class X>
+// A wave's LDS accesses up to here are done before those that follow (its lanes
+// read what others of its lanes wrote).
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// SPLIT: the waves' accumulators added up into wave 0, through LDS at `mem`
+// (3 waves' registers, no longer in use as tiles).
+template <int N>
+__device__ __forceinline__ void sum_waves(f32x16 (&acc)[N], float* mem, int wave, int lane) {
+  __syncthreads();
+  float4* blk = (float4*)mem + lane;
+  if (wave > 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        blk[64 * (4 * (N * (wave - 1) + i) + j)] =
+            float4{acc[i][4 * j], acc[i][4 * j + 1], acc[i][4 * j + 2], acc[i][4 * j + 3]};
+  }
+  __syncthreads();
+  if (wave == 0) {
+#pragma unroll
+    for (int w = 0; w < kF32Waves - 1; ++w)
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float4 y = blk[64 * (4 * (N * w + i) + j)];
+          acc[i][4 * j] += y.x;
+          acc[i][4 * j + 1] += y.y;
+          acc[i][4 * j + 2] += y.z;
+          acc[i][4 * j + 3] += y.w;
+        }
+  }
+}
+
+// dQ: one workgroup = 128 queries of one (b, h) (SPLIT: 32). With a bias, the
+// sums of dS by bucket go to part_table [b, h][tile][buckets].
+template <int D, bool CAUSAL, class X, bool SPLIT>
 __global__ __launch_bounds__(kF32Waves * 64) void bwd_dq_f32_kernel(
     const float* __restrict__ Q, const float* __restrict__ K, const float* __restrict__ V,
     const float* __restrict__ dO, const float* __restrict__ LD, float* __restrict__ dQ, int S,
     int Hq, int Hkv, float scale, int n_qt, int n_work, X x, float* __restrict__ part_table) {
   extern __shared__ __attribute__((aligned(16))) unsigned char bias_mem[];
-  constexpr int BM = 32 * kF32Waves;
+  constexpr int BM = SPLIT ? 32 : 32 * kF32Waves;
   constexpr int HD = D / 2, NOB = D / 32;
-  constexpr int KS = Stage2<D>::KS;
-  __shared__ __attribute__((aligned(16))) float Ks[2][kF32Tile * KS];
-  __shared__ __attribute__((aligned(16))) float Vs[2][kF32Tile * KS];
+  using St = Stage2<D, SPLIT ? 64 : kF32Waves * 64>;
+  constexpr int KS = St::KS;
+  constexpr int kBufs = SPLIT ? kF32Waves : 2;  // a wave's own, or two in turn
+  __shared__ __attribute__((aligned(16))) float Ks[kBufs][kF32Tile * KS];
+  __shared__ __attribute__((aligned(16))) float Vs[kBufs][kF32Tile * KS];
 
   const int work = xcd_remap(blockIdx.x, n_work);
   const int bh = work / n_qt;
@@ -149,7 +195,7 @@ __global__ __launch_bounds__(kF32Waves * 64) void bwd_dq_f32_kernel(
   const int tid = threadIdx.x;
   const int wave = tid >> 6, lane = tid & 63;
   const int l32 = lane & 31, hl = lane >> 5;
-  const int qw0 = q0 + 32 * wave;
+  const int qw0 = SPLIT ? q0 : q0 + 32 * wave;
   const int myq = qw0 + l32;
   const bool qvalid = myq < S;
   const float c2 = scale * kLog2e;
@@ -187,7 +233,7 @@ __global__ __launch_bounds__(kF32Waves * 64) void bwd_dq_f32_kernel(
 
   const int kv_end = CAUSAL ? min(n_keys, q0 + BM) : n_keys;
   const int n_tiles = (kv_end + kF32Tile - 1) / kF32Tile;
-  Stage2<D> st;
+  St st;
   f32x16 acc[NOB];  // dQ^T
 #pragma unroll
   for (int i = 0; i < NOB; ++i)
@@ -195,12 +241,16 @@ __global__ __launch_bounds__(kF32Waves * 64) void bwd_dq_f32_kernel(
     for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
   const int krow = krow32(l32);
 
-  if (n_tiles > 0) st.load(Kp, Vp, 0, n_keys, tid);
-  for (int t = 0; t < n_tiles; ++t) {
-    const int buf = t & 1;
-    st.store(Ks[buf], Vs[buf], tid);
-    __syncthreads();
-    if (t + 1 < n_tiles) st.load(Kp, Vp, (t + 1) * kF32Tile, n_keys, tid);
+  const int sid = SPLIT ? lane : tid;               // thread of the staging
+  const int t_first = SPLIT ? wave : 0, t_step = SPLIT ? kF32Waves : 1;
+  if (t_first < n_tiles) st.load(Kp, Vp, t_first * kF32Tile, n_keys, sid);
+  for (int t = t_first; t < n_tiles; t += t_step) {
+    const int buf = SPLIT ? wave : t & 1;
+    if constexpr (SPLIT) wave_sync();  // the tile before has been read
+    st.store(Ks[buf], Vs[buf], sid);
+    if constexpr (SPLIT) wave_sync();
+    else __syncthreads();
+    if (t + t_step < n_tiles) st.load(Kp, Vp, (t + t_step) * kF32Tile, n_keys, sid);
     const int k0 = t * kF32Tile;
     if (CAUSAL && k0 > qw0 + 31) continue;  // every key after every query of the wave
     // S^T = K Q^T, dP^T = V dO^T; register r of half hl <-> key k0 + 16 hl + r
@@ -268,23 +318,29 @@ __global__ __launch_bounds__(kF32Waves * 64) void bwd_dq_f32_kernel(
       part_table[((size_t)bh * n_qt + qt) * n_buckets + i] = t;
     }
   }
+  if constexpr (SPLIT) {
+    sum_waves<NOB>(acc, Ks[0], wave, lane);
+    if (wave > 0) return;
+  }
   if (qvalid) store_rowT_f32<NOB>(dQ + (qoff + myq) * D, acc, hl, scale);
 }
 
-// dK, dV: one workgroup = 128 keys of one (b, kv head); 32-query tiles of
-// every q head of the kv head.
-template <int D, bool CAUSAL, class X>
+// dK, dV: one workgroup = 128 keys of one (b, kv head) (SPLIT: 32); 32-query tiles
+// of every q head of the kv head.
+template <int D, bool CAUSAL, class X, bool SPLIT>
 __global__ __launch_bounds__(kF32Waves * 64) void bwd_dkv_f32_kernel(
     const float* __restrict__ Q, const float* __restrict__ K, const float* __restrict__ V,
     const float* __restrict__ dO, const float* __restrict__ LD, float* __restrict__ dK,
     float* __restrict__ dV, int S, int Hq, int Hkv, float scale, int n_kt, int n_work, X x) {
   extern __shared__ __attribute__((aligned(16))) unsigned char bias_mem[];
-  constexpr int BK = 32 * kF32Waves;
+  constexpr int BK = SPLIT ? 32 : 32 * kF32Waves;
   constexpr int HD = D / 2, NOB = D / 32;
-  constexpr int KS = Stage2<D>::KS;
-  __shared__ __attribute__((aligned(16))) float Qs[2][kF32Tile * KS];
-  __shared__ __attribute__((aligned(16))) float Gs[2][kF32Tile * KS];  // dO
-  __shared__ __attribute__((aligned(16))) float Ls[2][2 * kF32Tile];   // (LSE log2 e, D) pairs
+  using St = Stage2<D, SPLIT ? 64 : kF32Waves * 64>;
+  constexpr int KS = St::KS;
+  constexpr int kBufs = SPLIT ? kF32Waves : 2;  // a wave's own, or two in turn
+  __shared__ __attribute__((aligned(16))) float Qs[kBufs][kF32Tile * KS];
+  __shared__ __attribute__((aligned(16))) float Gs[kBufs][kF32Tile * KS];  // dO
+  __shared__ __attribute__((aligned(16))) float Ls[kBufs][2 * kF32Tile];   // (LSE log2 e, D) pairs
 
   const int work = xcd_remap(blockIdx.x, n_work);
   const int bhk = work / n_kt;
@@ -302,7 +358,7 @@ __global__ __launch_bounds__(kF32Waves * 64) void bwd_dkv_f32_kernel(
   const int tid = threadIdx.x;
   const int wave = tid >> 6, lane = tid & 63;
   const int l32 = lane & 31, hl = lane >> 5;
-  const int kw0 = K0 + 32 * wave;
+  const int kw0 = SPLIT ? K0 : K0 + 32 * wave;
   const int mykey = kw0 + l32;
   const bool kvalid = mykey < n_keys;
   const float c2 = scale * kLog2e;
@@ -324,16 +380,18 @@ __global__ __launch_bounds__(kF32Waves * 64) void bwd_dkv_f32_kernel(
   if constexpr (X::kCross)
     if (K0 >= n_keys) nt = 0;
   const int n_it = G * nt;
-  Stage2<D> st;
+  const int sid = SPLIT ? lane : tid;  // thread of the staging
+  constexpr int it_step = SPLIT ? kF32Waves : 1;
+  St st;
   float lreg = 0.f;
   auto gload = [&](int it) {
     const int hq = hk * G + it / nt;
     const int q0 = (t_begin + it % nt) * kF32Tile;
     const size_t qoff = (size_t)(b * Hq + hq) * S;
-    st.load(Q + qoff * D, dO + qoff * D, q0, S, tid);
-    if (tid < 2 * kF32Tile) {  // pair element tid of the tile's 32 rows
-      const int row = q0 + (tid >> 1);
-      lreg = row < S ? LD[2 * (qoff + row) + (tid & 1)] : ((tid & 1) ? 0.f : -kNegInf);
+    st.load(Q + qoff * D, dO + qoff * D, q0, S, sid);
+    if (sid < 2 * kF32Tile) {  // pair element sid of the tile's 32 rows
+      const int row = q0 + (sid >> 1);
+      lreg = row < S ? LD[2 * (qoff + row) + (sid & 1)] : ((sid & 1) ? 0.f : -kNegInf);
     }
   };
 
@@ -344,19 +402,31 @@ __global__ __launch_bounds__(kF32Waves * 64) void bwd_dkv_f32_kernel(
     for (int r = 0; r < 16; ++r) { dk[i][r] = 0.f; dv[i][r] = 0.f; }
   const int qrow = krow32(l32);
 
-  if (n_it > 0) gload(0);
-  for (int it = 0; it < n_it; ++it) {
-    const int buf = it & 1;
-    if constexpr (X::kBias) {
-      if (it % nt == 0) {
-        __syncthreads();  // every wave has read the last q head's bias
-        bias_fill(x, hk * G + it / nt, bias_mem, 64 * kF32Waves);
-      }
-    }
-    st.store(Qs[buf], Gs[buf], tid);
-    if (tid < 2 * kF32Tile) Ls[buf][tid] = lreg;
-    __syncthreads();
-    if (it + 1 < n_it) gload(it + 1);
+  // the next tile is loaded beside this one's products, where there are registers
+  // for it (SPLIT stages four times the rows a lane)
+  constexpr bool kAhead = !SPLIT || D == 64;
+  // With a bias the walk is one q head's tiles after the other's (LDS holds one
+  // head's bias), otherwise all tiles at once.
+  int g = 0;
+  do {
+  int it_first = SPLIT ? wave : 0, it_end = n_it;
+  if constexpr (X::kBias) {
+    if (nt == 0) break;
+    if (g > 0) __syncthreads();  // every wave has read the last head's
+    bias_fill(x, hk * G + g, bias_mem, 64 * kF32Waves);
+    it_first += g * nt;
+    it_end = (g + 1) * nt;
+  }
+  if (kAhead && it_first < it_end) gload(it_first);
+  for (int it = it_first; it < it_end; it += it_step) {
+    const int buf = SPLIT ? wave : it & 1;
+    if constexpr (!kAhead) gload(it);
+    if constexpr (SPLIT) wave_sync();  // the tile before has been read
+    st.store(Qs[buf], Gs[buf], sid);
+    if (sid < 2 * kF32Tile) Ls[buf][sid] = lreg;
+    if constexpr (SPLIT) wave_sync();
+    else __syncthreads();
+    if (kAhead && it + it_step < it_end) gload(it + it_step);
     const int q0 = (t_begin + it % nt) * kF32Tile;
     if (CAUSAL && q0 + 31 < kw0) continue;  // every query before every key of the wave
     // S = Q K^T, dP = dO V^T; register r of half hl <-> query q0 + 16 hl + r
@@ -408,6 +478,12 @@ __global__ __launch_bounds__(kF32Waves * 64) void bwd_dkv_f32_kernel(
       }
     }
   }
+  } while (X::kBias && ++g < G);
+  if constexpr (SPLIT) {
+    sum_waves<NOB>(dk, Qs[0], wave, lane);
+    sum_waves<NOB>(dv, Qs[0], wave, lane);
+    if (wave > 0) return;
+  }
   if constexpr (X::kCross) {
     if (!kvalid) {  // a padded key: 0
 #pragma unroll
@@ -422,15 +498,40 @@ __global__ __launch_bounds__(kF32Waves * 64) void bwd_dkv_f32_kernel(
   }
 }
 
+// Whether a launch over `heads` heads of `rows` rows takes 32 rows a workgroup,
+// their walk in four parts: where that shortens the busiest CU's work by a fifth,
+// and LDS holds the waves' tiles beside what a bias takes.
+bool bwd_f32_splits(long long heads, int rows, int D, size_t bias_lds) {
+  const size_t tiles = kF32Waves * (2 * kF32Tile * (D + 4) + 2 * kF32Tile) * sizeof(float);
+  if (tiles + bias_lds > 160 * 1024) return false;
+  const long long cus = device_cus() > 0 ? device_cus() : 1;
+  const long long whole = heads * ((rows + 127) / 128), split = heads * ((rows + 31) / 32);
+  return 10 * ((split + cus - 1) / cus) < 8 * 4 * ((whole + cus - 1) / cus);
+}
+
 template <int D, bool CAUSAL, class X>
 hipError_t launch_bwd_f32_t(const float* q, const float* k, const float* v, const float* o,
                             const float* dout, const float* lse, float* dq, float* dk, float* dv,
                             int B, int Hq, int Hkv, int S, int Skv, float scale, float* ws, const X& x,
-                            size_t dkv_lds, size_t dq_lds, float* part_table, hipStream_t stream) {
+                            size_t dkv_lds, size_t dq_lds, float* part_table, void* dtable,
+                            hipStream_t stream) {
   const long long rows = (long long)B * Hq * S;
   const long long g0 = (rows * (D / 4) + 255) / 256;
-  const int n_qt = (S + 32 * kF32Waves - 1) / (32 * kF32Waves);
-  const int n_kt = (Skv + 32 * kF32Waves - 1) / (32 * kF32Waves);
+  auto dqk = &bwd_dq_f32_kernel<D, CAUSAL, X, false>;
+  auto dkvk = &bwd_dkv_f32_kernel<D, CAUSAL, X, false>;
+  int bm = 32 * kF32Waves, bk = 32 * kF32Waves;
+  if constexpr (X::kCross) {
+    if (bwd_f32_splits((long long)B * Hq, S, D, dq_lds)) {
+      dqk = &bwd_dq_f32_kernel<D, CAUSAL, X, true>;
+      bm = 32;
+    }
+    if (bwd_f32_splits((long long)B * Hkv, Skv, D, dkv_lds)) {
+      dkvk = &bwd_dkv_f32_kernel<D, CAUSAL, X, true>;
+      bk = 32;
+    }
+  }
+  const int n_qt = (S + bm - 1) / bm;
+  const int n_kt = (Skv + bk - 1) / bk;
   const long long gq = (long long)B * Hq * n_qt;
   const long long gk = (long long)B * Hkv * n_kt;
   if (g0 > 0x7fffffffLL || gq > 0x7fffffffLL || gk > 0x7fffffffLL) return hipErrorInvalidValue;
@@ -442,16 +543,19 @@ hipError_t launch_bwd_f32_t(const float* q, const float* k, const float* v, cons
     if (e != hipSuccess) return e;
   }
   if (gk > 0) {
-    hipLaunchKernelGGL((bwd_dkv_f32_kernel<D, CAUSAL, X>), dim3((unsigned)gk), dim3(kF32Waves * 64), dkv_lds,
+    hipLaunchKernelGGL(dkvk, dim3((unsigned)gk), dim3(kF32Waves * 64), dkv_lds,
                        stream, q, k, v, dout, ws, dk, dv, S, Hq, Hkv, scale, n_kt, (int)gk, x);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
   if (gq > 0) {
-    hipLaunchKernelGGL((bwd_dq_f32_kernel<D, CAUSAL, X>), dim3((unsigned)gq), dim3(kF32Waves * 64), dq_lds,
+    hipLaunchKernelGGL(dqk, dim3((unsigned)gq), dim3(kF32Waves * 64), dq_lds,
                        stream, q, k, v, dout, ws, dq, S, Hq, Hkv, scale, n_qt, (int)gq, x, part_table);
     e = hipGetLastError();
+    if (e != hipSuccess) return e;
   }
+  if constexpr (X::kBias)
+    return launch_bias_grad(part_table, dtable, x.table_dtype, B, Hq, n_qt, x.one_sided ? x.side : 2 * x.side, stream);
   return e;
 }
 
@@ -466,7 +570,7 @@ hipError_t launch_flash_bwd_f32(const float* q, const float* k, const float* v, 
   const SelfX x;
 #define CA_BWD32(DD, CAUSAL)                                                                                      \
   launch_bwd_f32_t<DD, CAUSAL>(q, k, v, o, dout, lse, dq, dk, dv, B, Hq, Hkv, S, S, scale, w, x, 0, 0, nullptr, \
-                               stream)
+                               nullptr, stream)
   if (D == 64) return causal ? CA_BWD32(64, true) : CA_BWD32(64, false);
   if (D == 128) return causal ? CA_BWD32(128, true) : CA_BWD32(128, false);
 #undef CA_BWD32
@@ -479,7 +583,7 @@ hipError_t launch_cross_bwd_f32(const float* q, const float* k, const float* v, 
                                 hipStream_t stream) {
 #define CA_BWD32(DD, CAUSAL, X, DKV, DQ, PART)                                                               \
   launch_bwd_f32_t<DD, CAUSAL>(q, k, v, o, dout, lse, dq, dk, dv, s.B, s.Hq, s.Hkv, s.Sq, s.Skv, s.scale, ws, \
-                               X, DKV, DQ, PART, stream)
+                               X, DKV, DQ, PART, dtable, stream)
   if (!bias) {
     CrossX x;
     x.kv_lens = s.kv_lens;
@@ -492,13 +596,10 @@ hipError_t launch_cross_bwd_f32(const float* q, const float* k, const float* v, 
   const size_t dkv = bias_lds_bytes(x.reach);
   const size_t dqb = bias_grad_lds_bytes(x.reach, bias->buckets(), kF32Waves) + kF32Waves * BiasGrad::kScratchB;
   float* part = ws + 2 * (size_t)s.B * s.Hq * s.Sq;
-  hipError_t e = hipErrorInvalidValue;
-  if (s.D == 64) e = causal ? CA_BWD32(64, true, x, dkv, dqb, part) : CA_BWD32(64, false, x, dkv, dqb, part);
-  if (s.D == 128) e = causal ? CA_BWD32(128, true, x, dkv, dqb, part) : CA_BWD32(128, false, x, dkv, dqb, part);
+  if (s.D == 64) return causal ? CA_BWD32(64, true, x, dkv, dqb, part) : CA_BWD32(64, false, x, dkv, dqb, part);
+  if (s.D == 128) return causal ? CA_BWD32(128, true, x, dkv, dqb, part) : CA_BWD32(128, false, x, dkv, dqb, part);
 #undef CA_BWD32
-  if (e != hipSuccess) return e;
-  return launch_bias_grad(part, dtable, bias->table_dtype, s.B, s.Hq, (s.Sq + 32 * kF32Waves - 1) / (32 * kF32Waves), bias->buckets(),
-                          stream);
+  return hipErrorInvalidValue;
 }
 
 }  // namespace ca

@@ -184,7 +184,7 @@ ca_status ca_relative_bias_attention_bwd(ca_dtype dtype, const void* q, const vo
 
 /* Bytes of the workspace of either backward (num_buckets 0: cross attention's):
  * per query row the pair of ca_flash_attention_bwd, and per bucket and tile of
- * 128 query rows a float. */
+ * 32 query rows a float. */
 size_t ca_encoder_decoder_bwd_workspace_bytes(int batch, int num_q_heads, int q_len,
                                               int num_buckets);
 
