@@ -161,6 +161,14 @@ template <int D, int KG>
 constexpr int dkv_stages() {
   return D == 64 || KG == 8 ? 4 : KG == 4 ? 3 : 2;
 }
+// its LDS: V rows, ring (Q and dO tiles of 32 rows, pairs), or what reduce_parts takes
+template <int D, int KG>
+constexpr int dkv_lds() {
+  constexpr int QS = kNW / KG, kRowB = 2 * D;
+  constexpr int kLdsB = KG * 32 * kRowB + dkv_stages<D, KG>() * QS * (2 * 32 * kRowB + 1024);
+  constexpr int kRedB = QS > 1 ? kNW / 2 * 2 * (D / 32) * 4096 : 0;
+  return kLdsB > kRedB ? kLdsB : kRedB;
+}
 struct TrOfs {
   uint32_t a, b;
 };
@@ -554,9 +562,9 @@ __device__ CA_INLINE void bwd_dkv_dma_tile(const uint16_t* __restrict__ Q,
   constexpr int kT = kTileB / 1024;
   constexpr int kLoads = QS * 2 * kT / kNW;     // per wave per stage (+ QS pair loads, wave 0)
   static_assert(kLoads * kNW == QS * 2 * kT, "whole loads per wave");
-  constexpr int kRedB = QS > 1 ? kNW / 2 * 2 * kNOB * 4096 : 0;  // reduce_parts
-  constexpr int kLdsB = KG * kVB + kStages * kStageB;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[kLdsB > kRedB ? kLdsB : kRedB];
+  constexpr int kLdsB = dkv_lds<D, KG>();
+  static_assert(kLdsB >= KG * kVB + kStages * kStageB, "V rows and the ring");
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[kLdsB];
 
   const int b = bhk / Hkv, hk = bhk % Hkv;
   const int G = Hq / Hkv;
@@ -579,9 +587,10 @@ __device__ CA_INLINE void bwd_dkv_dma_tile(const uint16_t* __restrict__ Q,
   const int mykey = kw0 + l32;
   const bool kvalid = mykey < n_keys;
   float c2 = scale * kLog2e;
-  // LDS: the lane's bias of a block that starts at distance r0; register r is
-  // 4 (l32 + 23 - 8 hl + 8 - off(r)) bytes past it, off = 16 (r / 8) + r % 8
-  uint32_t bofs = 0;
+  // LDS: distance 0's bias; of a block that starts at distance r0 the lane's
+  // register r is 4 (l32 + 8 - 8 hl + 23 - off(r)) bytes past entry r0, off = 16
+  // (r / 8) + r % 8
+  uint32_t bias0 = 0;
   if constexpr (X::kBias) c2 = x.scale_log2;
 
   // the key group's V rows -> LDS (rows past S read as zero); its other parts
@@ -670,7 +679,9 @@ __device__ CA_INLINE void bwd_dkv_dma_tile(const uint16_t* __restrict__ Q,
     f32x16 s, dp;
     u32x2 br[X::kBias ? 8 : 1];
     if constexpr (X::kBias) {
-      const uint32_t ba = bofs + 4 * (uint32_t)bias_block(x, kw0 - q0 - 31);
+      // (the lane's part recomputed: a register less across the loop)
+      const int ln = lane_here();
+      const uint32_t ba = bias0 + 4 * (uint32_t)bias_block(x, kw0 - q0 - 31) + 4 * ((ln & 31) + 8 - 8 * (ln >> 5));
       auto bread = [&](auto i) CA_INLINE {
         constexpr int off = 23 - 16 * (decltype(i)::value >> 2) - 2 * (decltype(i)::value & 3);
         br[decltype(i)::value] = lds_read2_b32<off, off - 1>(ba);
@@ -784,7 +795,7 @@ __device__ CA_INLINE void bwd_dkv_dma_tile(const uint16_t* __restrict__ Q,
     if constexpr (X::kBias) {
       // the next q head's bias (every wave has read the one before: the barrier)
       if (it * QS % ntp == 0)
-        bofs = bias_fill(x, hk * G + it * QS / ntp, bias_mem, 64 * kNW) + 4 * (l32 + 8 - 8 * hl);
+        bias0 = __builtin_amdgcn_readfirstlane(bias_fill(x, hk * G + it * QS / ntp, bias_mem, 64 * kNW));
     }
     const int u = it * QS + part;
     const int q0 = (t_begin + u % ntp) * BQ;
@@ -890,8 +901,10 @@ hipError_t launch_bwd_t(const void* q, const void* k, const void* v, const void*
   const long long threads = rows * (D / 8);
   const long long g0 = (threads + 255) / 256;
   if (g0 > 0x7fffffffLL) return hipErrorInvalidValue;
-  // (two waves to a key group's tiles only where LDS holds a bias beside them)
-  const BwdSplit sk = bwd_split(B, Hkv, bx.Skv, CAUSAL, D == 64 ? 122 : 109, X::kBias ? 0 : D == 64 ? 168 : 142);
+  // (four waves to a key group only where LDS holds a bias beside their tiles)
+  constexpr size_t kLds2 = bwdma::dkv_lds<D, 2>();
+  const BwdSplit sk = bwd_split(B, Hkv, bx.Skv, CAUSAL, D == 64 ? 122 : 109,
+                                kLds2 + bx.dkv_lds > 160 * 1024 ? 0 : D == 64 ? 168 : 142);
   const BwdSplit sq = bwd_split(B, Hq, S, CAUSAL, 110, 0);
   if (sk.grid > 0x7fffffffLL || sq.grid > 0x7fffffffLL) return hipErrorInvalidValue;
   hipError_t e = hipSuccess;
@@ -903,9 +916,9 @@ hipError_t launch_bwd_t(const void* q, const void* k, const void* v, const void*
     if (e != hipSuccess) return e;
   }
   if (sk.grid > 0) {
-    auto dkv = sk.groups == 8 ? &bwd_dkv_dma_kernel<Tr, D, CAUSAL, 8, X> : &bwd_dkv_dma_kernel<Tr, D, CAUSAL, 4, X>;
-    if constexpr (!X::kBias)
-      if (sk.groups == 2) dkv = &bwd_dkv_dma_kernel<Tr, D, CAUSAL, 2, X>;
+    const auto dkv = sk.groups == 8   ? &bwd_dkv_dma_kernel<Tr, D, CAUSAL, 8, X>
+                     : sk.groups == 4 ? &bwd_dkv_dma_kernel<Tr, D, CAUSAL, 4, X>
+                                      : &bwd_dkv_dma_kernel<Tr, D, CAUSAL, 2, X>;
     hipLaunchKernelGGL(dkv, dim3((unsigned)sk.grid), block, bx.dkv_lds, stream, (const uint16_t*)q,
                        (const uint16_t*)k, (const uint16_t*)v, (const uint16_t*)dout, ws, (uint16_t*)dk,
                        (uint16_t*)dv, S, Hq, Hkv, scale, sk.n_tiles, B * Hkv, (int)sk.grid, sk.order, bx.x);

@@ -30,6 +30,8 @@ namespace ca {
 namespace {
 
 constexpr int kWaves = 8;
+template <int D>
+constexpr int kStepTiles = D == 64 ? 4 : 2;
 
 struct CrossArgs {
   const uint16_t* q;
@@ -63,11 +65,13 @@ __device__ CA_INLINE void cross_tile(const CrossArgs& a, const X& x, unsigned ch
   constexpr int kKK = kBN / 16;                  // PV k-steps per tile
   constexpr int kRowB = Gm::kRowB, kNKS = Gm::kNKS, kNOB = Gm::kNOB;
   constexpr int kTileB = kBN * kRowB;            // K (or V) tile
-  constexpr int kGroupB = KS * 2 * kTileB;       // one K and one V tile per part
+  // key tiles per part and barrier: a SIMD's two waves may drift apart by that many
+  constexpr int NT = KS == 1 ? kStepTiles<D> : 1;
+  constexpr int kGroupB = KS * NT * 2 * kTileB;  // NT K and V tiles per part
   constexpr int kGroups = 128 * 1024 / kGroupB;  // ring, groups
   static_assert(kGroups >= 2, "a group loads while another is read");
   constexpr int kT = kTileB / 1024;              // 1-KB loads per tile
-  constexpr int kLoads = KS * 2 * kT / kNW;      // loads per wave per group
+  constexpr int kLoads = KS * NT * 2 * kT / kNW; // loads per wave per group
   static_assert(kT % kNW == 0, "a tile's loads are dealt to all waves");
   constexpr int NR = 16 * kNOB / KS;             // O^T registers a part combines
   constexpr int kMeetB = QG * KS * (KS - 1) * NR * 256;  // the others' registers
@@ -94,7 +98,7 @@ __device__ CA_INLINE void cross_tile(const CrossArgs& a, const X& x, unsigned ch
   // this split's tiles [t0, t0 + n_tiles)
   const int t0 = (int)((long long)n_all * split / a.n_split);
   const int n_tiles = (int)((long long)n_all * (split + 1) / a.n_split) - t0;
-  const int n_groups = (n_tiles + KS - 1) / KS;
+  const int n_groups = (n_tiles + KS * NT - 1) / (KS * NT);
   // tiles this row group computes; the last of the whole walk holds the
   // diagonal or the end
   const int w_end = CAUSAL ? min(kv_end, qw0 + 32) : kv_end;
@@ -108,17 +112,20 @@ __device__ CA_INLINE void cross_tile(const CrossArgs& a, const X& x, unsigned ch
     const int row = Gm::kRpk * wave + lane / Gm::kLpr;
     off0 = row * kRowB + 16 * ((lane % Gm::kLpr) ^ Gm::swz(row));
   }
+  // load j of the group's tile `sub`: K loads, then V loads
+  constexpr int kPer = kT / kNW;  // loads of a wave per tile, of K and of V
+  auto issue_one = [&](int g, int sub, int j) CA_INLINE {
+    const int is_v = j / kPer, p = j % kPer;
+    const uint32_t t = (uint32_t)(t0 + g * KS * NT + sub);
+    dma16_buf(make_rsrc_at(is_v ? Vp : Kp, t * kTileB, (uint32_t)kv_end * kRowB),
+              (CA_LDS void*)(lds + (g % kGroups) * kGroupB + (2 * sub + is_v) * kTileB + 1024 * (kNW * p + wave)),
+              off0 + 1024u * kNW * p);  // swz repeats every 16 rows
+  };
   auto issue = [&](int g) CA_INLINE {
-    unsigned char* st = lds + (g % kGroups) * kGroupB;
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-      constexpr int kPer = kT / kNW;  // loads of a wave per tile
-      const int sub = j / (2 * kPer), is_v = (j / kPer) % 2, p = j % kPer;
-      const uint32_t t = (uint32_t)(t0 + g * KS + sub);
-      dma16_buf(make_rsrc_at(is_v ? Vp : Kp, t * kTileB, (uint32_t)kv_end * kRowB),
-                (CA_LDS void*)(st + (2 * sub + is_v) * kTileB + 1024 * (kNW * p + wave)),
-                off0 + 1024u * kNW * p);  // swz repeats every 16 rows
-    }
+    for (int sub = 0; sub < KS * NT; ++sub)
+#pragma unroll
+      for (int j = 0; j < 2 * kPer; ++j) issue_one(g, sub, j);
   };
 #pragma unroll
   for (int g = 0; g < kGroups - 1; ++g) issue(g);
@@ -165,7 +172,9 @@ __device__ CA_INLINE void cross_tile(const CrossArgs& a, const X& x, unsigned ch
   // lane's sum passes what P's type and O hold (stale_softmax in prefill.hip), or
   // a row has met no finite logit yet (a bias of -inf).
   // MASK: the row group's last tile (diagonal, end of the keys).
-  auto tile = [&](uint32_t st, int k0, auto first_tag, auto mask_tag) CA_INLINE {
+  // NT > 1: the loads of the tile a ring ahead (group g, tile sub) go out between
+  // the QK steps: all at once, the 8 waves' loads queue behind each other.
+  auto tile = [&](uint32_t st, int k0, int g, int sub, auto first_tag, auto mask_tag) CA_INLINE {
     constexpr bool FIRST = decltype(first_tag)::value, MASK = decltype(mask_tag)::value;
     // bias reads: pair i of the lane's kBN / 4 (logits 2 i, 2 i + 1)
     constexpr int NB2 = BIAS ? 8 * kMB : 1;
@@ -212,6 +221,11 @@ __device__ CA_INLINE void cross_tile(const CrossArgs& a, const X& x, unsigned ch
       for (int mb = 0; mb < kMB; ++mb) {
         after_wait(kr[ks][mb]);
         s[mb] = Tr::mfma32(__builtin_bit_cast(vec8, kr[ks][mb]), qv[ks], s[mb]);
+      }
+      if constexpr (NT > 1) {
+        constexpr int kEvery = kNKS / (2 * kPer);
+        if (ks % kEvery == kEvery - 1) issue_one(g, sub, ks / kEvery);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
     // the first V^T fragments land under the softmax
@@ -278,7 +292,7 @@ __device__ CA_INLINE void cross_tile(const CrossArgs& a, const X& x, unsigned ch
     l_run += sum[0] + sum[1];
 
     // O^T += V^T P^T
-    auto step = [&](auto i) CA_INLINE {
+    auto pv_step = [&](auto i) CA_INLINE {
       constexpr int st_ = decltype(i)::value;
       if constexpr (st_ + VD < NST) vread(std::integral_constant<int, st_ + VD>{});
       wait_lgkm<2 * (VD < NST - 1 - st_ ? VD : NST - 1 - st_)>();
@@ -287,32 +301,45 @@ __device__ CA_INLINE void cross_tile(const CrossArgs& a, const X& x, unsigned ch
       const u32x4 w = {vr[st_][0][0], vr[st_][0][1], vr[st_][1][0], vr[st_][1][1]};
       o[st_ / kKK] = Tr::mfma32(__builtin_bit_cast(vec8, w), pb[st_ % kKK], o[st_ / kKK]);
     };
-    for_const<NST>(step);
+    for_const<NST>(pv_step);
   };
 
-  // one iteration per group: the part's tile of group g is t0 + g KS + part
+  // NT == 1: a group's loads go out at its barrier; else with the tiles
+  static_assert(NT == 1 || kGroups == 2, "all loads are awaited at a barrier");
   auto sync = [&](int g) CA_INLINE {
     wait_vmcnt<kLoads * (kGroups - 2)>();  // this wave's loads of group g landed
     __builtin_amdgcn_s_barrier();          // ... and every wave's; group g - 1 is read
-    issue(g + kGroups - 1);
+    if (NT == 1) issue(g + kGroups - 1);
     return lds0 + (uint32_t)((g % kGroups) * kGroupB + part * 2 * kTileB);
+  };
+  // the part's i-th tile of this split is tile t0 + tile_of(i); its LDS bytes
+  auto tile_of = [&](int i) CA_INLINE { return NT == 1 ? i * KS + part : i; };
+  uint32_t st = 0;
+  auto fetch = [&](int i) CA_INLINE { st = i % NT == 0 ? sync(i / NT) : st + 2 * kTileB; };
+  auto step = [&](int i, auto first_tag, auto mask_tag) CA_INLINE {
+    fetch(i);
+    tile(st, (t0 + tile_of(i)) * kBN, i / NT + 1, i % NT, first_tag, mask_tag);
   };
   using T_ = std::true_type;
   using F_ = std::false_type;
-  int g = 0;
+  int i = 0;
   const int w_full = min(w_tiles, w_last);  // tiles before the masked one
-  if (part < w_full) {
-    tile(sync(0), (t0 + part) * kBN, T_{}, F_{});
+  if (tile_of(0) < w_full) {
+    step(0, T_{}, F_{});
 #pragma clang loop unroll(disable)
-    for (g = 1; g * KS + part < w_full; ++g) tile(sync(g), (t0 + g * KS + part) * kBN, F_{}, F_{});
+    for (i = 1; tile_of(i) < w_full; ++i) step(i, F_{}, F_{});
   }
-  if (w_full < w_tiles && g * KS + part == w_full) {
-    const uint32_t st = sync(g);
-    if (g == 0) tile(st, (t0 + g * KS + part) * kBN, T_{}, T_{});
-    else tile(st, (t0 + g * KS + part) * kBN, F_{}, T_{});
-    ++g;
+  if (w_full < w_tiles && tile_of(i) == w_full) {
+    if (i == 0) step(i, T_{}, T_{});
+    else step(i, F_{}, T_{});
+    ++i;
   }
-  for (; g < n_groups; ++g) sync(g);
+  for (; i < n_groups * NT; ++i) {
+    fetch(i);
+    if (NT > 1)
+#pragma unroll
+      for (int j = 0; j < 2 * kPer; ++j) issue_one(i / NT + 1, i % NT, j);
+  }
   wait_vmcnt<0>();
   const float l_part = pair32_sum(l_run);
   if (hl == 0) {

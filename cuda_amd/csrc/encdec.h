@@ -98,7 +98,8 @@ __device__ __forceinline__ float BiasX::value(int bucket, int h) const {
 __device__ __forceinline__ uint32_t bias_fill(const BiasX& x, int h, unsigned char* mem, int threads) {
   uint16_t* first = (uint16_t*)mem;
   float* e = (float*)(mem + kBiasSearchB);
-  const int tid = threadIdx.x;
+  // (not from the work-item id, which would stay in a register up to here)
+  const int tid = 64 * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) + lane_here();
   for (int i = tid; i < x.side; i += threads) first[i] = x.first[i];
   __syncthreads();
   const int zero = x.reach + kBiasMargin;
