@@ -285,12 +285,14 @@ __device__ CA_INLINE void bwd_dq_dma_tile(const uint16_t* __restrict__ Q,
   constexpr int kStageB = 2 * kTileB;          // K tile, then V tile
   constexpr int kDma = kTileB / 1024 / kNW;    // 1-KB loads per wave per K (and V) tile
   static_assert(kDma * 1024 * kNW == kTileB, "whole 1-KB loads per wave");
-  // (the bias and its totals take up to 30 KB of LDS)
+  // (the bias and its sums take LDS)
   constexpr int kStages = X::kBias && D == 128 ? bwdma::kStages - 1 : bwdma::kStages;
   constexpr int kDist = kStages - 1;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[kStages * kStageB];
-  // per wave: 32 dQ rows x 128 bytes, staging the dQ store
-  __shared__ __attribute__((aligned(16))) unsigned char qstg[kNW * 32 * 128];
+  // per wave: 32 dQ rows x 128 bytes, staging the dQ store (with a bias, in the ring)
+  constexpr int kStgB = kNW * 32 * 128;
+  static_assert(kStages * kStageB >= kStgB, "the ring holds the staging");
+  __shared__ __attribute__((aligned(16))) unsigned char qstg[X::kBias ? 16 : kStgB];
 
   const int b = bh / Hq, h = bh % Hq;
   const int hk = h / (Hq / Hkv);
@@ -311,18 +313,16 @@ __device__ CA_INLINE void bwd_dq_dma_tile(const uint16_t* __restrict__ Q,
   const int myq = qw0 + l32;
   const bool qvalid = myq < S;
   float c2 = scale * kLog2e;
-  uint32_t bofs = 0, id_ofs = 0;  // LDS: the lane's bias of a block, its distances' bucket ids
-  BiasGrad grad;
-  float* totals = nullptr;        // [wave][buckets]
+  uint32_t bofs = 0;  // LDS: the lane's bias of a block
+  typename X::Grad grad;
   int n_buckets = 0;
   if constexpr (X::kBias) {
     c2 = x.scale_log2;
-    unsigned char* ids = bias_mem + bias_lds_bytes(x.reach);
-    totals = (float*)(ids + bias_id_bytes(x.reach));
+    float* sums = (float*)(bias_mem + bias_lds_bytes(x.reach));
     n_buckets = x.one_sided ? x.side : 2 * x.side;
     bofs = bias_fill(x, h, bias_mem, 64 * kNW) + 4 * (31 - l32 + 8 * hl);
-    id_ofs = bias_fill_ids(x, bias_mem, ids, 64 * kNW) + min(lane, 62);
-    grad.init(lds_off(qstg) + (uint32_t)(wave * BiasGrad::kScratchB), lds_off(totals + wave * n_buckets), n_buckets);
+    if constexpr (X::kWide) grad.template init<8>(x, sums, n_buckets, wave, kNW, bias_mem);
+    else grad.template init<8>(x, sums, n_buckets, wave, kNW);
     __syncthreads();
   }
   float lse2 = -kNegInf, dd = 0.f;  // a query past S: P = 0
@@ -385,12 +385,9 @@ __device__ CA_INLINE void bwd_dq_dma_tile(const uint16_t* __restrict__ Q,
     // S^T = K Q^T, dP^T = V dO^T: register r of half hl <-> key
     // k0 + 16 (r/8) + 8 hl + r%8, column = this lane's query
     f32x16 s, dp;
-    uint32_t id = 0;   // bucket of distance k0 - qw0 - 31 + min(lane, 62)
     u32x2 br[X::kBias ? 8 : 1];
     if constexpr (X::kBias) {
-      const int r0 = bias_block(x, k0 - qw0 - 31);
-      id = lds_read_u8<0>(id_ofs + (uint32_t)r0);
-      const uint32_t ba = bofs + 4 * (uint32_t)r0;
+      const uint32_t ba = bofs + 4 * (uint32_t)bias_block(x, k0 - qw0 - 31);
       auto bread = [&](auto i) CA_INLINE {
         constexpr int off = 16 * (decltype(i)::value >> 2) + 2 * (decltype(i)::value & 3);
         br[decltype(i)::value] = lds_read2_b32<off, off + 1>(ba);
@@ -405,7 +402,6 @@ __device__ CA_INLINE void bwd_dq_dma_tile(const uint16_t* __restrict__ Q,
     vr[0] = lds_read_b128<0>(va);
     if constexpr (X::kBias) {
       wait_lgkm<2>();
-      after_wait(id);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         after_wait(br[i]);
@@ -468,7 +464,7 @@ __device__ CA_INLINE void bwd_dq_dma_tile(const uint16_t* __restrict__ Q,
       acc[ob] = Tr::mfma32(x0, pb[0], acc[ob]);
       acc[ob] = Tr::mfma32(x1, pb[1], acc[ob]);
     }
-    if constexpr (X::kBias) grad.template block<8>(dsv, (int)id);
+    if constexpr (X::kBias) grad.template block<8>(x, dsv, k0 - qw0 - 31);
   };
 
 #pragma unroll
@@ -487,21 +483,12 @@ __device__ CA_INLINE void bwd_dq_dma_tile(const uint16_t* __restrict__ Q,
     }
   }
   wait_vmcnt<0>();  // no load may still target this workgroup's LDS when it exits
-  if constexpr (X::kBias) {
-    grad.flush();
-    wait_lgkm<0>();
-    __syncthreads();
-    for (int i = threadIdx.x; i < n_buckets; i += 64 * kNW) {
-      float t = 0.f;
-#pragma unroll
-      for (int w = 0; w < kNW; ++w) t += totals[w * n_buckets + i];
-      part_table[i] = t;
-    }
-  }
+  if constexpr (X::kBias) grad.finish(x, part_table, n_buckets, wave, kNW);
   if constexpr (KS > 1) reduce_parts<kNOB, QG, KS>(acc, lds, part, qg, lane);
+  // (with a bias the staging is the ring, which every wave has read: finish's barrier)
   if (part == 0)
     store_rowsT_lds<Tr, kNOB, 128>(dQ + qoff * D, qw0, S, acc, scale,
-                                   lds_off(qstg) + (uint32_t)(qg * 32 * 128), lane);
+                                   lds_off(X::kBias ? lds : qstg) + (uint32_t)(qg * 32 * 128), lane);
 }
 
 template <typename Tr, int D, bool CAUSAL, int QG, class X>
@@ -520,7 +507,7 @@ __global__ __launch_bounds__(64 * bwdma::kNW) void bwd_dq_dma_kernel(
     const int bh = pass ? wk.bh1 : wk.bh0, qt = pass ? wk.qt1 : wk.qt0;
     float* pt = nullptr;
     if constexpr (X::kBias) {
-      if (pass) __syncthreads();  // ... and the totals
+      if (pass) __syncthreads();  // ... and the sums
       pt = part_table + ((size_t)bh * n_qt + qt) * (x.one_sided ? x.side : 2 * x.side);
     }
     bwd_dq_dma_tile<Tr, D, CAUSAL, QG, X>(Q, K, V, dO, LD, dQ, S, Hq, Hkv, scale, x, bias_mem, pt, bh, qt);
@@ -886,11 +873,20 @@ BwdSplit bwd_split(int B, int heads, int S, bool causal, int cost4, int cost2) {
 // The X of a launch, what its kernels need beside it, and its table's gradient.
 template <class X>
 struct BwdX {
-  X x;
+  X x;                             // of the dQ kernel; dK/dV's is its base
   int Skv;
   size_t dkv_lds = 0, dq_lds = 0;  // dynamic
   float* part_table = nullptr;
   void* dtable = nullptr;
+};
+
+template <class X>
+struct DkvX {
+  using type = X;
+};
+template <>
+struct DkvX<BiasWideX> {
+  using type = BiasX;
 };
 
 template <typename Tr, int D, bool CAUSAL, class X>
@@ -916,9 +912,10 @@ hipError_t launch_bwd_t(const void* q, const void* k, const void* v, const void*
     if (e != hipSuccess) return e;
   }
   if (sk.grid > 0) {
-    const auto dkv = sk.groups == 8   ? &bwd_dkv_dma_kernel<Tr, D, CAUSAL, 8, X>
-                     : sk.groups == 4 ? &bwd_dkv_dma_kernel<Tr, D, CAUSAL, 4, X>
-                                      : &bwd_dkv_dma_kernel<Tr, D, CAUSAL, 2, X>;
+    using XK = typename DkvX<X>::type;
+    const auto dkv = sk.groups == 8   ? &bwd_dkv_dma_kernel<Tr, D, CAUSAL, 8, XK>
+                     : sk.groups == 4 ? &bwd_dkv_dma_kernel<Tr, D, CAUSAL, 4, XK>
+                                      : &bwd_dkv_dma_kernel<Tr, D, CAUSAL, 2, XK>;
     hipLaunchKernelGGL(dkv, dim3((unsigned)sk.grid), block, bx.dkv_lds, stream, (const uint16_t*)q,
                        (const uint16_t*)k, (const uint16_t*)v, (const uint16_t*)dout, ws, (uint16_t*)dk,
                        (uint16_t*)dv, S, Hq, Hkv, scale, sk.n_tiles, B * Hkv, (int)sk.grid, sk.order, bx.x);
@@ -1039,21 +1036,29 @@ hipError_t launch_cross_bwd(int dtype, const void* q, const void* k, const void*
     return hipErrorInvalidValue;
   }
   const float eff = bias_scale(s.scale);
-  BwdX<BiasX> bx;
-  bx.x = bias_x(s, *bias, eff, 1.f / eff);
-  bx.Skv = s.Skv;
-  bx.dkv_lds = bias_lds_bytes(bx.x.reach);
-  bx.dq_lds = bias_grad_lds_bytes(bx.x.reach, bias->buckets(), bwdma::kNW);
-  bx.part_table = w + 2 * (size_t)s.B * s.Hq * s.Sq;
-  bx.dtable = dtable;
+  const BiasX x = bias_x(s, *bias, eff, 1.f / eff);
+  // LDS of the dQ kernel beside the bias: its ring
+  const size_t room = 160 * 1024 - 64 - (s.D == 128 ? 3 : 4) * 256 * (size_t)s.D - bias_lds_bytes(x.reach);
+  const bool wide = BiasGrad::lds_bytes(x.reach, bias->buckets(), bwdma::kNW) > room;
+  auto run = [&](auto wide_tag) {
+    using X = std::conditional_t<decltype(wide_tag)::value, BiasWideX, BiasX>;
+    BwdX<X> bx;
+    (BiasX&)bx.x = x;
+    bx.Skv = s.Skv;
+    bx.dkv_lds = bias_lds_bytes(x.reach);
+    bx.dq_lds = bx.dkv_lds + X::Grad::lds_bytes(x.reach, bias->buckets(), bwdma::kNW);
+    bx.part_table = w + 2 * (size_t)s.B * s.Hq * s.Sq;
+    bx.dtable = dtable;
 #define CA_CASE(TR, DD)                   \
   if (causal) CA_BWD_CASE(TR, DD, true)   \
   CA_BWD_CASE(TR, DD, false)
-  CA_BWD_TYPES(CA_CASE)
+    CA_BWD_TYPES(CA_CASE)
 #undef CA_CASE
+    return hipErrorInvalidValue;
+  };
+  return wide ? run(std::true_type{}) : run(std::false_type{});
 #undef CA_BWD_TYPES
 #undef CA_BWD_CASE
-  return hipErrorInvalidValue;
 }
 
 }  // namespace ca

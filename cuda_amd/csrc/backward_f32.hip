@@ -215,19 +215,13 @@ __global__ __launch_bounds__(kF32Waves * 64) void bwd_dq_f32_kernel(
   }
 
   const float* be = nullptr;  // distance 0's bias, at the lane's query and its first key of a block
-  uint32_t id_ofs = 0;        // LDS: the bucket ids of a block's distances
-  BiasGrad grad;
-  float* totals = nullptr;    // [wave][buckets]
+  BiasGradWide grad;
   int n_buckets = 0;
   if constexpr (X::kBias) {
-    unsigned char* ids = bias_mem + bias_lds_bytes(x.reach);
-    totals = (float*)(ids + bias_id_bytes(x.reach));
     n_buckets = x.one_sided ? x.side : 2 * x.side;
-    unsigned char* scratch = (unsigned char*)totals + 4 * kF32Waves * n_buckets + wave * BiasGrad::kScratchB;
     bias_fill(x, h, bias_mem, 64 * kF32Waves);
     be = bias_zero(x, bias_mem) + 31 - l32 + 16 * hl;
-    id_ofs = bias_fill_ids(x, bias_mem, ids, 64 * kF32Waves) + min(lane, 62);
-    grad.init(lds_off(scratch), lds_off(totals + wave * n_buckets), n_buckets);
+    grad.init<16>(x, (float*)(bias_mem + bias_lds_bytes(x.reach)), n_buckets, wave, kF32Waves, bias_mem);
     __syncthreads();
   }
 
@@ -276,11 +270,7 @@ __global__ __launch_bounds__(kF32Waves * 64) void bwd_dq_f32_kernel(
         CAUSAL ? (k0 + kF32Tile - 1 > qw0 || (X::kCross && k0 + kF32Tile > n_keys)) : (k0 + kF32Tile > n_keys);
     float ds[16];  // dS^T / scale
     const float* bb = be;
-    int r0 = 0;
-    if constexpr (X::kBias) {
-      r0 = bias_block(x, k0 - qw0 - 31);
-      bb += r0;
-    }
+    if constexpr (X::kBias) bb += bias_block(x, k0 - qw0 - 31);
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       float e = __builtin_fmaf(s[r], c2, -lse2);
@@ -300,24 +290,10 @@ __global__ __launch_bounds__(kF32Waves * 64) void bwd_dq_f32_kernel(
       for (int r = 0; r < 16; ++r)
         acc[ob] = __builtin_amdgcn_mfma_f32_32x32x2f32(kt[r * KS], ds[r], acc[ob], 0, 0, 0);
     }
-    if constexpr (X::kBias) {
-      uint32_t id = lds_read_u8<0>(id_ofs + (uint32_t)r0);
-      wait_lgkm<0>();
-      after_wait(id);
-      grad.template block<16>(ds, (int)id);
-    }
+    if constexpr (X::kBias) grad.template block<16>(x, ds, k0 - qw0 - 31);
   }
-  if constexpr (X::kBias) {
-    grad.flush();
-    wait_lgkm<0>();
-    __syncthreads();
-    for (int i = tid; i < n_buckets; i += 64 * kF32Waves) {
-      float t = 0.f;
-#pragma unroll
-      for (int w = 0; w < kF32Waves; ++w) t += totals[w * n_buckets + i];
-      part_table[((size_t)bh * n_qt + qt) * n_buckets + i] = t;
-    }
-  }
+  if constexpr (X::kBias)
+    grad.finish(x, part_table + ((size_t)bh * n_qt + qt) * n_buckets, n_buckets, wave, kF32Waves);
   if constexpr (SPLIT) {
     sum_waves<NOB>(acc, Ks[0], wave, lane);
     if (wave > 0) return;
@@ -594,7 +570,7 @@ hipError_t launch_cross_bwd_f32(const float* q, const float* k, const float* v, 
   }
   const BiasX x = bias_x(s, *bias, s.scale, kLog2e);
   const size_t dkv = bias_lds_bytes(x.reach);
-  const size_t dqb = bias_grad_lds_bytes(x.reach, bias->buckets(), kF32Waves) + kF32Waves * BiasGrad::kScratchB;
+  const size_t dqb = dkv + BiasGradWide::lds_bytes(x.reach, bias->buckets(), kF32Waves);
   float* part = ws + 2 * (size_t)s.B * s.Hq * s.Sq;
   if (s.D == 64) return causal ? CA_BWD32(64, true, x, dkv, dqb, part) : CA_BWD32(64, false, x, dkv, dqb, part);
   if (s.D == 128) return causal ? CA_BWD32(128, true, x, dkv, dqb, part) : CA_BWD32(128, false, x, dkv, dqb, part);

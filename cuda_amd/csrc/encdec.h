@@ -33,10 +33,12 @@ constexpr float kMaxBias = 32768.f;
 
 struct SelfX {
   static constexpr bool kCross = false, kBias = false;
+  struct Grad {};
 };
 
 struct CrossX {
   static constexpr bool kCross = true, kBias = false;
+  struct Grad {};
   const int32_t* kv_lens;  // [B], null: Skv for all
   int Skv;
   // keys of sequence b
@@ -46,8 +48,11 @@ struct CrossX {
   }
 };
 
+struct BiasGrad;
+struct BiasGradWide;
 struct BiasX : CrossX {
-  static constexpr bool kBias = true;
+  static constexpr bool kBias = true, kWide = false;
+  using Grad = BiasGrad;
   const void* table;   // [buckets][Hq] of table_dtype
   int table_dtype;     // kDtypeF32, ...
   float mul;           // table values times this are the kernel's
@@ -58,6 +63,12 @@ struct BiasX : CrossX {
   int Hq;
   uint16_t first[kMaxBuckets];  // first distance of a side's bucket
   __device__ __forceinline__ float value(int bucket, int h) const;
+};
+
+// BiasX of a dQ launch whose LDS does not hold BiasGrad
+struct BiasWideX : BiasX {
+  static constexpr bool kWide = true;
+  using Grad = BiasGradWide;
 };
 
 // ---------------------------------------------------------------------------
@@ -120,22 +131,6 @@ __device__ __forceinline__ int bias_block(const BiasX& x, int r0) {
   return min(max(r0, -(x.reach + kBiasMargin - 1)), x.reach + 1);
 }
 
-// With the ids of the distances' buckets, and the totals of `waves` waves.
-constexpr int bias_id_bytes(int reach) { return (bias_entries(reach) + 15) / 16 * 16; }
-constexpr size_t bias_grad_lds_bytes(int reach, int buckets, int waves) {
-  return bias_lds_bytes(reach) + bias_id_bytes(reach) + 4 * (size_t)buckets * waves;
-}
-
-// Ids of the distances' buckets in LDS, beside the entries (all threads; a
-// barrier must follow). Returns the byte offset of distance 0's id.
-__device__ __forceinline__ uint32_t bias_fill_ids(const BiasX& x, const unsigned char* mem, unsigned char* ids,
-                                                  int threads) {
-  const int zero = x.reach + kBiasMargin;
-  for (int i = threadIdx.x; i < bias_entries(x.reach); i += threads)
-    ids[i] = (unsigned char)bias_bucket(x, (const uint16_t*)mem, i - zero);
-  return lds_off(ids + zero);
-}
-
 // LDS dwords at a + 4 O0 and a + 4 O1
 template <int O0, int O1>
 __device__ __forceinline__ u32x2 lds_read2_b32(uint32_t a) {
@@ -194,35 +189,166 @@ __device__ __forceinline__ void decode_bias(const DecodeBias& d, int n0, float (
 }
 
 // ---------------------------------------------------------------------------
-// The table's gradient: sums of dS by bucket, of one wave
+// The table's gradient: sums of dS by bucket
 // ---------------------------------------------------------------------------
-// A 32 x 32 block of dS (lane l32: query, 16 registers: keys) goes to the
-// buckets of its 63 distances. Where they are all one bucket, each lane adds its
-// registers to a running sum, which is joined when the bucket changes. Otherwise
-// the block is skewed through LDS, 16 queries at a time: row q of 64 floats holds
-// key j at column j - q + 15, so a column is a distance; lanes add up the columns
-// (lane c: distance r0 + c), a segmented scan joins the lanes of a bucket, and
-// its last lane adds the sum to the wave's total. No atomics: every total has one
-// writer at a time, in program order.
-// LDS accesses are hand-issued: the compiler would wait for the tile loads in
-// flight before its own.
+// A wave has 32 x 32 blocks of dS (lane l32: query, 16 registers: keys; HALF = 8:
+// register r of half hl is key 8 hl + 16 (r / 8) + r % 8, HALF = 16: key 16 hl + r)
+// whose 63 distances start at r0. Blocks that lie wholly past the reach on one
+// side are one bucket: each lane adds its registers to a running sum of the side.
+// No sum depends on timing: each has one writer at a time, in program order. LDS
+// accesses are hand-issued: the compiler would wait for the tile loads in flight
+// before its own.
+//
+// BiasGrad (HALF = 8): in LDS a sum for every distance (bias_entries), for each
+// wave and lane half. Within a row of 16 lanes (queries j) and a run of 8 keys e,
+// shifting by a lane between two keys adds up distances: y = ds[e] + (y of lane j
+// + 1), e falling, leaves distance -j in lane j (all of it), and z = ds[e] + (z of
+// lane j - 1), e rising, distance 7 - j, of which 7 .. 1 (lanes 0 .. 6) are z's
+// alone. The row's z belongs 9 lanes up beside the y of the row 16 distances
+// ahead; the four rows and two runs then meet in two registers, whose 64 lanes
+// each have a distance of their own half, read, added to and written back. (LDS
+// float atomics take a cycle a lane: 16 x 64 of them made a block three times as
+// long; through LDS with a segmented scan it took 1.5 us.)
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
 struct BiasGrad {
-  static constexpr int kScratchB = 16 * 64 * 4;
-  uint32_t scratch, hist;  // LDS byte offsets: the wave's rows, its totals
-  float run;               // the lane's part of the current bucket's sum
-  int run_id;
+  uint32_t at_m, at_q;  // LDS: the lane's entries of the two registers, of a block from distance 0
+  float run[2];         // the lane's sums of the blocks past the reach, before and after
+  float* mem;           // [waves][2][bias_entries]
 
-  // zeroes the wave's totals and rows (`scratch_mem`, kScratchB)
-  __device__ __forceinline__ void init(uint32_t scratch_mem, uint32_t hist_mem, int buckets) {
-    scratch = scratch_mem;
-    hist = hist_mem;
-    run = 0.f;
-    run_id = 0;
-    const int lane = lane_here();
-    for (int i = lane; i < buckets; i += 64) lds_write_b32<0>(hist + 4 * i, 0.f);
+  static constexpr size_t lds_bytes(int reach, int /*buckets*/, int waves) {
+    return (size_t)waves * 2 * bias_entries(reach) * sizeof(float);
+  }
+
+  // (all threads; a barrier must follow)
+  template <int HALF>
+  __device__ __forceinline__ void init(const BiasX& x, float* m, int /*buckets*/, int wave, int waves) {
+    static_assert(HALF == 8, "runs of 8 keys, the halves' 8 apart");
+    const int lane = lane_here(), j = lane & 15, qh = (lane >> 4) & 1, hl = lane >> 5, n = bias_entries(x.reach);
+    mem = m;
+    run[0] = run[1] = 0.f;
+    for (int i = 64 * wave + lane; i < waves * 2 * n; i += 64 * waves) m[i] = 0.f;
+    // (r0 is 31 before the distance of the block's first key and query)
+    const uint32_t zero = lds_off(m + (2 * wave + hl) * n + x.reach + kBiasMargin) + 4 * (31 + 8 * hl - j);
+    at_m = zero + (qh ? 0 : 64);
+    at_q = zero + (qh ? -64 : 128);
+  }
+
+  template <int HALF>
+  __device__ __forceinline__ void block(const BiasX& x, const float (&ds)[16], int r0) {
+    if (r0 > x.reach || r0 + 62 < -x.reach) {
+      float t[4];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) lds_write_b32<0>(scratch + 4 * (64 * i + lane), 0.f);
+      for (int i = 0; i < 4; ++i) t[i] = (ds[4 * i] + ds[4 * i + 1]) + (ds[4 * i + 2] + ds[4 * i + 3]);
+      run[r0 > 0] += (t[0] + t[1]) + (t[2] + t[3]);
+      return;
+    }
+    const uint32_t am = at_m + 4 * (uint32_t)r0, aq = at_q + 4 * (uint32_t)r0;
+    uint32_t om = lds_read_b32<0>(am), oq = lds_read_b32<0>(aq);
+    float y[2], z[2];
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      y[kk] = ds[8 * kk + 7];
+      z[kk] = ds[8 * kk];
+    }
+#pragma unroll
+    for (int e = 1; e < 8; ++e)
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        y[kk] = ds[8 * kk + 7 - e] + dpp<0x101>(y[kk]);  // row_shl:1
+        z[kk] = ds[8 * kk + e] + dpp<0x111>(z[kk]);      // row_shr:1
+      }
+    // rows (qh) of m: distances 16 and 0 ahead of lane j's -j; of y[0]: 0, -16; of z[1]: 32, 16
+    float m = y[1] + dpp<0x119>(z[0]);                   // row_shr:9
+    const float z1 = dpp<0x119>(z[1]);
+    const auto w = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, z1),
+                                                    __builtin_bit_cast(uint32_t, y[0]), false, false);
+    // [z1 row 0, y0 row 0] and [z1 row 1, y0 row 1]
+    const uint32_t w0 = w[0], w1 = w[1];
+    const bool qh = (lane_here() >> 4) & 1;
+    m += __builtin_bit_cast(float, qh ? w0 : w1);
+    const float q = __builtin_bit_cast(float, qh ? w1 : w0);
     wait_lgkm<0>();
+    after_wait(om);
+    after_wait(oq);
+    lds_write_b32<0>(am, m + __builtin_bit_cast(float, om));
+    lds_write_b32<0>(aq, q + __builtin_bit_cast(float, oq));
+  }
+
+  // Sums by bucket of all waves to out [buckets] (all threads; begins with a
+  // barrier). A wave takes every waves-th bucket, its lanes the bucket's distances.
+  __device__ __forceinline__ void finish(const BiasX& x, float* __restrict__ out, int buckets, int wave, int waves) {
+    const int lane = lane_here(), n = bias_entries(x.reach), zero = x.reach + kBiasMargin;
+    // the running sums join their sides' outermost entries, a lane half to its array
+    // (past the reach, so in the last bucket: the entries of one lane's distances)
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+      float v = run[side];
+#pragma unroll
+      for (int m = 16; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+      const int hl = lane >> 5;
+      const uint32_t at = lds_off(mem + (2 * wave + hl) * n + (side ? n - 1 : 0));
+      uint32_t t = lds_read_b32<0>(at);
+      wait_lgkm<0>();
+      after_wait(t);
+      if ((lane & 31) == 0) lds_write_b32<0>(at, v + __builtin_bit_cast(float, t));
+    }
+    wait_lgkm<0>();
+    __syncthreads();
+    for (int b = wave; b < buckets; b += waves) {
+      const bool after = b >= x.side;
+      const int s = after ? b - x.side : b;
+      // distances n0 .. n1 of the bucket (those after their query from 1 on; past
+      // the last bucket's start everything)
+      const int n0 = max((int)x.first[s], after ? 1 : 0);
+      const int n1 = s + 1 < x.side ? x.first[s + 1] - 1 : x.reach + kBiasMargin;
+      float t = 0.f;
+      for (int i = n0 + lane; i <= n1; i += 64) {
+        const int e = after ? zero + i : zero - i;
+        if (e < 0 || e >= n) continue;
+        for (int w = 0; w < 2 * waves; ++w) t += mem[w * n + e];
+      }
+#pragma unroll
+      for (int m = 32; m >= 1; m >>= 1) t += __shfl_xor(t, m, 64);
+      if (lane == 0) out[b] = t;
+    }
+  }
+};
+
+// BiasGradWide, where LDS does not hold that: bucket totals of each wave. A block
+// of more than one bucket is skewed through LDS, 16 queries at a time: row q of 64
+// floats holds key j at column j - q + 15, so a column is a distance; lanes add up
+// the columns (lane c: distance r0 + c), a segmented scan joins the lanes of a
+// bucket, and its last lane adds the sum to the total.
+struct BiasGradWide {
+  static constexpr int kScratchB = 16 * 64 * 4;
+  uint32_t scratch, hist, ids;  // LDS: the wave's rows, its totals; distance 0's bucket id
+  float run[2];
+  float* totals;
+
+  __host__ __device__ static constexpr int id_bytes(int reach) { return (bias_entries(reach) + 15) / 16 * 16; }
+  static constexpr size_t lds_bytes(int reach, int buckets, int waves) {
+    return id_bytes(reach) + waves * (kScratchB + 4 * (size_t)buckets);
+  }
+
+  // (all threads, after bias_fill at `bias_mem`; a barrier must follow)
+  template <int HALF>
+  __device__ __forceinline__ void init(const BiasX& x, float* m, int buckets, int wave, int waves,
+                                       const unsigned char* bias_mem) {
+    const int lane = lane_here();
+    unsigned char* id = (unsigned char*)m + waves * kScratchB;
+    totals = (float*)(id + id_bytes(x.reach));
+    scratch = lds_off((unsigned char*)m + wave * kScratchB);
+    hist = lds_off(totals + wave * buckets);
+    const int zero = x.reach + kBiasMargin;
+    for (int i = 64 * wave + lane; i < bias_entries(x.reach); i += 64 * waves)
+      id[i] = (unsigned char)bias_bucket(x, (const uint16_t*)bias_mem, i - zero);
+    for (int i = lane; i < buckets; i += 64) totals[wave * buckets + i] = 0.f;
+    for (int i = lane; i < kScratchB / 4; i += 64) m[wave * (kScratchB / 4) + i] = 0.f;
+    ids = lds_off(id + zero);
+    run[0] = run[1] = 0.f;
   }
 
   __device__ __forceinline__ void add(int id, float v) const {
@@ -232,32 +358,17 @@ struct BiasGrad {
     lds_write_b32<0>(hist + 4 * id, __builtin_bit_cast(float, t) + v);
   }
 
-  __device__ __forceinline__ void flush() {
-    float v = run;
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
-    if (lane_here() == 0) add(run_id, v);
-    run = 0.f;
-  }
-
-  // The block's dS; register r of half hl is key HALF hl + off(r): HALF = 8, off =
-  // 16 (r / 8) + r % 8, or HALF = 16, off = r. `id`: the bucket of distance r0 +
-  // min(lane, 62).
   template <int HALF>
-  __device__ __forceinline__ void block(const float (&ds)[16], int id) {
-    const int id0 = __builtin_amdgcn_readlane(id, 0), id1 = __builtin_amdgcn_readlane(id, 62);
-    if (id0 == id1) {
-      if (id0 != run_id) {
-        flush();
-        run_id = id0;
-      }
+  __device__ __forceinline__ void block(const BiasX& x, const float (&ds)[16], int r0) {
+    if (r0 > x.reach || r0 + 62 < -x.reach) {
       float t[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) t[i] = (ds[4 * i] + ds[4 * i + 1]) + (ds[4 * i + 2] + ds[4 * i + 3]);
-      run += (t[0] + t[1]) + (t[2] + t[3]);
+      run[r0 > 0] += (t[0] + t[1]) + (t[2] + t[3]);
       return;
     }
     const int lane = lane_here(), l32 = lane & 31, hl = lane >> 5, row = l32 & 15;
+    uint32_t id = lds_read_u8<0>(ids + (uint32_t)(r0 + min(lane, 62)));
     const uint32_t wa = scratch + 4 * (63 * row + 15 + HALF * hl);
     float v = 0.f;
 #pragma unroll
@@ -275,6 +386,7 @@ struct BiasGrad {
       auto get = [&](auto i) CA_INLINE { c[decltype(i)::value] = lds_read_b32<256 * decltype(i)::value>(ra); };
       for_const<16>(get);
       wait_lgkm<0>();
+      after_wait(id);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         after_wait(c[i]);
@@ -284,11 +396,29 @@ struct BiasGrad {
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) {
       const float up = __shfl_up(v, s, 64);
-      const int uid = __shfl_up(id, s, 64);
+      const uint32_t uid = __shfl_up(id, s, 64);
       if (lane >= s && uid == id) v += up;
     }
-    const int next = __shfl_down(id, 1, 64);
+    const uint32_t next = __shfl_down(id, 1, 64);
     if (lane == 62 || (lane < 62 && next != id)) add(id, v);
+  }
+
+  __device__ __forceinline__ void finish(const BiasX& x, float* __restrict__ out, int buckets, int wave, int waves) {
+    const int lane = lane_here();
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+      float v = run[side];
+#pragma unroll
+      for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+      if (lane == 0 && !(side && x.one_sided)) add(side ? 2 * x.side - 1 : x.side - 1, v);
+    }
+    wait_lgkm<0>();
+    __syncthreads();
+    for (int i = 64 * wave + lane; i < buckets; i += 64 * waves) {
+      float t = 0.f;
+      for (int w = 0; w < waves; ++w) t += totals[w * buckets + i];
+      out[i] = t;
+    }
   }
 };
 
@@ -301,8 +431,9 @@ inline float bias_scale(float scale) {
 
 // The device's form of a bias; sizes bound the distances that matter. mul:
 // what the kernel's bias is of the table's.
-inline BiasX bias_x(const EncDecShape& s, const BiasSpec& spec, float eff, float mul) {
-  BiasX x;
+template <class X = BiasX>
+inline X bias_x(const EncDecShape& s, const BiasSpec& spec, float eff, float mul) {
+  X x;
   x.kv_lens = s.kv_lens;
   x.Skv = s.Skv;
   x.table = spec.table;
