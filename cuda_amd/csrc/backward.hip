@@ -314,16 +314,17 @@ __device__ CA_INLINE void bwd_dq_dma_tile(const uint16_t* __restrict__ Q,
   const bool qvalid = myq < S;
   float c2 = scale * kLog2e;
   uint32_t bofs = 0;  // LDS: the lane's bias of a block
+  FarBias far{};
   typename X::Grad grad;
   int n_buckets = 0;
   if constexpr (X::kBias) {
     c2 = x.scale_log2;
     float* sums = (float*)(bias_mem + bias_lds_bytes(x.reach));
-    n_buckets = x.one_sided ? x.side : 2 * x.side;
-    bofs = bias_fill(x, h, bias_mem, 64 * kNW) + 4 * (31 - l32 + 8 * hl);
-    if constexpr (X::kWide) grad.template init<8>(x, sums, n_buckets, wave, kNW, bias_mem);
-    else grad.template init<8>(x, sums, n_buckets, wave, kNW);
-    __syncthreads();
+    n_buckets = x.buckets();
+    grad.template init<8>(x, sums, n_buckets, wave, kNW);
+    bofs = bias_fill<false>(x, h, bias_mem, 64 * kNW);
+    far = far_bias(x, bofs);
+    bofs += 4 * (31 - l32 + 8 * hl);
   }
   float lse2 = -kNegInf, dd = 0.f;  // a query past S: P = 0
   vec8 qv[kNKS], gv[kNKS];          // Q and dO as B operands (column = this lane's query)
@@ -385,31 +386,42 @@ __device__ CA_INLINE void bwd_dq_dma_tile(const uint16_t* __restrict__ Q,
     // S^T = K Q^T, dP^T = V dO^T: register r of half hl <-> key
     // k0 + 16 (r/8) + 8 hl + r%8, column = this lane's query
     f32x16 s, dp;
-    u32x2 br[X::kBias ? 8 : 1];
+    const int r0 = k0 - qw0 - 31;
     if constexpr (X::kBias) {
-      const uint32_t ba = bofs + 4 * (uint32_t)bias_block(x, k0 - qw0 - 31);
-      auto bread = [&](auto i) CA_INLINE {
-        constexpr int off = 16 * (decltype(i)::value >> 2) + 2 * (decltype(i)::value & 3);
-        br[decltype(i)::value] = lds_read2_b32<off, off + 1>(ba);
-      };
-      for_const<8>(bread);
+      // S starts as the bias: read from LDS where it is more than one value. (The
+      // reads land within the branch: one in flight at its end could have its
+      // register copied.)
+      if (bias_near<62>(x, r0)) {
+        const uint32_t ba = bofs + 4 * (uint32_t)r0;
+        u32x2 br[8];
+        auto bread = [&](auto i) CA_INLINE {
+          constexpr int off = 16 * (decltype(i)::value >> 2) + 2 * (decltype(i)::value & 3);
+          br[decltype(i)::value] = lds_read2_b32<off, off + 1>(ba);
+        };
+        for_const<8>(bread);
+        wait_lgkm<0>();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          after_wait(br[i]);
+          const uint32_t lo = br[i][0], hi = br[i][1];
+          s[2 * i] = __builtin_bit_cast(float, lo);
+          s[2 * i + 1] = __builtin_bit_cast(float, hi);
+        }
+      } else {
+        const float c = far.of(r0);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = c;
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = 0.f;
     }
 #pragma unroll
-    for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
+    for (int r = 0; r < 16; ++r) dp[r] = 0.f;
     const uint32_t ka = hb + rofs, va = ka + kTileB;
     u32x4 kr[2], vr[2];
     kr[0] = lds_read_b128<0>(ka);
     vr[0] = lds_read_b128<0>(va);
-    if constexpr (X::kBias) {
-      wait_lgkm<2>();
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        after_wait(br[i]);
-        const uint32_t lo = br[i][0], hi = br[i][1];
-        s[2 * i] = __builtin_bit_cast(float, lo);
-        s[2 * i + 1] = __builtin_bit_cast(float, hi);
-      }
-    }
 #pragma unroll
     for (int ks = 0; ks < kNKS; ++ks) {
       const int cb = ks & 1;
@@ -464,7 +476,7 @@ __device__ CA_INLINE void bwd_dq_dma_tile(const uint16_t* __restrict__ Q,
       acc[ob] = Tr::mfma32(x0, pb[0], acc[ob]);
       acc[ob] = Tr::mfma32(x1, pb[1], acc[ob]);
     }
-    if constexpr (X::kBias) grad.template block<8>(x, dsv, k0 - qw0 - 31);
+    if constexpr (X::kBias) grad.template block<8>(x, dsv, r0);
   };
 
 #pragma unroll
@@ -504,11 +516,13 @@ __global__ __launch_bounds__(64 * bwdma::kNW) void bwd_dq_dma_kernel(
 #pragma clang loop unroll(disable)
   for (int pass = 0; pass < n_pass; ++pass) {
     if (pass) __builtin_amdgcn_s_barrier();  // every wave is done reading the ring
-    const int bh = pass ? wk.bh1 : wk.bh0, qt = pass ? wk.qt1 : wk.qt0;
+    int bh = pass ? wk.bh1 : wk.bh0;
+    const int qt = pass ? wk.qt1 : wk.qt0;
+    if constexpr (X::kCross) bh = x.head(bh, Hq);
     float* pt = nullptr;
     if constexpr (X::kBias) {
       if (pass) __syncthreads();  // ... and the sums
-      pt = part_table + ((size_t)bh * n_qt + qt) * (x.one_sided ? x.side : 2 * x.side);
+      pt = part_table + ((size_t)bh * n_qt + qt) * (X::Grad::kByDistance ? bias_entries(x.reach) : x.buckets());
     }
     bwd_dq_dma_tile<Tr, D, CAUSAL, QG, X>(Q, K, V, dO, LD, dQ, S, Hq, Hkv, scale, x, bias_mem, pt, bh, qt);
   }
@@ -578,6 +592,7 @@ __device__ CA_INLINE void bwd_dkv_dma_tile(const uint16_t* __restrict__ Q,
   // register r is 4 (l32 + 8 - 8 hl + 23 - off(r)) bytes past entry r0, off = 16
   // (r / 8) + r % 8
   uint32_t bias0 = 0;
+  FarBias far{};
   if constexpr (X::kBias) c2 = x.scale_log2;
 
   // the key group's V rows -> LDS (rows past S read as zero); its other parts
@@ -664,34 +679,43 @@ __device__ CA_INLINE void bwd_dkv_dma_tile(const uint16_t* __restrict__ Q,
     // S = Q K^T, dP = dO V^T: register r of half hl <-> query
     // q0 + 16 (r/8) + 8 hl + r%8, column = this lane's key
     f32x16 s, dp;
-    u32x2 br[X::kBias ? 8 : 1];
     if constexpr (X::kBias) {
-      // (the lane's part recomputed: a register less across the loop)
-      const int ln = lane_here();
-      const uint32_t ba = bias0 + 4 * (uint32_t)bias_block(x, kw0 - q0 - 31) + 4 * ((ln & 31) + 8 - 8 * (ln >> 5));
-      auto bread = [&](auto i) CA_INLINE {
-        constexpr int off = 23 - 16 * (decltype(i)::value >> 2) - 2 * (decltype(i)::value & 3);
-        br[decltype(i)::value] = lds_read2_b32<off, off - 1>(ba);
-      };
-      for_const<8>(bread);
+      // as in the dQ kernel
+      const int r0 = kw0 - q0 - 31;
+      if (bias_near<62>(x, r0)) {
+        // (the lane's part recomputed: a register less across the loop)
+        const int ln = lane_here();
+        const uint32_t ba = bias0 + 4 * (uint32_t)r0 + 4 * ((ln & 31) + 8 - 8 * (ln >> 5));
+        u32x2 br[8];
+        auto bread = [&](auto i) CA_INLINE {
+          constexpr int off = 23 - 16 * (decltype(i)::value >> 2) - 2 * (decltype(i)::value & 3);
+          br[decltype(i)::value] = lds_read2_b32<off, off - 1>(ba);
+        };
+        for_const<8>(bread);
+        wait_lgkm<0>();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          after_wait(br[i]);
+          const uint32_t lo = br[i][0], hi = br[i][1];
+          s[2 * i] = __builtin_bit_cast(float, lo);
+          s[2 * i + 1] = __builtin_bit_cast(float, hi);
+        }
+      } else {
+        const float c = far.of(r0);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = c;
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = 0.f;
     }
 #pragma unroll
-    for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
+    for (int r = 0; r < 16; ++r) dp[r] = 0.f;
     const uint32_t qa = sb + rofs, ga = qa + kTileB;
     u32x4 qr[2], gr[2], vr[2];
     qr[0] = lds_read_b128<0>(qa);
     gr[0] = lds_read_b128<0>(ga);
     vr[0] = lds_read_b128<0>(vofs);
-    if constexpr (X::kBias) {
-      wait_lgkm<3>();
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        after_wait(br[i]);
-        const uint32_t lo = br[i][0], hi = br[i][1];
-        s[2 * i] = __builtin_bit_cast(float, lo);
-        s[2 * i + 1] = __builtin_bit_cast(float, hi);
-      }
-    }
 #pragma unroll
     for (int ks = 0; ks < kNKS; ++ks) {
       const int cb = ks & 1;
@@ -782,7 +806,10 @@ __device__ CA_INLINE void bwd_dkv_dma_tile(const uint16_t* __restrict__ Q,
     if constexpr (X::kBias) {
       // the next q head's bias (every wave has read the one before: the barrier)
       if (it * QS % ntp == 0)
-        bias0 = __builtin_amdgcn_readfirstlane(bias_fill(x, hk * G + it * QS / ntp, bias_mem, 64 * kNW));
+      {
+        bias0 = __builtin_amdgcn_readfirstlane(bias_fill<true>(x, hk * G + it * QS / ntp, bias_mem, 64 * kNW));
+        far = far_bias(x, bias0);
+      }
     }
     const int u = it * QS + part;
     const int q0 = (t_begin + u % ntp) * BQ;
@@ -826,8 +853,9 @@ __global__ __launch_bounds__(64 * bwdma::kNW) void bwd_dkv_dma_kernel(
 #pragma clang loop unroll(disable)
   for (int pass = 0; pass < n_pass; ++pass) {
     if (pass) __builtin_amdgcn_s_barrier();  // every wave is done reading the ring and V
-    bwd_dkv_dma_tile<Tr, D, CAUSAL, KG, X>(Q, K, V, dO, LD, dK, dV, S, Hq, Hkv, scale, x, bias_mem,
-                                pass ? wk.bh1 : wk.bh0, n_kt - 1 - (pass ? wk.qt1 : wk.qt0));
+    int bhk = pass ? wk.bh1 : wk.bh0;
+    if constexpr (X::kCross) bhk = x.head(bhk, Hkv);
+    bwd_dkv_dma_tile<Tr, D, CAUSAL, KG, X>(Q, K, V, dO, LD, dK, dV, S, Hq, Hkv, scale, x, bias_mem, bhk, n_kt - 1 - (pass ? wk.qt1 : wk.qt0));
   }
 }
 
@@ -932,41 +960,57 @@ hipError_t launch_bwd_t(const void* q, const void* k, const void* v, const void*
     if (e != hipSuccess) return e;
   }
   if constexpr (X::kBias)
-    return launch_bias_grad(bx.part_table, bx.dtable, bx.x.table_dtype, B, Hq, sq.n_tiles, bx.x.one_sided ? bx.x.side : 2 * bx.x.side,
-                            stream);
+    return launch_bias_grad(bx.part_table, X::Grad::kByDistance, bx.dtable, B, sq.n_tiles, bx.x, stream);
   return e;
 }
 
-// dtable[bucket][h] = the sum over sequences and tiles of part [B][Hq][n_qt]
-// [buckets]: a wave per entry, its lanes' terms in a fixed order, in 64 bits
-// (terms of both signs that nearly cancel), rounded once to the table's type.
+// dtable[bucket][h] = the sum over sequences and tiles (and the bucket's
+// distances) of part: a workgroup per entry, its threads over tiles and distances,
+// their terms in a fixed order, in 64 bits (terms of both signs that nearly
+// cancel), rounded once to the table's type.
 template <typename Tr>
-__global__ __launch_bounds__(64) void bias_grad_kernel(const float* __restrict__ part, void* __restrict__ dtable,
-                                                       int B, int Hq, int n_qt, int buckets) {
-  const int lane = threadIdx.x, bucket = blockIdx.x / Hq, h = blockIdx.x % Hq;
+__global__ __launch_bounds__(256) void bias_grad_kernel(const float* __restrict__ part, int by_distance,
+                                                        void* __restrict__ dtable, int B, int n_qt, BiasX x) {
+  const int tid = threadIdx.x, bucket = blockIdx.x / x.Hq, h = blockIdx.x % x.Hq;
+  BucketRange r{bucket, bucket + 1, 1};
+  int zero = 0, stride = x.buckets();
+  if (by_distance) {
+    r = bucket_range(x, bucket);
+    zero = x.reach + kBiasMargin;
+    stride = bias_entries(x.reach);
+  }
+  const int len = max(r.n1 - r.n0, 0);
+  int width = 1;  // threads to a tile
+  while (width < min(len, 256)) width *= 2;
+  const int d = tid & (width - 1), step = 256 / width;
+  const uint32_t tiles = (uint32_t)B * n_qt;
   double t = 0.;
-  for (long long i = lane; i < (long long)B * n_qt; i += 64) {
-    const long long b = i / n_qt, qt = i % n_qt;
-    t += (double)part[((b * Hq + h) * n_qt + qt) * buckets + bucket];
+#pragma unroll 4
+  for (uint32_t i = tid / width; i < tiles; i += step) {
+    const float* p = part + (((size_t)(i / n_qt) * x.Hq + h) * n_qt + i % n_qt) * stride + zero + r.sign * r.n0;
+    for (int e = d; e < len; e += width) t += (double)p[r.sign * e];
   }
 #pragma unroll
   for (int m = 32; m >= 1; m >>= 1) t += __shfl_xor(t, m, 64);
-  if (lane == 0) Tr::store(dtable, blockIdx.x, (float)t);
+  __shared__ double waves[4];
+  if ((tid & 63) == 0) waves[tid >> 6] = t;
+  __syncthreads();
+  if (tid == 0) Tr::store(dtable, blockIdx.x, (float)((waves[0] + waves[1]) + (waves[2] + waves[3])));
 }
 
 }  // namespace
 
 size_t bwd_workspace_bytes(int B, int Hq, int S) { return (size_t)B * Hq * S * 2 * sizeof(float); }
 
-hipError_t launch_bias_grad(const float* part, void* dtable, int dtype, int B, int Hq, int n_qt, int buckets,
+hipError_t launch_bias_grad(const float* part, bool by_distance, void* dtable, int B, int n_qt, const BiasX& x,
                             hipStream_t stream) {
-  const long long grid = (long long)Hq * buckets;
-  if (grid > 0x7fffffffLL / 64) return hipErrorInvalidValue;
+  const long long grid = (long long)x.Hq * x.buckets();
+  if (grid > 0x7fffffffLL / 256 || (long long)B * n_qt > 0x7fffffffLL) return hipErrorInvalidValue;
   if (grid == 0) return hipSuccess;
-  const auto kernel = dtype == kDtypeF32    ? &bias_grad_kernel<F32>
-                      : dtype == kDtypeBF16 ? &bias_grad_kernel<BF16>
-                                            : &bias_grad_kernel<F16>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64), 0, stream, part, dtable, B, Hq, n_qt, buckets);
+  const auto kernel = x.table_dtype == kDtypeF32    ? &bias_grad_kernel<F32>
+                      : x.table_dtype == kDtypeBF16 ? &bias_grad_kernel<BF16>
+                                                    : &bias_grad_kernel<F16>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, stream, part, (int)by_distance, dtable, B, n_qt, x);
   return hipGetLastError();
 }
 
@@ -999,12 +1043,20 @@ hipError_t launch_flash_bwd(int dtype, const void* q, const void* k, const void*
   return hipErrorInvalidValue;
 }
 
-// The row pairs, then (buckets > 0) a total per bucket and tile of 32 queries (the
-// least that a workgroup has).
+// LDS that BiasGrad may take beside a dQ ring of head dim D and the bias.
+static size_t grad_room(int D, int reach) {
+  return 160 * 1024 - 64 - (D == 128 ? 3 : 4) * 256 * (size_t)D - bias_lds_bytes(reach);
+}
+
+// The row pairs, then (buckets > 0) the tiles' parts of the table's gradient: per
+// bucket for tiles of 32 queries at least, or per distance for tiles of 128 (as
+// many distances as LDS may hold sums of).
 size_t cross_bwd_workspace_bytes(const EncDecShape& s, int buckets) {
-  const size_t rows = (size_t)s.B * s.Hq * s.Sq;
-  const size_t tiles = (size_t)s.B * s.Hq * ((s.Sq + 31) / 32);
-  return (2 * rows + tiles * buckets) * sizeof(float);
+  const size_t rows = (size_t)s.B * s.Hq * s.Sq, heads = (size_t)s.B * s.Hq;
+  constexpr size_t kMostEntries = (160 * 1024 - 64 - 4 * 256 * 64) / (4 + 4 * 2 * bwdma::kNW);
+  const size_t part = buckets ? std::max(heads * ((s.Sq + 31) / 32) * buckets,
+                                         heads * ((s.Sq + 127) / 128) * kMostEntries) : 0;
+  return (2 * rows + part) * sizeof(float);
 }
 
 hipError_t launch_cross_bwd(int dtype, const void* q, const void* k, const void* v, const void* o, const void* dout,
@@ -1030,6 +1082,7 @@ hipError_t launch_cross_bwd(int dtype, const void* q, const void* k, const void*
     BwdX<CrossX> bx;
     bx.x.kv_lens = s.kv_lens;
     bx.x.Skv = bx.Skv = s.Skv;
+    bx.x.B = s.B;
 #define CA_CASE(TR, DD) CA_BWD_CASE(TR, DD, false)
     CA_BWD_TYPES(CA_CASE)
 #undef CA_CASE
@@ -1037,9 +1090,7 @@ hipError_t launch_cross_bwd(int dtype, const void* q, const void* k, const void*
   }
   const float eff = bias_scale(s.scale);
   const BiasX x = bias_x(s, *bias, eff, 1.f / eff);
-  // LDS of the dQ kernel beside the bias: its ring
-  const size_t room = 160 * 1024 - 64 - (s.D == 128 ? 3 : 4) * 256 * (size_t)s.D - bias_lds_bytes(x.reach);
-  const bool wide = BiasGrad::lds_bytes(x.reach, bias->buckets(), bwdma::kNW) > room;
+  const bool wide = BiasGrad::lds_bytes(x.reach, bias->buckets(), bwdma::kNW) > grad_room(s.D, x.reach);
   auto run = [&](auto wide_tag) {
     using X = std::conditional_t<decltype(wide_tag)::value, BiasWideX, BiasX>;
     BwdX<X> bx;

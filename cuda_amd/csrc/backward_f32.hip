@@ -178,7 +178,8 @@ __global__ __launch_bounds__(kF32Waves * 64) void bwd_dq_f32_kernel(
   __shared__ __attribute__((aligned(16))) float Vs[kBufs][kF32Tile * KS];
 
   const int work = xcd_remap(blockIdx.x, n_work);
-  const int bh = work / n_qt;
+  int bh = work / n_qt;
+  if constexpr (X::kCross) bh = x.head(bh, Hq);
   const int qt = n_qt - 1 - (work % n_qt);  // longest causal walks first
   const int b = bh / Hq, h = bh % Hq;
   const int hk = h / (Hq / Hkv);
@@ -218,11 +219,10 @@ __global__ __launch_bounds__(kF32Waves * 64) void bwd_dq_f32_kernel(
   BiasGradWide grad;
   int n_buckets = 0;
   if constexpr (X::kBias) {
-    n_buckets = x.one_sided ? x.side : 2 * x.side;
-    bias_fill(x, h, bias_mem, 64 * kF32Waves);
+    n_buckets = x.buckets();
+    grad.init<16>(x, (float*)(bias_mem + bias_lds_bytes(x.reach)), n_buckets, wave, kF32Waves);
+    bias_fill<false>(x, h, bias_mem, 64 * kF32Waves);
     be = bias_zero(x, bias_mem) + 31 - l32 + 16 * hl;
-    grad.init<16>(x, (float*)(bias_mem + bias_lds_bytes(x.reach)), n_buckets, wave, kF32Waves, bias_mem);
-    __syncthreads();
   }
 
   const int kv_end = CAUSAL ? min(n_keys, q0 + BM) : n_keys;
@@ -319,7 +319,8 @@ __global__ __launch_bounds__(kF32Waves * 64) void bwd_dkv_f32_kernel(
   __shared__ __attribute__((aligned(16))) float Ls[kBufs][2 * kF32Tile];   // (LSE log2 e, D) pairs
 
   const int work = xcd_remap(blockIdx.x, n_work);
-  const int bhk = work / n_kt;
+  int bhk = work / n_kt;
+  if constexpr (X::kCross) bhk = x.head(bhk, Hkv);
   const int kt = work % n_kt;  // causal: the first key tiles have the longest query walks
   const int b = bhk / Hkv, hk = bhk % Hkv;
   const int G = Hq / Hkv;
@@ -389,7 +390,7 @@ __global__ __launch_bounds__(kF32Waves * 64) void bwd_dkv_f32_kernel(
   if constexpr (X::kBias) {
     if (nt == 0) break;
     if (g > 0) __syncthreads();  // every wave has read the last head's
-    bias_fill(x, hk * G + g, bias_mem, 64 * kF32Waves);
+    bias_fill<false>(x, hk * G + g, bias_mem, 64 * kF32Waves);
     it_first += g * nt;
     it_end = (g + 1) * nt;
   }
@@ -531,7 +532,7 @@ hipError_t launch_bwd_f32_t(const float* q, const float* k, const float* v, cons
     if (e != hipSuccess) return e;
   }
   if constexpr (X::kBias)
-    return launch_bias_grad(part_table, dtable, x.table_dtype, B, Hq, n_qt, x.one_sided ? x.side : 2 * x.side, stream);
+    return launch_bias_grad(part_table, false, dtable, B, n_qt, x, stream);
   return e;
 }
 
@@ -564,6 +565,7 @@ hipError_t launch_cross_bwd_f32(const float* q, const float* k, const float* v, 
     CrossX x;
     x.kv_lens = s.kv_lens;
     x.Skv = s.Skv;
+    x.B = s.B;
     if (s.D == 64) return CA_BWD32(64, false, x, 0, 0, nullptr);
     if (s.D == 128) return CA_BWD32(128, false, x, 0, 0, nullptr);
     return hipErrorInvalidValue;

@@ -156,7 +156,7 @@ __device__ CA_INLINE void cross_tile(const CrossArgs& a, const X& x, unsigned ch
   // the bias of the lane's query and its first key of a block that starts at
   // distance r0: register i is 4 (31 - l32 + 8 hl + off(i)) bytes past entry r0
   uint32_t bofs = 0;
-  if constexpr (BIAS) bofs = bias_fill(x, g_in_b, bias_mem, 64 * kNW) + 4 * (31 - l32 + 8 * hl);
+  if constexpr (BIAS) bofs = bias_fill<true>(x, g_in_b, bias_mem, 64 * kNW) + 4 * (31 - l32 + 8 * hl);
 
   f32x16 o[kNOB];
 #pragma unroll
@@ -174,6 +174,8 @@ __device__ CA_INLINE void cross_tile(const CrossArgs& a, const X& x, unsigned ch
   // MASK: the row group's last tile (diagonal, end of the keys).
   // NT > 1: the loads of the tile a ring ahead (group g, tile sub) go out between
   // the QK steps: all at once, the 8 waves' loads queue behind each other.
+  // (Tiles past the reach, of one bias, read it all the same: a copy of the tile
+  // that adds it to the exponents instead was 2-5 % slower for both.)
   auto tile = [&](uint32_t st, int k0, int g, int sub, auto first_tag, auto mask_tag) CA_INLINE {
     constexpr bool FIRST = decltype(first_tag)::value, MASK = decltype(mask_tag)::value;
     // bias reads: pair i of the lane's kBN / 4 (logits 2 i, 2 i + 1)
@@ -436,7 +438,7 @@ __global__ __launch_bounds__(64 * kWaves) void cross_kernel(CrossArgs a, X x) {
 #pragma clang loop unroll(disable)
   for (int pass = 0; pass < n_pass; ++pass) {
     if (pass) __syncthreads();  // every wave has stored its rows from LDS
-    cross_tile<Tr, D, X, CAUSAL, QG>(a, x, bias_mem, pass ? wk.bh1 : wk.bh0, pass ? wk.qt1 : wk.qt0, split);
+    cross_tile<Tr, D, X, CAUSAL, QG>(a, x, bias_mem, x.head(pass ? wk.bh1 : wk.bh0, a.per_b), pass ? wk.qt1 : wk.qt0, split);
   }
 }
 
@@ -609,6 +611,7 @@ hipError_t launch_cross(int dtype, const void* q, const void* k, const void* v, 
   CrossX cx;
   cx.kv_lens = s.kv_lens;
   cx.Skv = s.Skv;
+  cx.B = s.B;
 #define CA_CROSS_CASE(TR, DD)                                                                              \
   if (s.D == DD) {                                                                                         \
     if (!bias) return launch_t<TR, DD, CrossX, false>(a, cx, p, 0, stream);                                \

@@ -1546,6 +1546,7 @@ hipError_t launch_encdec_decode(int dtype, const void* q, const void* k, const v
   CrossX cx;
   cx.kv_lens = s.kv_lens;
   cx.Skv = s.Skv;
+  cx.B = s.B;
   // query rows of a kv head are its heads' one after the other, as decode's heads are
   const int Hq = s.Hq * s.Sq;
   if (dtype == kDtypeF32) {

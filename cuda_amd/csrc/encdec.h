@@ -40,7 +40,13 @@ struct CrossX {
   static constexpr bool kCross = true, kBias = false;
   struct Grad {};
   const int32_t* kv_lens;  // [B], null: Skv for all
-  int Skv;
+  int Skv, B;
+  // Head j of a launch's order among `per_b` heads of each sequence: a sequence's
+  // heads lie B apart, so that every XCD's share of the order (common.h) has all
+  // sequences in it, whatever their lengths (head by head, two of eight XCDs had
+  // the longest of four sequences to themselves: 4 x 32 heads x 2048 queries, 1792
+  // to 4096 keys, 466 -> XCDFIG us).
+  __device__ __forceinline__ int head(int j, int per_b) const { return j % B * per_b + j / B; }
   // keys of sequence b
   __device__ __forceinline__ int kv_len(int b) const {
     const int n = kv_lens ? kv_lens[b] : Skv;
@@ -62,6 +68,7 @@ struct BiasX : CrossX {
   int reach;           // distances from here on are in a side's last bucket
   int Hq;
   uint16_t first[kMaxBuckets];  // first distance of a side's bucket
+  __host__ __device__ __forceinline__ int buckets() const { return one_sided ? side : 2 * side; }
   __device__ __forceinline__ float value(int bucket, int h) const;
 };
 
@@ -75,9 +82,7 @@ struct BiasWideX : BiasX {
 // A head's bias by distance in LDS (dynamic: bias_lds_bytes)
 // ---------------------------------------------------------------------------
 __host__ __device__ constexpr int bias_entries(int reach) { return 2 * reach + 2 * kBiasMargin; }
-// the search table, the entries
-constexpr int kBiasSearchB = 2 * kMaxBuckets;
-constexpr size_t bias_lds_bytes(int reach) { return kBiasSearchB + 4 * (size_t)bias_entries(reach); }
+constexpr size_t bias_lds_bytes(int reach) { return 4 * (size_t)bias_entries(reach); }
 
 // bucket of distance rel, `first` in LDS
 __device__ __forceinline__ int bias_bucket(const BiasX& x, const uint16_t* first, int rel) {
@@ -104,25 +109,83 @@ __device__ __forceinline__ float BiasX::value(int bucket, int h) const {
   return bias_clamp(v) * mul;
 }
 
-// Fills the workgroup's bias of head h at `mem` (all threads; ends with a
-// barrier). Returns the LDS byte offset of distance 0's entry.
-__device__ __forceinline__ uint32_t bias_fill(const BiasX& x, int h, unsigned char* mem, int threads) {
-  uint16_t* first = (uint16_t*)mem;
-  float* e = (float*)(mem + kBiasSearchB);
-  // (not from the work-item id, which would stay in a register up to here)
-  const int tid = 64 * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) + lane_here();
-  for (int i = tid; i < x.side; i += threads) first[i] = x.first[i];
-  __syncthreads();
-  const int zero = x.reach + kBiasMargin;
-  for (int i = tid; i < bias_entries(x.reach); i += threads)
-    e[i] = x.value(bias_bucket(x, first, i - zero), h);
-  __syncthreads();
-  return lds_off(e + zero);
+// The entries of a bucket's distances: from n0 to before n1, distance n of those
+// at or before their query at zero - n, of the others (from 1 on) at zero + n.
+// The last bucket of a side has the margin.
+struct BucketRange {
+  int n0, n1, sign;
+};
+__device__ __forceinline__ BucketRange bucket_range(const BiasX& x, int b) {
+  const bool after = b >= x.side;
+  const int s = after ? b - x.side : b;
+  const int end = x.reach + kBiasMargin + (after ? 0 : 1);
+  return {max((int)x.first[s], after ? 1 : 0), s + 1 < x.side ? min((int)x.first[s + 1], end) : end, after ? 1 : -1};
 }
 
-// Distance 0's entry in what bias_fill has filled.
+// write(entry, value(bucket)) for all entries, 16 threads to a bucket: a value is
+// one load, and its entries a few writes behind it (searching each entry's bucket
+// took 1.2 us a workgroup).
+template <class V, class W>
+__device__ __forceinline__ void bias_spread(const BiasX& x, int threads, V value, W write) {
+  // (not from the work-item id, which would stay in a register up to here)
+  const int tid = 64 * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) + lane_here();
+  const int zero = x.reach + kBiasMargin, buckets = x.buckets();
+  for (int b = tid >> 4; b < buckets; b += threads >> 4) {
+    const auto v = value(b);
+    const BucketRange r = bucket_range(x, b);
+    for (int n = r.n0 + (tid & 15); n < r.n1; n += 16) write(zero + r.sign * n, v);
+  }
+}
+
+// Fills the workgroup's bias of head h at `mem` (all threads; ends with a
+// barrier). Returns the LDS byte offset of distance 0's entry. DMA: tile loads are
+// in flight, which the compiler would wait for before LDS writes of its own; then
+// LDS reads are hand-issued too.
+template <bool DMA>
+__device__ __forceinline__ uint32_t bias_fill(const BiasX& x, int h, unsigned char* mem, int threads) {
+  float* e = (float*)mem;
+  const uint32_t base = lds_off(mem);
+  auto write = [&](int i, float v) CA_INLINE {
+    if constexpr (DMA) lds_write_b32<0>(base + 4 * i, v);
+    else e[i] = v;
+  };
+  bias_spread(x, threads, [&](int b) CA_INLINE { return x.value(b, h); }, write);
+  if (x.one_sided) {  // (masked: any finite number)
+    const int tid = 64 * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) + lane_here();
+    for (int n = 1 + tid; n < x.reach + kBiasMargin; n += threads) write(x.reach + kBiasMargin + n, 0.f);
+  }
+  if constexpr (DMA) {
+    wait_lgkm<0>();
+    __builtin_amdgcn_s_barrier();
+  } else {
+    __syncthreads();
+  }
+  return base + 4 * (x.reach + kBiasMargin);
+}
+
+// Distance 0's entry in what bias_fill<false> has filled.
 __device__ __forceinline__ const float* bias_zero(const BiasX& x, const unsigned char* mem) {
-  return (const float*)(mem + kBiasSearchB) + x.reach + kBiasMargin;
+  return (const float*)mem + x.reach + kBiasMargin;
+}
+
+// Whether a block of distances [r0, r0 + SPAN] meets more than a side's last
+// bucket, and that bucket's bias if not: before their queries, or after.
+template <int SPAN>
+__device__ __forceinline__ bool bias_near(const BiasX& x, int r0) {
+  return r0 <= x.reach && r0 + SPAN >= -x.reach;
+}
+struct FarBias {
+  float before, after;
+  __device__ __forceinline__ float of(int r0) const { return r0 > 0 ? after : before; }
+};
+__device__ __forceinline__ FarBias far_bias(const BiasX& x, uint32_t zero) {
+  uint32_t a = lds_read_b32<0>(zero - 4 * (x.reach + kBiasMargin));
+  uint32_t b = lds_read_b32<0>(zero + 4 * (x.reach + kBiasMargin - 1));
+  wait_lgkm<0>();
+  after_wait(a);
+  after_wait(b);
+  return {__builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(a)),
+          __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(b))};
 }
 
 // First distance of a block of distances [r0, r0 + 94], moved into the margin
@@ -151,20 +214,19 @@ struct DecodeBias {
   float far;             // the lane's head from `reach` on
 };
 constexpr size_t decode_bias_lds_bytes(int side, int reach) {
-  return kBiasSearchB + 64 * (size_t)side + (size_t)(reach + 16) / 16 * 16;
+  return 64 * (size_t)side + (size_t)(reach + 16) / 16 * 16;
 }
 // All threads; ends with a barrier. Heads h0 .. h0 + n_heads - 1; the lane's is l16.
 __device__ __forceinline__ DecodeBias decode_bias_fill(const BiasX& x, int h0, int n_heads, unsigned char* mem,
                                                        int threads, int l16) {
-  uint16_t* first = (uint16_t*)mem;
-  float* col = (float*)(mem + kBiasSearchB);
+  float* col = (float*)mem;
   unsigned char* ids = (unsigned char*)(col + 16 * x.side);
-  const int tid = threadIdx.x;
-  for (int i = tid; i < x.side; i += threads) first[i] = x.first[i];
-  for (int i = tid; i < 16 * x.side; i += threads)
+  for (int i = threadIdx.x; i < 16 * x.side; i += threads)
     col[i] = (i & 15) < n_heads ? x.value(i >> 4, h0 + (i & 15)) : 0.f;
-  __syncthreads();
-  for (int i = tid; i <= x.reach; i += threads) ids[i] = (unsigned char)bias_bucket(x, first, -i);
+  bias_spread(x, threads, [](int b) CA_INLINE { return b; }, [&](int e, int b) CA_INLINE {
+    const int n = x.reach + kBiasMargin - e;
+    if (n <= x.reach) ids[n] = (unsigned char)b;
+  });
   __syncthreads();
   return {lds_off(ids), lds_off(col + l16), x.reach, col[16 * ids[x.reach] + l16]};
 }
@@ -214,6 +276,7 @@ __device__ __forceinline__ float dpp(float x) {
   return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
 }
 struct BiasGrad {
+  static constexpr bool kByDistance = true;  // finish's sums are by distance
   uint32_t at_m, at_q;  // LDS: the lane's entries of the two registers, of a block from distance 0
   float run[2];         // the lane's sums of the blocks past the reach, before and after
   float* mem;           // [waves][2][bias_entries]
@@ -277,18 +340,16 @@ struct BiasGrad {
     lds_write_b32<0>(aq, q + __builtin_bit_cast(float, oq));
   }
 
-  // Sums by bucket of all waves to out [buckets] (all threads; begins with a
-  // barrier). A wave takes every waves-th bucket, its lanes the bucket's distances.
-  __device__ __forceinline__ void finish(const BiasX& x, float* __restrict__ out, int buckets, int wave, int waves) {
-    const int lane = lane_here(), n = bias_entries(x.reach), zero = x.reach + kBiasMargin;
-    // the running sums join their sides' outermost entries, a lane half to its array
-    // (past the reach, so in the last bucket: the entries of one lane's distances)
+  // Sums of all waves by distance to out [bias_entries] (all threads; a barrier
+  // within). The running sums join their sides' outermost entries, which are of
+  // the last bucket, a lane half's in its own array.
+  __device__ __forceinline__ void finish(const BiasX& x, float* __restrict__ out, int /*buckets*/, int wave, int waves) {
+    const int lane = lane_here(), n = bias_entries(x.reach), hl = lane >> 5;
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
       float v = run[side];
 #pragma unroll
       for (int m = 16; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
-      const int hl = lane >> 5;
       const uint32_t at = lds_off(mem + (2 * wave + hl) * n + (side ? n - 1 : 0));
       uint32_t t = lds_read_b32<0>(at);
       wait_lgkm<0>();
@@ -297,22 +358,11 @@ struct BiasGrad {
     }
     wait_lgkm<0>();
     __syncthreads();
-    for (int b = wave; b < buckets; b += waves) {
-      const bool after = b >= x.side;
-      const int s = after ? b - x.side : b;
-      // distances n0 .. n1 of the bucket (those after their query from 1 on; past
-      // the last bucket's start everything)
-      const int n0 = max((int)x.first[s], after ? 1 : 0);
-      const int n1 = s + 1 < x.side ? x.first[s + 1] - 1 : x.reach + kBiasMargin;
+    for (int e = 64 * wave + lane; e < n; e += 64 * waves) {
       float t = 0.f;
-      for (int i = n0 + lane; i <= n1; i += 64) {
-        const int e = after ? zero + i : zero - i;
-        if (e < 0 || e >= n) continue;
-        for (int w = 0; w < 2 * waves; ++w) t += mem[w * n + e];
-      }
 #pragma unroll
-      for (int m = 32; m >= 1; m >>= 1) t += __shfl_xor(t, m, 64);
-      if (lane == 0) out[b] = t;
+      for (int w = 0; w < 2 * waves; ++w) t += mem[w * n + e];
+      out[e] = t;
     }
   }
 };
@@ -323,6 +373,7 @@ struct BiasGrad {
 // the columns (lane c: distance r0 + c), a segmented scan joins the lanes of a
 // bucket, and its last lane adds the sum to the total.
 struct BiasGradWide {
+  static constexpr bool kByDistance = false;  // finish's sums are by bucket
   static constexpr int kScratchB = 16 * 64 * 4;
   uint32_t scratch, hist, ids;  // LDS: the wave's rows, its totals; distance 0's bucket id
   float run[2];
@@ -333,18 +384,19 @@ struct BiasGradWide {
     return id_bytes(reach) + waves * (kScratchB + 4 * (size_t)buckets);
   }
 
-  // (all threads, after bias_fill at `bias_mem`; a barrier must follow)
+  // (all threads; a barrier must follow)
   template <int HALF>
-  __device__ __forceinline__ void init(const BiasX& x, float* m, int buckets, int wave, int waves,
-                                       const unsigned char* bias_mem) {
+  __device__ __forceinline__ void init(const BiasX& x, float* m, int buckets, int wave, int waves) {
     const int lane = lane_here();
     unsigned char* id = (unsigned char*)m + waves * kScratchB;
     totals = (float*)(id + id_bytes(x.reach));
     scratch = lds_off((unsigned char*)m + wave * kScratchB);
     hist = lds_off(totals + wave * buckets);
     const int zero = x.reach + kBiasMargin;
-    for (int i = 64 * wave + lane; i < bias_entries(x.reach); i += 64 * waves)
-      id[i] = (unsigned char)bias_bucket(x, (const uint16_t*)bias_mem, i - zero);
+    bias_spread(x, 64 * waves, [](int b) CA_INLINE { return b; },
+                [&](int e, int b) CA_INLINE { id[e] = (unsigned char)b; });
+    if (x.one_sided)  // (keys after their query: masked)
+      for (int i = 1 + 64 * wave + lane; i < zero; i += 64 * waves) id[zero + i] = 0;
     for (int i = lane; i < buckets; i += 64) totals[wave * buckets + i] = 0.f;
     for (int i = lane; i < kScratchB / 4; i += 64) m[wave * (kScratchB / 4) + i] = 0.f;
     ids = lds_off(id + zero);
@@ -429,6 +481,11 @@ inline float bias_scale(float scale) {
   return a >= 0x1p-60f ? scale : __builtin_copysignf(0x1p-60f, scale);
 }
 
+// Sums of the workgroups' part [B][Hq][n_qt] x [buckets], or x [bias_entries]
+// where they are by distance, into dtable (backward.hip).
+hipError_t launch_bias_grad(const float* part, bool by_distance, void* dtable, int B, int n_qt, const BiasX& x,
+                            hipStream_t stream);
+
 // The device's form of a bias; sizes bound the distances that matter. mul:
 // what the kernel's bias is of the table's.
 template <class X = BiasX>
@@ -436,6 +493,7 @@ inline X bias_x(const EncDecShape& s, const BiasSpec& spec, float eff, float mul
   X x;
   x.kv_lens = s.kv_lens;
   x.Skv = s.Skv;
+  x.B = s.B;
   x.table = spec.table;
   x.table_dtype = spec.table_dtype;
   x.mul = mul;

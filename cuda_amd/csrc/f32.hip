@@ -93,7 +93,7 @@ __device__ CA_INLINE void prefill_f32_qtile(
   // distance 0's bias, at the lane's query and its first key of a block
   const float* be = nullptr;
   if constexpr (X::kBias) {
-    bias_fill(x_, h, bias_mem, NW * 64);
+    bias_fill<false>(x_, h, bias_mem, NW * 64);
     be = bias_zero(x_, bias_mem) + 31 - l32 + 16 * hl;
   }
 
@@ -235,8 +235,9 @@ __global__ __launch_bounds__(256, 2) void prefill_f32_kernel(
   for (int pass = 0; pass < n_pass; ++pass) {
     // the second tile restages the LDS buffers: every wave must be done reading them
     if (pass) __syncthreads();
-    prefill_f32_qtile<D, CAUSAL, X>(Q, K, V, O, Lse, S, Hq, Hkv, scale_log2, pass ? wk.bh1 : wk.bh0,
-                                    pass ? wk.qt1 : wk.qt0, x, bias_mem);
+    int bh = pass ? wk.bh1 : wk.bh0;
+    if constexpr (X::kCross) bh = x.head(bh, Hq);
+    prefill_f32_qtile<D, CAUSAL, X>(Q, K, V, O, Lse, S, Hq, Hkv, scale_log2, bh, pass ? wk.qt1 : wk.qt0, x, bias_mem);
   }
 }
 
@@ -325,7 +326,7 @@ __device__ CA_INLINE void prefill_f32_split_walk(
   // distance 0's bias, at the lane's query and its first key of a block
   const float* be = nullptr;
   if constexpr (X::kBias) {
-    bias_fill(x, h, bias_mem, NW * 64);
+    bias_fill<false>(x, h, bias_mem, NW * 64);
     be = bias_zero(x, bias_mem) + 31 - l32 + 16 * hl;
   }
   const int na = n_tiles_of(qa);
@@ -565,7 +566,9 @@ __global__ __launch_bounds__(64 * SplitStage<D>::NW, 1) void prefill_f32_split_k
   extern __shared__ __attribute__((aligned(16))) unsigned char bias_mem[];
   __shared__ __attribute__((aligned(16))) SplitStage<D> stg;
   const int item = xcd_remap(blockIdx.x, n_work);
-  const int bh = item / per_head, p = item % per_head;
+  int bh = item / per_head;
+  const int p = item % per_head;
+  if constexpr (X::kCross) bh = x.head(bh, Hq);
   int p2 = CAUSAL ? n_qb - 1 - p : p + per_head;
   if (p2 == p || p2 >= n_qb) p2 = -1;
   prefill_f32_split_walk<D, CAUSAL, X>(Q, K, V, S, Hq, Hkv, scale_log2, bh, p, p2, stg, x, bias_mem);
@@ -643,6 +646,7 @@ hipError_t launch_cross_f32(const void* q, const void* k, const void* v, void* o
     CrossX x;
     x.kv_lens = s.kv_lens;
     x.Skv = s.Skv;
+    x.B = s.B;
     if (s.D == 64) return CA_F32_CASE(64, false, x, 0);
     if (s.D == 128) return CA_F32_CASE(128, false, x, 0);
     return hipErrorInvalidValue;

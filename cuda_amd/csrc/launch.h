@@ -110,10 +110,6 @@ hipError_t launch_cross_bwd_f32(const float* q, const float* k, const float* v, 
                                 const float* lse, float* dq, float* dk, float* dv, void* dtable,
                                 const EncDecShape& s, const BiasSpec* bias, bool causal, float* ws,
                                 hipStream_t stream);
-// Sums the workgroups' totals part [B][Hq][n_qt][buckets] of a table's gradient.
-hipError_t launch_bias_grad(const float* part, void* dtable, int dtype, int B, int Hq, int n_qt, int buckets,
-                            hipStream_t stream);
-
 // Compute units of the current device (cached per device; 0 if unknown).
 // Safe for concurrent first calls: each slot is an atomic, and every thread
 // that finds it empty stores the same attribute value.

