@@ -271,7 +271,8 @@ __device__ CA_INLINE void bwd_dq_dma_tile(const uint16_t* __restrict__ Q,
                                          const uint16_t* __restrict__ dO,
                                          const float* __restrict__ LD, uint16_t* __restrict__ dQ,
                                          int S, int Hq, int Hkv, float scale, const X& x,
-                                         unsigned char* bias_mem, float* __restrict__ part_table, int bh, int qt) {
+                                         unsigned char* bias_mem, float* __restrict__ part_table, int bh, int qt,
+                                         int n_keys) {
   using namespace bwdma;
   using Gm = Geom<D>;
   using vec8 = typename Tr::vec8;
@@ -297,11 +298,8 @@ __device__ CA_INLINE void bwd_dq_dma_tile(const uint16_t* __restrict__ Q,
   const int b = bh / Hq, h = bh % Hq;
   const int hk = h / (Hq / Hkv);
   const int q0 = qt * BM;
-  int Skv = S, n_keys = S;
-  if constexpr (X::kCross) {
-    Skv = x.Skv;
-    n_keys = x.kv_len(b);
-  }
+  int Skv = S;
+  if constexpr (X::kCross) Skv = x.Skv;
   const size_t qoff = (size_t)(b * Hq + h) * S;
   const uint16_t* Kp = K + (size_t)(b * Hkv + hk) * Skv * D;
   const uint16_t* Vp = V + (size_t)(b * Hkv + hk) * Skv * D;
@@ -518,13 +516,18 @@ __global__ __launch_bounds__(64 * bwdma::kNW) void bwd_dq_dma_kernel(
     if (pass) __builtin_amdgcn_s_barrier();  // every wave is done reading the ring
     int bh = pass ? wk.bh1 : wk.bh0;
     const int qt = pass ? wk.qt1 : wk.qt0;
-    if constexpr (X::kCross) bh = x.head(bh, Hq);
+    int n_keys = S;
+    if constexpr (X::kCross) {
+      const auto head = x.head(bh, Hq);
+      bh = head.bh;
+      n_keys = head.n_keys;
+    }
     float* pt = nullptr;
     if constexpr (X::kBias) {
       if (pass) __syncthreads();  // ... and the sums
       pt = part_table + ((size_t)bh * n_qt + qt) * (X::Grad::kByDistance ? bias_entries(x.reach) : x.buckets());
     }
-    bwd_dq_dma_tile<Tr, D, CAUSAL, QG, X>(Q, K, V, dO, LD, dQ, S, Hq, Hkv, scale, x, bias_mem, pt, bh, qt);
+    bwd_dq_dma_tile<Tr, D, CAUSAL, QG, X>(Q, K, V, dO, LD, dQ, S, Hq, Hkv, scale, x, bias_mem, pt, bh, qt, n_keys);
   }
 }
 
@@ -542,7 +545,7 @@ __device__ CA_INLINE void bwd_dkv_dma_tile(const uint16_t* __restrict__ Q,
                                           const float* __restrict__ LD, uint16_t* __restrict__ dK,
                                           uint16_t* __restrict__ dV, int S, int Hq, int Hkv,
                                           float scale, const X& x, unsigned char* bias_mem, int bhk,
-                                          int kt) {
+                                          int kt, int n_keys) {
   using namespace bwdma;
   using Gm = Geom<D>;
   using vec8 = typename Tr::vec8;
@@ -570,11 +573,8 @@ __device__ CA_INLINE void bwd_dkv_dma_tile(const uint16_t* __restrict__ Q,
   const int b = bhk / Hkv, hk = bhk % Hkv;
   const int G = Hq / Hkv;
   const int K0 = kt * BK;
-  int Skv = S, n_keys = S;
-  if constexpr (X::kCross) {
-    Skv = x.Skv;
-    n_keys = x.kv_len(b);
-  }
+  int Skv = S;
+  if constexpr (X::kCross) Skv = x.Skv;
   const size_t kvoff = (size_t)(b * Hkv + hk) * Skv;
   // The lane index is recomputed per call (lane_here): otherwise the
   // compiler hoists the lane-derived load offsets of both passes out of the
@@ -854,8 +854,14 @@ __global__ __launch_bounds__(64 * bwdma::kNW) void bwd_dkv_dma_kernel(
   for (int pass = 0; pass < n_pass; ++pass) {
     if (pass) __builtin_amdgcn_s_barrier();  // every wave is done reading the ring and V
     int bhk = pass ? wk.bh1 : wk.bh0;
-    if constexpr (X::kCross) bhk = x.head(bhk, Hkv);
-    bwd_dkv_dma_tile<Tr, D, CAUSAL, KG, X>(Q, K, V, dO, LD, dK, dV, S, Hq, Hkv, scale, x, bias_mem, bhk, n_kt - 1 - (pass ? wk.qt1 : wk.qt0));
+    int n_keys = S;
+    if constexpr (X::kCross) {
+      const auto head = x.head(bhk, Hkv);
+      bhk = head.bh;
+      n_keys = head.n_keys;
+    }
+    bwd_dkv_dma_tile<Tr, D, CAUSAL, KG, X>(Q, K, V, dO, LD, dK, dV, S, Hq, Hkv, scale, x, bias_mem, bhk,
+                                           n_kt - 1 - (pass ? wk.qt1 : wk.qt0), n_keys);
   }
 }
 

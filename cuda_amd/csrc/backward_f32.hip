@@ -179,7 +179,7 @@ __global__ __launch_bounds__(kF32Waves * 64) void bwd_dq_f32_kernel(
 
   const int work = xcd_remap(blockIdx.x, n_work);
   int bh = work / n_qt;
-  if constexpr (X::kCross) bh = x.head(bh, Hq);
+  if constexpr (X::kCross) bh = x.head(bh, Hq).bh;
   const int qt = n_qt - 1 - (work % n_qt);  // longest causal walks first
   const int b = bh / Hq, h = bh % Hq;
   const int hk = h / (Hq / Hkv);
@@ -320,7 +320,7 @@ __global__ __launch_bounds__(kF32Waves * 64) void bwd_dkv_f32_kernel(
 
   const int work = xcd_remap(blockIdx.x, n_work);
   int bhk = work / n_kt;
-  if constexpr (X::kCross) bhk = x.head(bhk, Hkv);
+  if constexpr (X::kCross) bhk = x.head(bhk, Hkv).bh;
   const int kt = work % n_kt;  // causal: the first key tiles have the longest query walks
   const int b = bhk / Hkv, hk = bhk % Hkv;
   const int G = Hq / Hkv;

@@ -51,8 +51,8 @@ struct CrossArgs {
 
 // Split `split` of the key walk of query tile qt of group bh.
 template <typename Tr, int D, class X, bool CAUSAL, int QG>
-__device__ CA_INLINE void cross_tile(const CrossArgs& a, const X& x, unsigned char* bias_mem, int bh, int qt,
-                                     int split) {
+__device__ CA_INLINE void cross_tile(const CrossArgs& a, const X& x, unsigned char* bias_mem, int bh, int n_keys,
+                                     int qt, int split) {
   using Gm = PfGeom<D>;
   using vec8 = typename Tr::vec8;
   using vec4 = typename Tr::vec4;
@@ -91,7 +91,6 @@ __device__ CA_INLINE void cross_tile(const CrossArgs& a, const X& x, unsigned ch
   const size_t khead = ((size_t)b * (a.per_b / a.ratio) + g_in_b / a.ratio) * x.Skv;
   const uint16_t* Kp = a.k + khead * D;
   const uint16_t* Vp = a.v + khead * D;
-  const int n_keys = x.kv_len(b);
 
   const int kv_end = CAUSAL ? min(n_keys, q0 + 32 * QG) : n_keys;
   const int n_all = (kv_end + kBN - 1) / kBN;
@@ -438,7 +437,8 @@ __global__ __launch_bounds__(64 * kWaves) void cross_kernel(CrossArgs a, X x) {
 #pragma clang loop unroll(disable)
   for (int pass = 0; pass < n_pass; ++pass) {
     if (pass) __syncthreads();  // every wave has stored its rows from LDS
-    cross_tile<Tr, D, X, CAUSAL, QG>(a, x, bias_mem, x.head(pass ? wk.bh1 : wk.bh0, a.per_b), pass ? wk.qt1 : wk.qt0, split);
+    const auto head = x.head(pass ? wk.bh1 : wk.bh0, a.per_b);
+    cross_tile<Tr, D, X, CAUSAL, QG>(a, x, bias_mem, head.bh, head.n_keys, pass ? wk.qt1 : wk.qt0, split);
   }
 }
 

@@ -41,12 +41,35 @@ struct CrossX {
   struct Grad {};
   const int32_t* kv_lens;  // [B], null: Skv for all
   int Skv, B;
-  // Head j of a launch's order among `per_b` heads of each sequence: a sequence's
-  // heads lie B apart, so that every XCD's share of the order (common.h) has all
-  // sequences in it, whatever their lengths (head by head, two of eight XCDs had
-  // the longest of four sequences to themselves: 4 x 32 heads x 2048 queries, 1792
-  // to 4096 keys, 466 -> XCDFIG us).
-  __device__ __forceinline__ int head(int j, int per_b) const { return j % B * per_b + j / B; }
+  // Head j of a launch's order among `per_b` heads of each sequence. A sequence's
+  // heads lie apart, so that every XCD's share of the order (an eighth, common.h)
+  // has all sequences in it, whatever their lengths; where 8 divides per_b, an XCD
+  // takes its heads of the longest sequence first, and the short ones fill the end.
+  // (4 x 32 heads x 2048 queries, 1792 to 4096 keys: 466 us head by head, when two
+  // XCDs had the longest sequence to themselves; 383 apart; LPTFIG longest first.)
+  struct Head {
+    int bh, n_keys;  // the head, its sequence's keys
+  };
+  __device__ __forceinline__ Head head(int j, int per_b) const {
+    auto plain = [&](int b, int h) CA_INLINE {
+      const int n = kv_lens ? kv_lens[b] : Skv;
+      return Head{b * per_b + h, __builtin_amdgcn_readfirstlane(min(max(n, 0), Skv))};
+    };
+    if (per_b % 8) return plain(j % B, j / B);
+    const int hx = per_b / 8, share = hx * B, xcd = j / share, i = j % share;
+    const int r = i / hx, h = xcd * hx + i % hx;
+    if (!kv_lens || B == 1 || B > 64) return plain(r, h);
+    // the sequence of rank r by length: lane l counts those that come before l
+    const int lane = lane_here();
+    const int n = lane < B ? min(max(kv_lens[lane], 0), Skv) : -1;
+    int rank = 0;
+    for (int l = 0; l < B; ++l) {
+      const int m = __builtin_amdgcn_readlane(n, l);
+      rank += m > n || (m == n && l < lane);
+    }
+    const int b = __builtin_ctzll(__ballot(lane < B && rank == r));
+    return Head{b * per_b + h, __builtin_amdgcn_readlane(n, b)};
+  }
   // keys of sequence b
   __device__ __forceinline__ int kv_len(int b) const {
     const int n = kv_lens ? kv_lens[b] : Skv;

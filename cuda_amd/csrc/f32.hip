@@ -236,7 +236,7 @@ __global__ __launch_bounds__(256, 2) void prefill_f32_kernel(
     // the second tile restages the LDS buffers: every wave must be done reading them
     if (pass) __syncthreads();
     int bh = pass ? wk.bh1 : wk.bh0;
-    if constexpr (X::kCross) bh = x.head(bh, Hq);
+    if constexpr (X::kCross) bh = x.head(bh, Hq).bh;
     prefill_f32_qtile<D, CAUSAL, X>(Q, K, V, O, Lse, S, Hq, Hkv, scale_log2, bh, pass ? wk.qt1 : wk.qt0, x, bias_mem);
   }
 }
@@ -568,7 +568,7 @@ __global__ __launch_bounds__(64 * SplitStage<D>::NW, 1) void prefill_f32_split_k
   const int item = xcd_remap(blockIdx.x, n_work);
   int bh = item / per_head;
   const int p = item % per_head;
-  if constexpr (X::kCross) bh = x.head(bh, Hq);
+  if constexpr (X::kCross) bh = x.head(bh, Hq).bh;
   int p2 = CAUSAL ? n_qb - 1 - p : p + per_head;
   if (p2 == p || p2 >= n_qb) p2 = -1;
   prefill_f32_split_walk<D, CAUSAL, X>(Q, K, V, S, Hq, Hkv, scale_log2, bh, p, p2, stg, x, bias_mem);
