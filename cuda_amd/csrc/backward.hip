@@ -317,7 +317,7 @@ __device__ CA_INLINE void bwd_dq_dma_tile(const uint16_t* __restrict__ Q,
   int n_buckets = 0;
   if constexpr (X::kBias) {
     c2 = x.scale_log2;
-    float* sums = (float*)(bias_mem + bias_lds_bytes(x.reach));
+    float* sums = (float*)(bias_mem + bias_lds_bytes(x));
     n_buckets = x.buckets();
     grad.template init<8>(x, sums, n_buckets, wave, kNW);
     bofs = bias_fill<false>(x, h, bias_mem, 64 * kNW);
@@ -525,7 +525,7 @@ __global__ __launch_bounds__(64 * bwdma::kNW) void bwd_dq_dma_kernel(
     float* pt = nullptr;
     if constexpr (X::kBias) {
       if (pass) __syncthreads();  // ... and the sums
-      pt = part_table + ((size_t)bh * n_qt + qt) * (X::Grad::kByDistance ? bias_entries(x.reach) : x.buckets());
+      pt = part_table + ((size_t)bh * n_qt + qt) * (X::Grad::kByDistance ? bias_entries(x) : x.buckets());
     }
     bwd_dq_dma_tile<Tr, D, CAUSAL, QG, X>(Q, K, V, dO, LD, dQ, S, Hq, Hkv, scale, x, bias_mem, pt, bh, qt, n_keys);
   }
@@ -983,7 +983,7 @@ __global__ __launch_bounds__(256) void bias_grad_kernel(const float* __restrict_
   if (by_distance) {
     r = bucket_range(x, bucket);
     zero = x.reach + kBiasMargin;
-    stride = bias_entries(x.reach);
+    stride = bias_entries(x);
   }
   const int len = max(r.n1 - r.n0, 0);
   int width = 1;  // threads to a tile
@@ -1050,8 +1050,8 @@ hipError_t launch_flash_bwd(int dtype, const void* q, const void* k, const void*
 }
 
 // LDS that BiasGrad may take beside a dQ ring of head dim D and the bias.
-static size_t grad_room(int D, int reach) {
-  return 160 * 1024 - 64 - (D == 128 ? 3 : 4) * 256 * (size_t)D - bias_lds_bytes(reach);
+static size_t grad_room(int D, const BiasX& x) {
+  return 160 * 1024 - 64 - (D == 128 ? 3 : 4) * 256 * (size_t)D - bias_lds_bytes(x);
 }
 
 // The row pairs, then (buckets > 0) the tiles' parts of the table's gradient: per
@@ -1096,14 +1096,14 @@ hipError_t launch_cross_bwd(int dtype, const void* q, const void* k, const void*
   }
   const float eff = bias_scale(s.scale);
   const BiasX x = bias_x(s, *bias, eff, 1.f / eff);
-  const bool wide = BiasGrad::lds_bytes(x.reach, bias->buckets(), bwdma::kNW) > grad_room(s.D, x.reach);
+  const bool wide = BiasGrad::lds_bytes(x, bwdma::kNW) > grad_room(s.D, x);
   auto run = [&](auto wide_tag) {
     using X = std::conditional_t<decltype(wide_tag)::value, BiasWideX, BiasX>;
     BwdX<X> bx;
     (BiasX&)bx.x = x;
     bx.Skv = s.Skv;
-    bx.dkv_lds = bias_lds_bytes(x.reach);
-    bx.dq_lds = bx.dkv_lds + X::Grad::lds_bytes(x.reach, bias->buckets(), bwdma::kNW);
+    bx.dkv_lds = bias_lds_bytes(x);
+    bx.dq_lds = bx.dkv_lds + X::Grad::lds_bytes(x, bwdma::kNW);
     bx.part_table = w + 2 * (size_t)s.B * s.Hq * s.Sq;
     bx.dtable = dtable;
 #define CA_CASE(TR, DD)                   \

@@ -220,7 +220,7 @@ __global__ __launch_bounds__(kF32Waves * 64) void bwd_dq_f32_kernel(
   int n_buckets = 0;
   if constexpr (X::kBias) {
     n_buckets = x.buckets();
-    grad.init<16>(x, (float*)(bias_mem + bias_lds_bytes(x.reach)), n_buckets, wave, kF32Waves);
+    grad.init<16>(x, (float*)(bias_mem + bias_lds_bytes(x)), n_buckets, wave, kF32Waves);
     bias_fill<false>(x, h, bias_mem, 64 * kF32Waves);
     be = bias_zero(x, bias_mem) + 31 - l32 + 16 * hl;
   }
@@ -571,8 +571,8 @@ hipError_t launch_cross_bwd_f32(const float* q, const float* k, const float* v, 
     return hipErrorInvalidValue;
   }
   const BiasX x = bias_x(s, *bias, s.scale, kLog2e);
-  const size_t dkv = bias_lds_bytes(x.reach);
-  const size_t dqb = dkv + BiasGradWide::lds_bytes(x.reach, bias->buckets(), kF32Waves);
+  const size_t dkv = bias_lds_bytes(x);
+  const size_t dqb = dkv + BiasGradWide::lds_bytes(x, kF32Waves);
   float* part = ws + 2 * (size_t)s.B * s.Hq * s.Sq;
   if (s.D == 64) return causal ? CA_BWD32(64, true, x, dkv, dqb, part) : CA_BWD32(64, false, x, dkv, dqb, part);
   if (s.D == 128) return causal ? CA_BWD32(128, true, x, dkv, dqb, part) : CA_BWD32(128, false, x, dkv, dqb, part);

@@ -616,7 +616,7 @@ hipError_t launch_cross(int dtype, const void* q, const void* k, const void* v, 
   if (s.D == DD) {                                                                                         \
     if (!bias) return launch_t<TR, DD, CrossX, false>(a, cx, p, 0, stream);                                \
     const BiasX bx = bias_x(s, *bias, eff, 1.f / __builtin_fabsf(eff));                                         \
-    const size_t lds = bias_lds_bytes(bx.reach);                                                           \
+    const size_t lds = bias_lds_bytes(bx);                                                           \
     return causal ? launch_t<TR, DD, BiasX, true>(a, bx, p, lds, stream)                                   \
                   : launch_t<TR, DD, BiasX, false>(a, bx, p, lds, stream);                                 \
   }

@@ -10,8 +10,9 @@
 // with first[b] <= n, n = |j - i|; keys after their query (j > i) have a side of
 // their own unless only those before it count (one_sided: n = 0 there). Past
 // `reach`, the last bucket's first distance, the bias of a side is one value.
-// Kernels keep a head's bias by distance in LDS, [-(reach + 96), reach + 95],
-// and move a block whose distances all lie past the reach into that margin.
+// Kernels keep a head's bias by distance in LDS, [-(reach + 96), reach + 95] (one
+// side: up to 95), and move a block whose distances all lie past the reach into
+// that margin.
 #pragma once
 
 #include <algorithm>
@@ -104,8 +105,10 @@ struct BiasWideX : BiasX {
 // ---------------------------------------------------------------------------
 // A head's bias by distance in LDS (dynamic: bias_lds_bytes)
 // ---------------------------------------------------------------------------
-__host__ __device__ constexpr int bias_entries(int reach) { return 2 * reach + 2 * kBiasMargin; }
-constexpr size_t bias_lds_bytes(int reach) { return 4 * (size_t)bias_entries(reach); }
+__host__ __device__ __forceinline__ int bias_entries(const BiasX& x) {
+  return x.reach + (x.one_sided ? 0 : x.reach) + 2 * kBiasMargin;
+}
+__host__ __device__ __forceinline__ size_t bias_lds_bytes(const BiasX& x) { return 4 * (size_t)bias_entries(x); }
 
 // bucket of distance rel, `first` in LDS
 __device__ __forceinline__ int bias_bucket(const BiasX& x, const uint16_t* first, int rel) {
@@ -175,7 +178,7 @@ __device__ __forceinline__ uint32_t bias_fill(const BiasX& x, int h, unsigned ch
   bias_spread(x, threads, [&](int b) CA_INLINE { return x.value(b, h); }, write);
   if (x.one_sided) {  // (masked: any finite number)
     const int tid = 64 * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) + lane_here();
-    for (int n = 1 + tid; n < x.reach + kBiasMargin; n += threads) write(x.reach + kBiasMargin + n, 0.f);
+    for (int n = 1 + tid; n < kBiasMargin; n += threads) write(x.reach + kBiasMargin + n, 0.f);
   }
   if constexpr (DMA) {
     wait_lgkm<0>();
@@ -203,7 +206,7 @@ struct FarBias {
 };
 __device__ __forceinline__ FarBias far_bias(const BiasX& x, uint32_t zero) {
   uint32_t a = lds_read_b32<0>(zero - 4 * (x.reach + kBiasMargin));
-  uint32_t b = lds_read_b32<0>(zero + 4 * (x.reach + kBiasMargin - 1));
+  uint32_t b = lds_read_b32<0>(zero + 4 * (bias_entries(x) - x.reach - kBiasMargin - 1));
   wait_lgkm<0>();
   after_wait(a);
   after_wait(b);
@@ -214,7 +217,7 @@ __device__ __forceinline__ FarBias far_bias(const BiasX& x, uint32_t zero) {
 // First distance of a block of distances [r0, r0 + 94], moved into the margin
 // where all of them lie past the reach.
 __device__ __forceinline__ int bias_block(const BiasX& x, int r0) {
-  return min(max(r0, -(x.reach + kBiasMargin - 1)), x.reach + 1);
+  return min(max(r0, -(x.reach + kBiasMargin - 1)), x.one_sided ? 1 : x.reach + 1);
 }
 
 // LDS dwords at a + 4 O0 and a + 4 O1
@@ -304,15 +307,13 @@ struct BiasGrad {
   float run[2];         // the lane's sums of the blocks past the reach, before and after
   float* mem;           // [waves][2][bias_entries]
 
-  static constexpr size_t lds_bytes(int reach, int /*buckets*/, int waves) {
-    return (size_t)waves * 2 * bias_entries(reach) * sizeof(float);
-  }
+  static size_t lds_bytes(const BiasX& x, int waves) { return (size_t)waves * 2 * bias_entries(x) * sizeof(float); }
 
   // (all threads; a barrier must follow)
   template <int HALF>
   __device__ __forceinline__ void init(const BiasX& x, float* m, int /*buckets*/, int wave, int waves) {
     static_assert(HALF == 8, "runs of 8 keys, the halves' 8 apart");
-    const int lane = lane_here(), j = lane & 15, qh = (lane >> 4) & 1, hl = lane >> 5, n = bias_entries(x.reach);
+    const int lane = lane_here(), j = lane & 15, qh = (lane >> 4) & 1, hl = lane >> 5, n = bias_entries(x);
     mem = m;
     run[0] = run[1] = 0.f;
     for (int i = 64 * wave + lane; i < waves * 2 * n; i += 64 * waves) m[i] = 0.f;
@@ -367,7 +368,7 @@ struct BiasGrad {
   // within). The running sums join their sides' outermost entries, which are of
   // the last bucket, a lane half's in its own array.
   __device__ __forceinline__ void finish(const BiasX& x, float* __restrict__ out, int /*buckets*/, int wave, int waves) {
-    const int lane = lane_here(), n = bias_entries(x.reach), hl = lane >> 5;
+    const int lane = lane_here(), n = bias_entries(x), hl = lane >> 5;
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
       float v = run[side];
@@ -402,9 +403,9 @@ struct BiasGradWide {
   float run[2];
   float* totals;
 
-  __host__ __device__ static constexpr int id_bytes(int reach) { return (bias_entries(reach) + 15) / 16 * 16; }
-  static constexpr size_t lds_bytes(int reach, int buckets, int waves) {
-    return id_bytes(reach) + waves * (kScratchB + 4 * (size_t)buckets);
+  __host__ __device__ __forceinline__ static int id_bytes(const BiasX& x) { return (bias_entries(x) + 15) / 16 * 16; }
+  static size_t lds_bytes(const BiasX& x, int waves) {
+    return id_bytes(x) + waves * (kScratchB + 4 * (size_t)x.buckets());
   }
 
   // (all threads; a barrier must follow)
@@ -412,14 +413,14 @@ struct BiasGradWide {
   __device__ __forceinline__ void init(const BiasX& x, float* m, int buckets, int wave, int waves) {
     const int lane = lane_here();
     unsigned char* id = (unsigned char*)m + waves * kScratchB;
-    totals = (float*)(id + id_bytes(x.reach));
+    totals = (float*)(id + id_bytes(x));
     scratch = lds_off((unsigned char*)m + wave * kScratchB);
     hist = lds_off(totals + wave * buckets);
     const int zero = x.reach + kBiasMargin;
     bias_spread(x, 64 * waves, [](int b) CA_INLINE { return b; },
                 [&](int e, int b) CA_INLINE { id[e] = (unsigned char)b; });
     if (x.one_sided)  // (keys after their query: masked)
-      for (int i = 1 + 64 * wave + lane; i < zero; i += 64 * waves) id[zero + i] = 0;
+      for (int i = 1 + 64 * wave + lane; i < kBiasMargin; i += 64 * waves) id[zero + i] = 0;
     for (int i = lane; i < buckets; i += 64) totals[wave * buckets + i] = 0.f;
     for (int i = lane; i < kScratchB / 4; i += 64) m[wave * (kScratchB / 4) + i] = 0.f;
     ids = lds_off(id + zero);

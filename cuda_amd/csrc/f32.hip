@@ -652,7 +652,7 @@ hipError_t launch_cross_f32(const void* q, const void* k, const void* v, void* o
     return hipErrorInvalidValue;
   }
   const BiasX x = bias_x(s, *bias, s.scale, kLog2e);
-  const size_t lds = bias_lds_bytes(x.reach);
+  const size_t lds = bias_lds_bytes(x);
   if (s.D == 64) return causal ? CA_F32_CASE(64, true, x, lds) : CA_F32_CASE(64, false, x, lds);
   if (s.D == 128) return causal ? CA_F32_CASE(128, true, x, lds) : CA_F32_CASE(128, false, x, lds);
 #undef CA_F32_CASE
