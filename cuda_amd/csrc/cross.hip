@@ -488,10 +488,16 @@ struct CrossPlan {
 };
 
 // Row groups per workgroup (8, 4, 2) and, where those leave the chip idle,
-// splits of the key walk. Times in 0.1 us, as in prefill_rows.hip: a key step of
-// a workgroup (64 keys of 8 groups; 128 of 4; 128, at D = 64 256, of 2) and what
-// a tile costs beside its steps; a launch takes its busiest CU's. A split launch
-// also writes and reads its partials and launches the merge.
+// splits of the key walk. Times in 0.1 us: a key step of a workgroup (64 keys of 8
+// groups; 128 of 4; 128, at D = 64 256, of 2) and what a tile costs beside its
+// steps, its first keys' way from HBM among it; a launch takes its busiest CU's
+// rounds (of 2 groups, which fetch K and V most often, a fifth more where there is
+// more than one). A split launch also writes and reads its partials and launches
+// the merge. Fitted to 11 shapes x 3 group counts x 7 splits; the choice was
+// within 8 % of the best there: 8 kv heads x 200 rows x 4001 keys x 128, 2 groups,
+// 8 splits 17.7 us (8 groups unsplit 87, 2 unsplit 38, 2 x 16 25); 32 heads x 200 x
+// 1500 x 64, 2 groups unsplit 12.3 (8: 26; 2 x 4: 19); 4 x 6000 x 6000 x 64, 4
+// groups unsplit 52 (8: 87, 2: 64).
 CrossPlan cross_plan(long long n_bh, int rows, int Skv, int D, bool bias, bool causal) {
   const double cus = std::max(device_cus(), 1);
   const bool d64 = D == 64;
@@ -499,8 +505,12 @@ CrossPlan cross_plan(long long n_bh, int rows, int Skv, int D, bool bias, bool c
   double best_cost = 0;
   for (int groups = 8; groups >= 2; groups /= 2) {
     const int keys = groups == 8 ? 64 : groups == 4 || !d64 ? 128 : 256;
-    const double step = groups == 8 ? (d64 ? 9 : 11) : groups == 4 ? (d64 ? 12 : 17) : (d64 ? 10.5 : 13);
-    const double tile = (groups == 8 ? 30 : groups == 4 ? 28 : 39) + (bias ? 10 : 0);
+    const double step = groups == 8 ? (d64 ? 9 : 12) : groups == 4 ? (d64 ? 10 : 14.5) : (d64 ? 10 : 10.5);
+    const double tile = (groups == 8 ? (d64 ? 40 : 45) : groups == 4 ? 31 : 29) + (bias ? 8 : 0);
+    auto rounds = [&](double wgs) {
+      const double r = std::ceil(wgs / cus);
+      return groups == 2 && r > 1 ? 1.2 * r : r;
+    };
     CrossPlan p;
     p.groups = groups;
     p.n_qt = (rows + 32 * groups - 1) / (32 * groups);
@@ -510,20 +520,20 @@ CrossPlan cross_plan(long long n_bh, int rows, int Skv, int D, bool bias, bool c
     if (causal) {
       // the mean of a causal tile's steps: half the longest's and a half step
       const double mean = tile + step * (0.5 * steps + 0.5), longest = tile + step * steps;
-      cost = p.order == kOrderPairs ? std::ceil(p.grid / cus) * 2 * mean
+      cost = p.order == kOrderPairs ? rounds((double)p.grid) * 2 * mean
                                     : std::max(longest, 1.1 * n_bh * p.n_qt * mean / cus);
     } else {
-      cost = std::ceil(p.grid / cus) * (tile + step * steps);
+      cost = rounds((double)p.grid) * (tile + step * steps);
       for (int n = 2; n <= std::min(kMaxSplits, steps); ++n) {
         const double bytes = 2.0 * n_bh * rows * n * D * 4;
-        const double c = std::ceil(p.grid * n / cus) * (tile + step * ((steps + n - 1) / n)) + 45 + bytes / 4e5;
-        if (c < 0.9 * cost) {
+        const double c = rounds((double)p.grid * n) * (tile + step * ((steps + n - 1) / n)) + 45 + bytes / 4e5;
+        if (c < 0.95 * cost) {
           cost = c;
           p.n_split = n;
         }
       }
     }
-    if (groups == 8 || cost < 0.9 * best_cost) {
+    if (groups == 8 || cost < 0.95 * best_cost) {
       best = p;
       best_cost = cost;
     }
