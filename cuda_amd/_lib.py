@@ -34,10 +34,10 @@ SIGNATURES = {
     "ca_cross_attention_workspace_bytes": (_Z, [_I, _I, _I, _I, _I, _I, _I, _I]),
     "ca_cross_attention_bwd": (_I, [_I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P,
                                     _Z, _P]),
-    "ca_relative_bias_attention": (_I, [_I, _P, _P, _P, _P, _I, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I,
+    "ca_relative_bias_attention": (_I, [_I, _P, _P, _P, _P, _I, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I,
                                         _P, _Z, _P]),
     "ca_relative_bias_attention_workspace_bytes": (_Z, [_I, _I, _I, _I, _I, _I, _I, _I]),
-    "ca_relative_bias_attention_bwd": (_I, [_I, _P, _P, _P, _P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I,
+    "ca_relative_bias_attention_bwd": (_I, [_I, _P, _P, _P, _P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I,
                                             _I, _I, _I, _I, _F, _I, _P, _Z, _P]),
     "ca_encoder_decoder_bwd_workspace_bytes": (_Z, [_I, _I, _I, _I]),
     "ca_relative_bias_decode": (_I, [_I, _P, _P, _P, _P, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _F, _P, _Z, _P]),

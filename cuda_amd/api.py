@@ -311,16 +311,17 @@ def _encdec_checks(q, k, v, kv_lens):
         _check(kv_lens.dim() == 1 and kv_lens.numel() == b, "kv_lens must be [batch]")
         _check(not kv_lens.is_floating_point() and not kv_lens.is_complex() and kv_lens.dtype != torch.bool,
                "kv_lens must hold integers")
-        kv_lens = kv_lens.to(torch.int32).contiguous()
+        if kv_lens.dtype != torch.int32:
+            kv_lens = kv_lens.clamp(0, skv).to(torch.int32)
+        kv_lens = kv_lens.contiguous()
     return b, hq, hkv, sq, skv, d, kv_lens
 
 
-@functools.lru_cache(maxsize=64)
+@functools.lru_cache(maxsize=None)   # (its address stays good: callers keep that alone)
 def _bucket_starts(num_buckets, is_causal, max_distance):
-    """First distance of each bucket of a side, as the C ABI takes them, and its
-    address: the
-    first half of the side's buckets hold one distance each, the others
-    distances that grow as a power up to max_distance: bucket e + j starts at
+    """First distance of each bucket of a side, as the C ABI takes them, and the
+    address of it: the first half of the side's buckets hold one distance each,
+    the others distances that grow as a power up to max_distance: bucket e + j starts at
     the first n with (n / e) ** span >= (max_distance / e) ** j, e buckets
     below it and span from it on, found in whole numbers."""
     side = num_buckets if is_causal else num_buckets // 2
@@ -361,8 +362,9 @@ def _starts_address(bias_table, is_causal, max_distance):
     return _bucket_starts(bias_table.shape[0], bool(is_causal), max_distance)[1]
 
 
-def _encdec_forward(q, k, v, kv_lens, softmax_scale, want_lse, bias=None, is_causal=False):
-    """(out, lse or None); bias: (table, max_distance) or None."""
+def _encdec_forward(q, k, v, kv_lens, softmax_scale, want_lse, bias=None, is_causal=False, want_low=False):
+    """(out, lse or None), with want_low (out, lse, low); bias: (table,
+    max_distance) or None."""
     b, hq, hkv, sq, skv, d, lens = _encdec_checks(q, k, v, kv_lens)
     what = "Cross Attention" if bias is None else "Relative Bias Attention"
     dt = _dtype_code(q, what)
@@ -379,16 +381,18 @@ def _encdec_forward(q, k, v, kv_lens, softmax_scale, want_lse, bias=None, is_cau
             _lib.call("ca_cross_attention", dt, _ptr(q), _ptr(k), _ptr(v), _ptr(lens), _ptr(out), _ptr(lse),
                       b, hq, hkv, sq, skv, d, _scale(softmax_scale, d), _ptr(ws), nbytes, _stream())
         else:
+            low = torch.empty_like(q) if want_low and dt != _lib.CA_F32 else None
             nbytes = lib.ca_relative_bias_attention_workspace_bytes(dt, b, hq, hkv, sq, skv, d, int(bool(is_causal)))
             ws, nbytes = _workspace(nbytes, q.device)
             _lib.call("ca_relative_bias_attention", dt, _ptr(q), _ptr(k), _ptr(v), _ptr(table),
-                      _DT[table.dtype], starts, table.shape[0], _ptr(lens), _ptr(out), _ptr(lse), b, hq, hkv, sq, skv, d,
+                      _DT[table.dtype], starts, table.shape[0], _ptr(lens), _ptr(out), _ptr(low), _ptr(lse), b,
+                      hq, hkv, sq, skv, d,
                       _scale(softmax_scale, d), int(bool(is_causal)), _ptr(ws), nbytes, _stream())
-    return out, lse
+    return (out, lse, low) if want_low else (out, lse)
 
 
-def _encdec_backward(dout, q, k, v, out, lse, kv_lens, softmax_scale, bias=None, is_causal=False):
-    """[dq, dk, dv] (with a bias, and dtable)."""
+def _encdec_backward(dout, q, k, v, out, lse, kv_lens, softmax_scale, bias=None, is_causal=False, low=None):
+    """[dq, dk, dv] (with a bias, and dtable). low: what out's rounding took."""
     b, hq, hkv, sq, skv, d, lens = _encdec_checks(q, k, v, kv_lens)
     for t in (dout, out, lse):
         _check(t.is_cuda and t.device == q.device, "Inputs must be on one device")
@@ -413,7 +417,7 @@ def _encdec_backward(dout, q, k, v, out, lse, kv_lens, softmax_scale, bias=None,
         dtable = torch.empty_like(table)
         _lib.call("ca_relative_bias_attention_bwd", dt, _ptr(q), _ptr(k), _ptr(v), _ptr(table),
                   _DT[table.dtype], starts, n_buckets,
-                  _ptr(lens), _ptr(out), _ptr(dout), _ptr(lse), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dtable), b, hq,
+                  _ptr(lens), _ptr(out), _ptr(low), _ptr(dout), _ptr(lse), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dtable), b, hq,
                   hkv, sq, skv, d, _scale(softmax_scale, d), int(bool(is_causal)), _ptr(ws), nbytes, _stream())
     return [dq, dk, dv, dtable]
 
@@ -512,28 +516,40 @@ def relative_bias_attention_backward(dout, q, k, v, out, lse, bias_table, kv_len
     """[dq, dk, dv, dtable] of relative_bias_attention_forward, given its output,
     the gradient of it and its LSE. dtable, of bias_table's type, is summed over
     the batch in an order that does not depend on timing."""
+    return _bias_backward(dout, q, k, v, out, lse, None, bias_table, kv_lens, is_causal, softmax_scale, max_distance)
+
+
+def _bias_backward(dout, q, k, v, out, lse, low, bias_table, kv_lens, is_causal, softmax_scale, max_distance):
     res = _native().relative_bias_attention_backward(dout, q, k, v, out, lse, bias_table, kv_lens, is_causal,
                                                      softmax_scale,
-                                                     _starts_address(bias_table, is_causal, max_distance))
+                                                     _starts_address(bias_table, is_causal, max_distance), low)
     if res is not None:
         return res
-    return _encdec_backward(dout, q, k, v, out, lse, kv_lens, softmax_scale, (bias_table, max_distance), is_causal)
+    return _encdec_backward(dout, q, k, v, out, lse, kv_lens, softmax_scale, (bias_table, max_distance), is_causal,
+                            low)
 
 
 class _RelativeBiasAttention(torch.autograd.Function):
+    """With a 16-bit output the forward also keeps what its rounding took: the
+    backward's rowsum(dout * out) otherwise has that error, which the table's
+    gradient, sums of terms that nearly cancel, shows."""
+
     @staticmethod
     def forward(ctx, q, k, v, bias_table, kv_lens, is_causal, softmax_scale, max_distance):
-        out, lse = relative_bias_attention_forward_lse(q, k, v, bias_table, kv_lens, is_causal, softmax_scale,
-                                                       max_distance)
-        ctx.save_for_backward(q, k, v, out, lse, bias_table, kv_lens)
+        res = _native().relative_bias_attention_forward_train(q, k, v, bias_table, kv_lens, is_causal, softmax_scale,
+                                                              _starts_address(bias_table, is_causal, max_distance))
+        if res is None:
+            res = _encdec_forward(q, k, v, kv_lens, softmax_scale, True, (bias_table, max_distance), is_causal, True)
+        out, lse, low = res if len(res) == 3 else (*res, None)
+        ctx.save_for_backward(q, k, v, out, lse, low, bias_table, kv_lens)
         ctx.rest = is_causal, softmax_scale, max_distance
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse, table, kv_lens = ctx.saved_tensors
-        grads = relative_bias_attention_backward(dout.contiguous(), q, k, v, out, lse, table, kv_lens, *ctx.rest)
+        q, k, v, out, lse, low, table, kv_lens = ctx.saved_tensors
+        grads = _bias_backward(dout.contiguous(), q, k, v, out, lse, low, table, kv_lens, *ctx.rest)
         return (*grads, None, None, None, None)
 
 

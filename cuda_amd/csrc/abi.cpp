@@ -227,7 +227,7 @@ static ca_status encdec_shape(const char* what, ca_dtype dtype, int batch, int h
   return CA_OK;
 }
 
-static ca_status bias_spec(const char* what, const void* table, ca_dtype table_dtype, const int32_t* starts, int num_buckets,
+static ca_status bias_spec(const char* what, ca_dtype dtype, void* o_low, const void* table, ca_dtype table_dtype, const int32_t* starts, int num_buckets,
                            bool one_sided, ca::BiasSpec* b) {
   if (num_buckets < 1 || num_buckets > 256 || (!one_sided && num_buckets % 2))
     return fail(CA_INVALID_ARGUMENT, "%s: num_buckets must be in [1, 256], and even when not causal (got %d)", what,
@@ -240,7 +240,10 @@ static ca_status bias_spec(const char* what, const void* table, ca_dtype table_d
   for (int i = 1; i < side; ++i)
     if (starts[i] < starts[i - 1] || starts[i] > 2048)
       return fail(CA_INVALID_ARGUMENT, "%s: bucket_starts must not fall, and stay within 2048", what);
-  *b = ca::BiasSpec{table, (int)table_dtype, side, one_sided, starts};
+  if (o_low && dtype == CA_F32)
+    return fail(CA_INVALID_ARGUMENT, "%s: o_low is for 16-bit outputs", what);
+  if (!aligned16(o_low)) return fail(CA_INVALID_ARGUMENT, "%s: pointers must be 16-byte aligned", what);
+  *b = ca::BiasSpec{table, (int)table_dtype, side, one_sided, starts, o_low};
   return CA_OK;
 }
 
@@ -347,7 +350,7 @@ ca_status ca_cross_attention_bwd(ca_dtype dtype, const void* q, const void* k, c
 
 ca_status ca_relative_bias_attention(ca_dtype dtype, const void* q, const void* k, const void* v,
                                      const void* bias_table, ca_dtype table_dtype, const int32_t* bucket_starts, int num_buckets,
-                                     const int32_t* kv_lens, void* o, float* lse, int batch, int num_q_heads,
+                                     const int32_t* kv_lens, void* o, void* o_low, float* lse, int batch, int num_q_heads,
                                      int num_kv_heads, int q_len, int kv_len, int head_dim, float softmax_scale,
                                      int is_causal, void* workspace, size_t workspace_bytes, void* stream) {
   const char* what = "relative_bias_attention";
@@ -356,13 +359,13 @@ ca_status ca_relative_bias_attention(ca_dtype dtype, const void* q, const void* 
   ca_status st = encdec_shape(what, dtype, batch, num_q_heads, num_kv_heads, q_len, kv_len, head_dim, softmax_scale,
                               kv_lens, &s);
   if (st != CA_OK) return st;
-  if ((st = bias_spec(what, bias_table, table_dtype, bucket_starts, num_buckets, is_causal != 0, &b)) != CA_OK) return st;
+  if ((st = bias_spec(what, dtype, o_low, bias_table, table_dtype, bucket_starts, num_buckets, is_causal != 0, &b)) != CA_OK) return st;
   return encdec_forward(what, dtype, q, k, v, o, lse, s, &b, is_causal != 0, workspace, workspace_bytes, stream);
 }
 
 ca_status ca_relative_bias_attention_bwd(ca_dtype dtype, const void* q, const void* k, const void* v,
                                          const void* bias_table, ca_dtype table_dtype, const int32_t* bucket_starts, int num_buckets,
-                                         const int32_t* kv_lens, const void* o, const void* dout, const float* lse,
+                                         const int32_t* kv_lens, const void* o, const void* o_low, const void* dout, const float* lse,
                                          void* dq, void* dk, void* dv, void* dtable, int batch, int num_q_heads,
                                          int num_kv_heads, int q_len, int kv_len, int head_dim, float softmax_scale,
                                          int is_causal, void* workspace, size_t workspace_bytes, void* stream) {
@@ -372,7 +375,7 @@ ca_status ca_relative_bias_attention_bwd(ca_dtype dtype, const void* q, const vo
   ca_status st = encdec_shape(what, dtype, batch, num_q_heads, num_kv_heads, q_len, kv_len, head_dim, softmax_scale,
                               kv_lens, &s);
   if (st != CA_OK) return st;
-  if ((st = bias_spec(what, bias_table, table_dtype, bucket_starts, num_buckets, is_causal != 0, &b)) != CA_OK) return st;
+  if ((st = bias_spec(what, dtype, const_cast<void*>(o_low), bias_table, table_dtype, bucket_starts, num_buckets, is_causal != 0, &b)) != CA_OK) return st;
   return encdec_backward(what, dtype, q, k, v, o, dout, lse, dq, dk, dv, dtable, s, &b, is_causal != 0, workspace,
                          workspace_bytes, stream);
 }
@@ -388,7 +391,7 @@ ca_status ca_relative_bias_decode(ca_dtype dtype, const void* q, const void* k, 
   ca_status st = encdec_shape(what, dtype, batch, num_q_heads, num_kv_heads, 1, kv_len, head_dim, softmax_scale,
                               context_lens, &s);
   if (st != CA_OK) return st;
-  if ((st = bias_spec(what, bias_table, table_dtype, bucket_starts, num_buckets, true, &b)) != CA_OK) return st;
+  if ((st = bias_spec(what, dtype, nullptr, bias_table, table_dtype, bucket_starts, num_buckets, true, &b)) != CA_OK) return st;
   if (batch == 0) return CA_OK;
   if ((st = check_pointers(what, {q, o}, true)) != CA_OK) return st;
   if ((st = check_pointers(what, {k, v}, kv_len > 0)) != CA_OK) return st;

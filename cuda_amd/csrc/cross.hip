@@ -38,6 +38,7 @@ struct CrossArgs {
   const uint16_t* k;
   const uint16_t* v;
   uint16_t* o;
+  uint16_t* o_low;  // what o's rounding took, or null
   float* lse;
   float* part_o;    // [rows of all groups][n_split][D], o / l, where n_split > 1
   float* part_lse;  // ... log2 of the sum of 2^x
@@ -403,25 +404,37 @@ __device__ CA_INLINE void cross_tile(const CrossArgs& a, const X& x, unsigned ch
     return;
   }
   if (a.lse && part == 0 && hl == 0 && q_in) a.lse[(size_t)bh * rows + myq] = row_lse(M, L);
-  // packed into the group's rows
+  // packed into the group's rows, which its KS waves store, 16 bytes a lane
   unsigned char* orows = lds + kMeetB + qg * 32 * kRowB;
 #pragma unroll
-  for (int j = 0; j < NR / 4; ++j) {
-    const vec2 lo = Tr::pack2(own[j][0] * inv, own[j][1] * inv), hi = Tr::pack2(own[j][2] * inv, own[j][3] * inv);
-    vec4 y;
-    y[0] = lo[0]; y[1] = lo[1]; y[2] = hi[0]; y[3] = hi[1];
-    const int c = part * (NR / 4) + j;  // 16-byte chunk: d = 8 c + 4 hl
-    *(u32x2*)(orows + l32 * kRowB + 16 * (c ^ (l32 % Gm::kLpr)) + 8 * hl) = __builtin_bit_cast(u32x2, y);
-  }
-  __syncthreads();
-  // the group's KS waves store its 32 rows, 16 bytes a lane
+  for (int j = 0; j < NR / 4; ++j) own[j] *= inv;
+  auto store_rows = [&](uint16_t* out) CA_INLINE {
 #pragma unroll
-  for (int j = 0; j < 32 * kRowB / 1024 / KS; ++j) {
-    const int p = 64 * (j * KS + part) + lane, r = p / Gm::kLpr, c = p % Gm::kLpr;
-    const int row = qw0 + r;
-    if (row < rows)
-      *(u32x4*)(a.o + ((size_t)bh * rows + row) * D + 8 * c) =
-          *(const u32x4*)(orows + r * kRowB + 16 * (c ^ (r % Gm::kLpr)));
+    for (int j = 0; j < NR / 4; ++j) {
+      const vec2 lo = Tr::pack2(own[j][0], own[j][1]), hi = Tr::pack2(own[j][2], own[j][3]);
+      vec4 y;
+      y[0] = lo[0]; y[1] = lo[1]; y[2] = hi[0]; y[3] = hi[1];
+      const int c = part * (NR / 4) + j;  // 16-byte chunk: d = 8 c + 4 hl
+      *(u32x2*)(orows + l32 * kRowB + 16 * (c ^ (l32 % Gm::kLpr)) + 8 * hl) = __builtin_bit_cast(u32x2, y);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 32 * kRowB / 1024 / KS; ++j) {
+      const int p = 64 * (j * KS + part) + lane, r = p / Gm::kLpr, c = p % Gm::kLpr;
+      const int row = qw0 + r;
+      if (row < rows)
+        *(u32x4*)(out + ((size_t)bh * rows + row) * D + 8 * c) =
+            *(const u32x4*)(orows + r * kRowB + 16 * (c ^ (r % Gm::kLpr)));
+    }
+  };
+  store_rows(a.o);
+  if (BIAS && a.o_low) {
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < NR / 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) own[j][e] -= (float)Tr::pack2(own[j][e], 0.f)[0];
+    store_rows(a.o_low);
   }
 }
 
@@ -448,8 +461,8 @@ constexpr int kMaxSplits = 16;
 template <typename Tr, int D>
 __global__ __launch_bounds__(256) void cross_merge_kernel(const float* __restrict__ part_o,
                                                           const float* __restrict__ part_lse,
-                                                          uint16_t* __restrict__ o, float* __restrict__ lse,
-                                                          long long n_rows, int n_split) {
+                                                          uint16_t* __restrict__ o, uint16_t* __restrict__ o_low,
+                                                          float* __restrict__ lse, long long n_rows, int n_split) {
   constexpr int PER = D / 64;
   const int lane = threadIdx.x & 63;
   const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -478,7 +491,11 @@ __global__ __launch_bounds__(256) void cross_merge_kernel(const float* __restric
     }
   const float inv = W > 0.f ? 1.f / W : 0.f;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) Tr::store(o, row * D + PER * lane + i, acc[i] * inv);
+  for (int i = 0; i < PER; ++i) {
+    const float x = acc[i] * inv;
+    Tr::store(o, row * D + PER * lane + i, x);
+    if (o_low) Tr::store(o_low, row * D + PER * lane + i, x - (float)Tr::pack2(x, 0.f)[0]);
+  }
   if (lse && lane == 0) lse[row] = row_lse(M, W);
 }
 
@@ -554,7 +571,7 @@ hipError_t launch_t(CrossArgs a, const X& x, const CrossPlan& p, size_t lds, hip
   const long long n_rows = (long long)a.n_bh * a.rows, wgs = (n_rows + 3) / 4;
   if (wgs > 0x7fffffffLL / 256) return hipErrorInvalidValue;
   hipLaunchKernelGGL((cross_merge_kernel<Tr, D>), dim3((unsigned)wgs), dim3(256), 0, stream, a.part_o, a.part_lse,
-                     a.o, a.lse, n_rows, p.n_split);
+                     a.o, a.o_low, a.lse, n_rows, p.n_split);
   return hipGetLastError();
 }
 
@@ -596,7 +613,8 @@ hipError_t launch_cross(int dtype, const void* q, const void* k, const void* v, 
   if ((long long)s.B * s.Hq * s.Sq == 0) return hipSuccess;
   if (few_rows(s, bias, lse)) return launch_encdec_decode(dtype, q, k, v, o, s, nullptr, ws, ws_bytes, stream);
   if (dtype == kDtypeF32) return launch_cross_f32(q, k, v, o, lse, s, bias, causal, stream);
-  CrossArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (uint16_t*)o, lse};
+  CrossArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (uint16_t*)o,
+              bias ? (uint16_t*)bias->o_low : nullptr, lse};
   const CrossRows r(s, bias);
   if (r.n_bh > 0x7fffffffLL) return hipErrorInvalidValue;
   a.rows = r.rows;

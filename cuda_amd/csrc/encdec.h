@@ -47,7 +47,7 @@ struct CrossX {
   // has all sequences in it, whatever their lengths; where 8 divides per_b, an XCD
   // takes its heads of the longest sequence first, and the short ones fill the end.
   // (4 x 32 heads x 2048 queries, 1792 to 4096 keys: 466 us head by head, when two
-  // XCDs had the longest sequence to themselves; 383 apart; LPTFIG longest first.)
+  // XCDs had the longest sequence to themselves; 383 apart; 360 longest first.)
   struct Head {
     int bh, n_keys;  // the head, its sequence's keys
   };

@@ -85,6 +85,7 @@ struct BiasSpec {
   int side;
   bool one_sided;
   const int32_t* first;
+  void* o_low;  // 16-bit: what o's rounding took, [B, Hq, Sq, D], or null
   int buckets() const { return one_sided ? side : 2 * side; }
 };
 // Forward (cross.hip; float32: f32.hip); bias may be null. ws holds

@@ -432,7 +432,7 @@ bool bias_of(PyObject* to, PyObject* address, const at::Tensor& q, const at::Ten
   return *starts != nullptr;
 }
 
-PyObject* bias_forward(PyObject* const* a, bool want_lse) {
+PyObject* bias_forward(PyObject* const* a, bool want_lse, bool want_low) {
   EncDec x;
   const at::Tensor* t;
   ca_dtype tdt;
@@ -441,38 +441,49 @@ PyObject* bias_forward(PyObject* const* a, bool want_lse) {
   if (!x.take(a[0], a[1], a[2], a[4], a[6]) || !bias_of(a[3], a[7], *x.q, t, &tdt, &starts) || !flag_of(a[5], &causal))
     return nullptr;
   const at::Tensor &q = *x.q, &k = *x.k, o = like(q);
-  at::Tensor lse;
+  at::Tensor lse, low;
   if (want_lse) lse = x.lse();
+  if (x.dt == CA_F32) want_low = false;
+  if (want_low) low = like(q);
   const Workspace ws(abi.relative_bias_attention_workspace_bytes(x.dt, n(q, 0), n(q, 1), n(k, 1), n(q, 2), n(k, 2),
                                                                  n(q, 3), causal), q);
   if (!ok([&] {
         return abi.relative_bias_attention(x.dt, in(q), in(k), in(*x.v), in(*t), tdt, starts, n(*t, 0), x.kv_lens(),
-                                           out(o), want_lse ? (float*)out(lse) : nullptr, n(q, 0), n(q, 1), n(k, 1),
+                                           out(o), want_low ? out(low) : nullptr, want_lse ? (float*)out(lse) : nullptr,
+                                           n(q, 0), n(q, 1), n(k, 1),
                                            n(q, 2), n(k, 2), n(q, 3), x.scale, causal, ws.ptr(), ws.bytes, stream());
       }))
     return nullptr;
   if (!want_lse) return THPVariable_Wrap(o);
+  if (want_low) return Py_BuildValue("(NNN)", THPVariable_Wrap(o), THPVariable_Wrap(lse), THPVariable_Wrap(low));
   return Py_BuildValue("(NN)", THPVariable_Wrap(o), THPVariable_Wrap(lse));
 }
 // (q, k, v, bias_table, kv_lens, is_causal, softmax_scale, address of the bucket starts) -> out or (out, lse)
-PyObject* relative_bias_attention_forward(PyObject* const* a) { return bias_forward(a, false); }
-PyObject* relative_bias_attention_forward_lse(PyObject* const* a) { return bias_forward(a, true); }
+PyObject* relative_bias_attention_forward(PyObject* const* a) { return bias_forward(a, false, false); }
+PyObject* relative_bias_attention_forward_lse(PyObject* const* a) { return bias_forward(a, true, false); }
+// ... -> (out, lse, low) (float32: (out, lse))
+PyObject* relative_bias_attention_forward_train(PyObject* const* a) { return bias_forward(a, true, true); }
 
-// (dout, q, k, v, out, lse, bias_table, kv_lens, is_causal, softmax_scale, address) -> [dq, dk, dv, dtable]
+// (dout, q, k, v, out, lse, bias_table, kv_lens, is_causal, softmax_scale, address, low or None)
+// -> [dq, dk, dv, dtable]
 PyObject* relative_bias_attention_backward(PyObject* const* a) {
   EncDec x;
-  const at::Tensor *g, *o, *l, *t;
+  const at::Tensor *g, *o, *l, *t, *low = nullptr;
   ca_dtype tdt;
   const int32_t* starts;
   int causal;
   if (!x.take(a[1], a[2], a[3], a[7], a[9]) || !x.backward(a[0], a[4], a[5], g, o, l) ||
       !bias_of(a[6], a[10], *x.q, t, &tdt, &starts) || !flag_of(a[8], &causal))
     return nullptr;
+  if (a[11] != Py_None && (!(low = plain(a[11], 4)) || low->sizes() != x.q->sizes() ||
+                           low->scalar_type() != x.q->scalar_type() || !EncDec::here(*low)))
+    return nullptr;
   const at::Tensor &q = *x.q, &k = *x.k, dq = like(q), dk = like(k), dv = like(*x.v), dt = like(*t);
   const Workspace ws(abi.encoder_decoder_bwd_workspace_bytes(n(q, 0), n(q, 1), n(q, 2), n(*t, 0)), q);
   if (!ok([&] {
         return abi.relative_bias_attention_bwd(x.dt, in(q), in(k), in(*x.v), in(*t), tdt, starts, n(*t, 0), x.kv_lens(),
-                                               in(*o), in(*g), (const float*)in(*l), out(dq), out(dk), out(dv), out(dt),
+                                               in(*o), low ? in(*low) : nullptr, in(*g), (const float*)in(*l), out(dq),
+                                               out(dk), out(dv), out(dt),
                                                n(q, 0), n(q, 1), n(k, 1), n(q, 2), n(k, 2), n(q, 3), x.scale, causal,
                                                ws.ptr(), ws.bytes, stream());
       }))
@@ -547,7 +558,8 @@ PyMethodDef methods[] = {{"bind", (PyCFunction)(void (*)(void))bind, METH_FASTCA
                          CA_FAST(cross_attention_backward, 8),
                          CA_FAST(relative_bias_attention_forward, 8),
                          CA_FAST(relative_bias_attention_forward_lse, 8),
-                         CA_FAST(relative_bias_attention_backward, 11),
+                         CA_FAST(relative_bias_attention_forward_train, 8),
+                         CA_FAST(relative_bias_attention_backward, 12),
                          CA_FAST(relative_bias_decode, 7),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -157,10 +157,13 @@ ca_status ca_cross_attention_bwd(ca_dtype dtype, const void* q, const void* k, c
  * bucket_starts, on the HOST, holds the first distance of each bucket of a
  * side: bucket_starts[0] = 0, never falling, at most 2048; distance n = |j - i|
  * is in the last bucket that starts at or before it. num_buckets <= 256.
+ * o_low (may be NULL; 16-bit o only): what the rounding of o took, rounded in
+ * turn, for the backward: its rowsum(dout o) otherwise has o's error, which the
+ * table's gradient, sums of terms that nearly cancel, shows.
  * workspace: ca_relative_bias_attention_workspace_bytes(...). */
 ca_status ca_relative_bias_attention(ca_dtype dtype, const void* q, const void* k, const void* v,
                                      const void* bias_table, ca_dtype table_dtype, const int32_t* bucket_starts,
-                                     int num_buckets, const int32_t* kv_lens, void* o, float* lse,
+                                     int num_buckets, const int32_t* kv_lens, void* o, void* o_low, float* lse,
                                      int batch, int num_q_heads, int num_kv_heads, int q_len,
                                      int kv_len, int head_dim, float softmax_scale, int is_causal,
                                      void* workspace, size_t workspace_bytes, void* stream);
@@ -175,7 +178,7 @@ size_t ca_relative_bias_attention_workspace_bytes(ca_dtype dtype, int batch, int
 ca_status ca_relative_bias_attention_bwd(ca_dtype dtype, const void* q, const void* k,
                                          const void* v, const void* bias_table, ca_dtype table_dtype,
                                          const int32_t* bucket_starts, int num_buckets,
-                                         const int32_t* kv_lens, const void* o, const void* dout,
+                                         const int32_t* kv_lens, const void* o, const void* o_low, const void* dout,
                                          const float* lse, void* dq, void* dk, void* dv,
                                          void* dtable, int batch, int num_q_heads,
                                          int num_kv_heads, int q_len, int kv_len, int head_dim,

@@ -129,8 +129,8 @@ GOOD = _starts(0, 1, 2, 5)
 
 
 def _bias(table=P, starts=GOOD, buckets=8, causal=0, sizes=SIZES, scale=0.1, dtype=L.CA_BF16, q=P,
-          table_dtype=L.CA_F32):
-    return L.load().ca_relative_bias_attention(dtype, q, P, P, table, table_dtype, starts, buckets, None, P, None, *sizes, scale,
+          table_dtype=L.CA_F32, low=None):
+    return L.load().ca_relative_bias_attention(dtype, q, P, P, table, table_dtype, starts, buckets, None, P, low, None, *sizes, scale,
                                                causal, P, 1 << 30, None)
 
 
@@ -158,6 +158,7 @@ def test_cross_refusals(kw, word):
     (dict(starts=_starts(0, 3, 2, 4)), "fall"), (dict(starts=_starts(0, 1, 2, 2049)), "2048"),
     (dict(starts=_starts(0, -1, 2, 3)), "fall"), (dict(scale=math.nan), "finite"), (dict(dtype=9), "dtype"),
     (dict(q=ODD), "aligned"), (dict(table_dtype=5), "dtype"),
+    (dict(dtype=L.CA_F32, low=P), "16-bit"), (dict(low=ODD), "aligned"),
 ])
 def test_bias_refusals(kw, word):
     assert _bias(**kw) == L.CA_INVALID_ARGUMENT
@@ -178,7 +179,7 @@ def test_backward_refusals():
 
     def bwd(lse=P, dq=P, ws=P, nbytes=1 << 30, scale=0.1, dtable=P, bias=True):
         if bias:
-            return lib.ca_relative_bias_attention_bwd(L.CA_BF16, P, P, P, P, L.CA_F32, GOOD, 8, None, P, P, lse, dq, P, P,
+            return lib.ca_relative_bias_attention_bwd(L.CA_BF16, P, P, P, P, L.CA_F32, GOOD, 8, None, P, None, P, lse, dq, P, P,
                                                       dtable, *SIZES, scale, 0, ws, nbytes, None)
         return lib.ca_cross_attention_bwd(L.CA_BF16, P, P, P, None, P, P, lse, dq, P, P, *SIZES, scale, ws, nbytes,
                                           None)
