@@ -37,7 +37,11 @@
 // attention (keys of another length; dK and dV of a sequence's padded keys are
 // 0) and of attention with a relative position bias: S starts as bias / scale in
 // the accumulators, and the dQ kernel, which has every dS, also sums them by
-// bucket (BiasGrad) for the gradient of the bias table.
+// bucket (BiasGrad) for the gradient of the bias table. What bounds them is what bounds
+// the self-attention's (LDS reads of the transposed operands beside the MFMAs), and
+// with a bias its reads and, in dQ, the sums by distance: 2 x 32 / 8 heads x 1000
+// queries x 1500 to 4096 keys x 128, dK/dV 250 us, dQ 171 (forward and backward
+// together 0.78 PFLOP/s); 8 x 16 x 1024 x 64 with a bias, 200 to 1024 keys, 102 and 63.
 #include <algorithm>
 
 #include "common.h"
@@ -56,8 +60,8 @@ __device__ __forceinline__ int rho32(int i) { return (i & 0x13) | ((i & 4) << 1)
 // per row, 8 elements each. X: rows without a key (LSE -inf) get +inf, with which
 // every P is 0. O_low (may be null): what O's rounding took. (With a bias: the
 // error of D goes into every dS of the row with one sign, and the table's gradient,
-// sums of dS that nearly cancel, shows it: 600 queries and keys, bf16, relative
-// error 5e-3, with O_low 2e-3.)
+// sums of dS that nearly cancel, shows it: with that rounding alone, in 64 bits, 600
+// queries and keys in bf16 have a relative error of 5e-3, with O_low 2e-3.)
 template <typename Tr, int D, class X>
 __global__ __launch_bounds__(256) void bwd_rowdot_kernel(const uint16_t* __restrict__ O,
                                                          const uint16_t* __restrict__ dO,

@@ -30,7 +30,12 @@
 // take their SPLIT form: a workgroup has 32 rows (queries, or keys), each wave
 // every fourth tile of their walk, staged in LDS of its own (no barriers), and
 // the waves add up at the end (2 x 8 heads x 300 queries x 1024 keys x 64: dQ
-// 120 -> 38 us, dK/dV 58 -> 46).
+// 120 -> 38 us, dK/dV 58 -> 46). Where both are SPLIT they are one launch, which
+// fills the CUs that either leaves idle (whole backward of the same, with two
+// workgroups a CU, 79 -> 69 us; 2 x 12 heads x 500 x 500 with a bias 114 -> 86; 8 / 2
+// heads x 700 x 700 182 -> 141).
+#include <algorithm>
+
 #include "common.h"
 #include "encdec.h"
 #include "launch.h"
@@ -161,23 +166,33 @@ __device__ __forceinline__ void sum_waves(f32x16 (&acc)[N], float* mem, int wave
   }
 }
 
+// Waves a SIMD: two of SPLIT at head dim 64, which then fit 256 registers (4 x 16
+// heads x 200 queries x 700 keys: 136 -> 106 us; with a bias, which takes more of
+// them, no gain).
+template <int D, class X, bool SPLIT>
+constexpr int kF32PerSimd = SPLIT && D == 64 && !X::kBias ? 2 : 1;
+
+// LDS of a workgroup: tiles of two tensors and their rows' (LSE log2 e, D) pairs,
+// two in turn (SPLIT: each wave's own).
+template <int D, bool SPLIT>
+using F32Tiles = float[SPLIT ? kF32Waves : 2][kF32Tile * (D + 4)];
+template <bool SPLIT>
+using F32Pairs = float[SPLIT ? kF32Waves : 2][2 * kF32Tile];
+
 // dQ: one workgroup = 128 queries of one (b, h) (SPLIT: 32). With a bias, the
 // sums of dS by bucket go to part_table [b, h][tile][buckets].
 template <int D, bool CAUSAL, class X, bool SPLIT>
-__global__ __launch_bounds__(kF32Waves * 64) void bwd_dq_f32_kernel(
-    const float* __restrict__ Q, const float* __restrict__ K, const float* __restrict__ V,
-    const float* __restrict__ dO, const float* __restrict__ LD, float* __restrict__ dQ, int S,
-    int Hq, int Hkv, float scale, int n_qt, int n_work, X x, float* __restrict__ part_table) {
-  extern __shared__ __attribute__((aligned(16))) unsigned char bias_mem[];
+__device__ CA_INLINE void bwd_dq_f32_tile(
+    const float* Q, const float* K, const float* V,
+    const float* dO, const float* LD, float* dQ, int S,
+    int Hq, int Hkv, float scale, int n_qt, int block, int n_work, const X& x, float* part_table,
+    F32Tiles<D, SPLIT>& Ks, F32Tiles<D, SPLIT>& Vs, unsigned char* bias_mem) {
   constexpr int BM = SPLIT ? 32 : 32 * kF32Waves;
   constexpr int HD = D / 2, NOB = D / 32;
   using St = Stage2<D, SPLIT ? 64 : kF32Waves * 64>;
   constexpr int KS = St::KS;
-  constexpr int kBufs = SPLIT ? kF32Waves : 2;  // a wave's own, or two in turn
-  __shared__ __attribute__((aligned(16))) float Ks[kBufs][kF32Tile * KS];
-  __shared__ __attribute__((aligned(16))) float Vs[kBufs][kF32Tile * KS];
 
-  const int work = xcd_remap(blockIdx.x, n_work);
+  const int work = xcd_remap(block, n_work);
   int bh = work / n_qt;
   if constexpr (X::kCross) bh = x.head(bh, Hq).bh;
   const int qt = n_qt - 1 - (work % n_qt);  // longest causal walks first
@@ -301,24 +316,31 @@ __global__ __launch_bounds__(kF32Waves * 64) void bwd_dq_f32_kernel(
   if (qvalid) store_rowT_f32<NOB>(dQ + (qoff + myq) * D, acc, hl, scale);
 }
 
+template <int D, bool CAUSAL, class X, bool SPLIT>
+__global__ __launch_bounds__(kF32Waves * 64, (kF32PerSimd<D, X, SPLIT>)) void bwd_dq_f32_kernel(
+    const float* __restrict__ Q, const float* __restrict__ K, const float* __restrict__ V,
+    const float* __restrict__ dO, const float* __restrict__ LD, float* __restrict__ dQ, int S,
+    int Hq, int Hkv, float scale, int n_qt, int n_work, X x, float* __restrict__ part_table) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char bias_mem[];
+  __shared__ __attribute__((aligned(16))) F32Tiles<D, SPLIT> Ks, Vs;
+  bwd_dq_f32_tile<D, CAUSAL, X, SPLIT>(Q, K, V, dO, LD, dQ, S, Hq, Hkv, scale, n_qt, blockIdx.x, n_work, x,
+                                       part_table, Ks, Vs, bias_mem);
+}
+
 // dK, dV: one workgroup = 128 keys of one (b, kv head) (SPLIT: 32); 32-query tiles
 // of every q head of the kv head.
 template <int D, bool CAUSAL, class X, bool SPLIT>
-__global__ __launch_bounds__(kF32Waves * 64) void bwd_dkv_f32_kernel(
-    const float* __restrict__ Q, const float* __restrict__ K, const float* __restrict__ V,
-    const float* __restrict__ dO, const float* __restrict__ LD, float* __restrict__ dK,
-    float* __restrict__ dV, int S, int Hq, int Hkv, float scale, int n_kt, int n_work, X x) {
-  extern __shared__ __attribute__((aligned(16))) unsigned char bias_mem[];
+__device__ CA_INLINE void bwd_dkv_f32_tile(
+    const float* Q, const float* K, const float* V,
+    const float* dO, const float* LD, float* dK,
+    float* dV, int S, int Hq, int Hkv, float scale, int n_kt, int block, int n_work, const X& x,
+    F32Tiles<D, SPLIT>& Qs, F32Tiles<D, SPLIT>& Gs, F32Pairs<SPLIT>& Ls, unsigned char* bias_mem) {
   constexpr int BK = SPLIT ? 32 : 32 * kF32Waves;
   constexpr int HD = D / 2, NOB = D / 32;
   using St = Stage2<D, SPLIT ? 64 : kF32Waves * 64>;
   constexpr int KS = St::KS;
-  constexpr int kBufs = SPLIT ? kF32Waves : 2;  // a wave's own, or two in turn
-  __shared__ __attribute__((aligned(16))) float Qs[kBufs][kF32Tile * KS];
-  __shared__ __attribute__((aligned(16))) float Gs[kBufs][kF32Tile * KS];  // dO
-  __shared__ __attribute__((aligned(16))) float Ls[kBufs][2 * kF32Tile];   // (LSE log2 e, D) pairs
 
-  const int work = xcd_remap(blockIdx.x, n_work);
+  const int work = xcd_remap(block, n_work);
   int bhk = work / n_kt;
   if constexpr (X::kCross) bhk = x.head(bhk, Hkv).bh;
   const int kt = work % n_kt;  // causal: the first key tiles have the longest query walks
@@ -381,7 +403,7 @@ __global__ __launch_bounds__(kF32Waves * 64) void bwd_dkv_f32_kernel(
 
   // the next tile is loaded beside this one's products, where there are registers
   // for it (SPLIT stages four times the rows a lane)
-  constexpr bool kAhead = !SPLIT || D == 64;
+  constexpr bool kAhead = !SPLIT || (D == 64 && kF32PerSimd<D, X, SPLIT> == 1);
   // With a bias the walk is one q head's tiles after the other's (LDS holds one
   // head's bias), otherwise all tiles at once.
   int g = 0;
@@ -475,12 +497,46 @@ __global__ __launch_bounds__(kF32Waves * 64) void bwd_dkv_f32_kernel(
   }
 }
 
+template <int D, bool CAUSAL, class X, bool SPLIT>
+__global__ __launch_bounds__(kF32Waves * 64, (kF32PerSimd<D, X, SPLIT>)) void bwd_dkv_f32_kernel(
+    const float* __restrict__ Q, const float* __restrict__ K, const float* __restrict__ V,
+    const float* __restrict__ dO, const float* __restrict__ LD, float* __restrict__ dK,
+    float* __restrict__ dV, int S, int Hq, int Hkv, float scale, int n_kt, int n_work, X x) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char bias_mem[];
+  __shared__ __attribute__((aligned(16))) F32Tiles<D, SPLIT> Qs, Gs;  // Q, dO
+  __shared__ __attribute__((aligned(16))) F32Pairs<SPLIT> Ls;
+  bwd_dkv_f32_tile<D, CAUSAL, X, SPLIT>(Q, K, V, dO, LD, dK, dV, S, Hq, Hkv, scale, n_kt,
+                                        blockIdx.x, n_work, x, Qs, Gs, Ls, bias_mem);
+}
+
+// Both in one launch, where both are SPLIT: the workgroups with the longer walks
+// first, the others behind them wherever a CU is free.
+template <int D, bool CAUSAL, class X>
+__global__ __launch_bounds__(kF32Waves * 64, (kF32PerSimd<D, X, true>)) void bwd_both_f32_kernel(
+    const float* __restrict__ Q, const float* __restrict__ K, const float* __restrict__ V,
+    const float* __restrict__ dO, const float* __restrict__ LD, float* __restrict__ dQ,
+    float* __restrict__ dK, float* __restrict__ dV, int S, int Hq, int Hkv, float scale, int n_qt, int n_kt,
+    int n_dq, int n_dkv, int dkv_first, X x, float* __restrict__ part_table) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char bias_mem[];
+  __shared__ __attribute__((aligned(16))) F32Tiles<D, true> As, Bs;
+  __shared__ __attribute__((aligned(16))) F32Pairs<true> Ls;
+  const int i = blockIdx.x, first = dkv_first ? n_dkv : n_dq;
+  if ((i < first) == (dkv_first != 0))
+    bwd_dkv_f32_tile<D, CAUSAL, X, true>(Q, K, V, dO, LD, dK, dV, S, Hq, Hkv, scale, n_kt,
+                                         dkv_first ? i : i - first, n_dkv, x, As, Bs, Ls, bias_mem);
+  else
+    bwd_dq_f32_tile<D, CAUSAL, X, true>(Q, K, V, dO, LD, dQ, S, Hq, Hkv, scale, n_qt,
+                                        dkv_first ? i - first : i, n_dq, x, part_table, As, Bs, bias_mem);
+}
+
 // Whether a launch over `heads` heads of `rows` rows takes 32 rows a workgroup,
 // their walk in four parts: where that shortens the busiest CU's work by a fifth,
 // and LDS holds the waves' tiles beside what a bias takes.
+bool bwd_f32_fits(int D, size_t bias_lds) {
+  return kF32Waves * (2 * kF32Tile * (D + 4) + 2 * kF32Tile) * sizeof(float) + bias_lds <= 160 * 1024;
+}
 bool bwd_f32_splits(long long heads, int rows, int D, size_t bias_lds) {
-  const size_t tiles = kF32Waves * (2 * kF32Tile * (D + 4) + 2 * kF32Tile) * sizeof(float);
-  if (tiles + bias_lds > 160 * 1024) return false;
+  if (!bwd_f32_fits(D, bias_lds)) return false;
   const long long cus = device_cus() > 0 ? device_cus() : 1;
   const long long whole = heads * ((rows + 127) / 128), split = heads * ((rows + 31) / 32);
   return 10 * ((split + cus - 1) / cus) < 8 * 4 * ((whole + cus - 1) / cus);
@@ -518,6 +574,20 @@ hipError_t launch_bwd_f32_t(const float* q, const float* k, const float* v, cons
                        lse, ws, rows);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
+  }
+  if constexpr (X::kCross) {
+    const size_t lds = std::max(dkv_lds, dq_lds);
+    if (bm == 32 && bk == 32 && gq + gk <= 0x7fffffffLL && bwd_f32_fits(D, lds)) {
+      // (walks in products of a tile: dQ's 3 over the keys, dK/dV's 4 over the kv head's queries)
+      const bool dkv_first = 4LL * (Hq / Hkv) * S > 3LL * Skv;
+      hipLaunchKernelGGL((bwd_both_f32_kernel<D, CAUSAL, X>), dim3((unsigned)(gq + gk)), dim3(kF32Waves * 64), lds,
+                         stream, q, k, v, dout, ws, dq, dk, dv, S, Hq, Hkv, scale, n_qt, n_kt, (int)gq, (int)gk,
+                         (int)dkv_first, x, part_table);
+      e = hipGetLastError();
+      if (e != hipSuccess) return e;
+      if constexpr (X::kBias) return launch_bias_grad(part_table, false, dtable, B, n_qt, x, stream);
+      return e;
+    }
   }
   if (gk > 0) {
     hipLaunchKernelGGL(dkvk, dim3((unsigned)gk), dim3(kF32Waves * 64), dkv_lds,

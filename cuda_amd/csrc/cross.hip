@@ -16,6 +16,13 @@
 //
 // The bias enters as the accumulators' start: S^T begins as bias / scale, so it
 // costs LDS reads (two dwords a lane for two logits) and no VALU work.
+//
+// What bounds it: long walks the matrix pipes with the softmax's VALU beside them.
+// bf16, 4 x 32 heads x 2048 queries x 1792 to 4096 keys x 128: 360 us, 1.10 PFLOP/s
+// (a large matrix product: 1.24 to 1.39); causal with a bias, 32 heads x 8192 x 64:
+// 320 us, 0.85 PFLOP/s (half the products a logit for the same exponential, and the
+// bias reads). Short ones the way of the first keys from HBM and the launch: 12
+// heads x 100 x 100 x 64 with a bias 7.7 us, of which an empty launch is 4.4.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -578,9 +585,11 @@ hipError_t launch_t(CrossArgs a, const X& x, const CrossPlan& p, size_t lds, hip
 }  // namespace
 
 // Whether a launch goes to decode's split walk: few enough query rows of a kv
-// head to be its heads, and no LSE, which that walk does not keep.
+// head to be its heads, and no LSE, which that walk does not keep. (64 x 16 heads x
+// 1 x 1500 keys x 64: 41 us, 5.8 TB/s, where tiles of 64 rows, nearly all of them
+// empty, pay a whole tile's products for each head.)
 static bool few_rows(const EncDecShape& s, bool bias, bool lse) {
-  return !bias && !lse && (long long)(s.Hq / s.Hkv) * s.Sq <= 16;
+  return !bias && !lse && (long long)(s.Hq / s.Hkv) * s.Sq <= 16 && (long long)s.B * s.Hq * s.Sq <= 0x7fffffff;
 }
 
 // A launch's rows: without positions a kv head's query heads are one run of rows.
