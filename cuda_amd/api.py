@@ -16,6 +16,9 @@ float32 q/k/v are accepted where the reference instantiates float (prefill,
 flash_decode, paged decode). ``flash_attention`` is differentiable (README.md:
 66-71) through ``flash_attention_backward`` (fp16 / bf16 / float32, as the
 reference instantiates it).
+
+Without a counterpart there: the attention of encoder-decoder models
+(``cross_attention``, ``relative_bias_attention``, ``relative_bias_decode``).
 """
 import ctypes
 import functools
