@@ -315,7 +315,7 @@ def _encdec_checks(q, k, v, kv_lens):
         _check(not kv_lens.is_floating_point() and not kv_lens.is_complex() and kv_lens.dtype != torch.bool,
                "kv_lens must hold integers")
         if kv_lens.dtype != torch.int32:
-            kv_lens = kv_lens.clamp(0, skv).to(torch.int32)
+            kv_lens = kv_lens.long().clamp(0, skv).to(torch.int32)
         kv_lens = kv_lens.contiguous()
     return b, hq, hkv, sq, skv, d, kv_lens
 

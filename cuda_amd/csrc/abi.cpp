@@ -8,6 +8,7 @@
 // launching, e.g. flash_attention_v2_kernel.cuh:233-304).
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -227,8 +228,8 @@ static ca_status encdec_shape(const char* what, ca_dtype dtype, int batch, int h
   return CA_OK;
 }
 
-static ca_status bias_spec(const char* what, ca_dtype dtype, void* o_low, const void* table, ca_dtype table_dtype, const int32_t* starts, int num_buckets,
-                           bool one_sided, ca::BiasSpec* b) {
+static ca_status bias_spec(const char* what, ca_dtype dtype, void* o_low, const void* table, ca_dtype table_dtype,
+                           const int32_t* starts, int num_buckets, bool one_sided, ca::BiasSpec* b) {
   if (num_buckets < 1 || num_buckets > 256 || (!one_sided && num_buckets % 2))
     return fail(CA_INVALID_ARGUMENT, "%s: num_buckets must be in [1, 256], and even when not causal (got %d)", what,
                 num_buckets);
@@ -266,6 +267,7 @@ static ca_status check_workspace(const char* what, const void* ws, size_t given,
 static bool encdec_sizes_ok(ca_dtype dtype, int batch, int hq, int hkv, int q_len, int kv_len, int head_dim) {
   return (dtype == CA_BF16 || dtype == CA_F16 || dtype == CA_F32) && batch > 0 && hq > 0 && hkv > 0 && hq % hkv == 0 &&
          q_len > 0 && kv_len > 0 && (head_dim == 64 || head_dim == 128) &&
+         (long long)std::max(q_len, kv_len) * head_dim * 4 <= INT_MAX &&
          product_at_most(1LL << 40, {batch, hq, q_len, head_dim}) &&
          product_at_most(1LL << 40, {batch, hkv, kv_len, head_dim}) && (long long)batch * hq <= INT_MAX;
 }
@@ -349,9 +351,9 @@ ca_status ca_cross_attention_bwd(ca_dtype dtype, const void* q, const void* k, c
 }
 
 ca_status ca_relative_bias_attention(ca_dtype dtype, const void* q, const void* k, const void* v,
-                                     const void* bias_table, ca_dtype table_dtype, const int32_t* bucket_starts, int num_buckets,
-                                     const int32_t* kv_lens, void* o, void* o_low, float* lse, int batch, int num_q_heads,
-                                     int num_kv_heads, int q_len, int kv_len, int head_dim, float softmax_scale,
+                                     const void* bias_table, ca_dtype table_dtype, const int32_t* bucket_starts,
+                                     int num_buckets, const int32_t* kv_lens, void* o, void* o_low, float* lse,
+                                     int batch, int num_q_heads, int num_kv_heads, int q_len, int kv_len, int head_dim, float softmax_scale,
                                      int is_causal, void* workspace, size_t workspace_bytes, void* stream) {
   const char* what = "relative_bias_attention";
   ca::EncDecShape s;
@@ -359,13 +361,15 @@ ca_status ca_relative_bias_attention(ca_dtype dtype, const void* q, const void* 
   ca_status st = encdec_shape(what, dtype, batch, num_q_heads, num_kv_heads, q_len, kv_len, head_dim, softmax_scale,
                               kv_lens, &s);
   if (st != CA_OK) return st;
-  if ((st = bias_spec(what, dtype, o_low, bias_table, table_dtype, bucket_starts, num_buckets, is_causal != 0, &b)) != CA_OK) return st;
+  st = bias_spec(what, dtype, o_low, bias_table, table_dtype, bucket_starts, num_buckets, is_causal != 0, &b);
+  if (st != CA_OK) return st;
   return encdec_forward(what, dtype, q, k, v, o, lse, s, &b, is_causal != 0, workspace, workspace_bytes, stream);
 }
 
 ca_status ca_relative_bias_attention_bwd(ca_dtype dtype, const void* q, const void* k, const void* v,
-                                         const void* bias_table, ca_dtype table_dtype, const int32_t* bucket_starts, int num_buckets,
-                                         const int32_t* kv_lens, const void* o, const void* o_low, const void* dout, const float* lse,
+                                         const void* bias_table, ca_dtype table_dtype,
+                                         const int32_t* bucket_starts, int num_buckets, const int32_t* kv_lens,
+                                         const void* o, const void* o_low, const void* dout, const float* lse,
                                          void* dq, void* dk, void* dv, void* dtable, int batch, int num_q_heads,
                                          int num_kv_heads, int q_len, int kv_len, int head_dim, float softmax_scale,
                                          int is_causal, void* workspace, size_t workspace_bytes, void* stream) {
@@ -375,14 +379,16 @@ ca_status ca_relative_bias_attention_bwd(ca_dtype dtype, const void* q, const vo
   ca_status st = encdec_shape(what, dtype, batch, num_q_heads, num_kv_heads, q_len, kv_len, head_dim, softmax_scale,
                               kv_lens, &s);
   if (st != CA_OK) return st;
-  if ((st = bias_spec(what, dtype, const_cast<void*>(o_low), bias_table, table_dtype, bucket_starts, num_buckets, is_causal != 0, &b)) != CA_OK) return st;
+  st = bias_spec(what, dtype, const_cast<void*>(o_low), bias_table, table_dtype, bucket_starts, num_buckets,
+                 is_causal != 0, &b);
+  if (st != CA_OK) return st;
   return encdec_backward(what, dtype, q, k, v, o, dout, lse, dq, dk, dv, dtable, s, &b, is_causal != 0, workspace,
                          workspace_bytes, stream);
 }
 
 ca_status ca_relative_bias_decode(ca_dtype dtype, const void* q, const void* k, const void* v, const void* bias_table,
-                                  ca_dtype table_dtype,
-                                  const int32_t* bucket_starts, int num_buckets, const int32_t* context_lens, void* o,
+                                  ca_dtype table_dtype, const int32_t* bucket_starts, int num_buckets,
+                                  const int32_t* context_lens, void* o,
                                   int batch, int num_q_heads, int num_kv_heads, int kv_len, int head_dim,
                                   float softmax_scale, void* workspace, size_t workspace_bytes, void* stream) {
   const char* what = "relative_bias_decode";
@@ -391,7 +397,8 @@ ca_status ca_relative_bias_decode(ca_dtype dtype, const void* q, const void* k, 
   ca_status st = encdec_shape(what, dtype, batch, num_q_heads, num_kv_heads, 1, kv_len, head_dim, softmax_scale,
                               context_lens, &s);
   if (st != CA_OK) return st;
-  if ((st = bias_spec(what, dtype, nullptr, bias_table, table_dtype, bucket_starts, num_buckets, true, &b)) != CA_OK) return st;
+  st = bias_spec(what, dtype, nullptr, bias_table, table_dtype, bucket_starts, num_buckets, true, &b);
+  if (st != CA_OK) return st;
   if (batch == 0) return CA_OK;
   if ((st = check_pointers(what, {q, o}, true)) != CA_OK) return st;
   if ((st = check_pointers(what, {k, v}, kv_len > 0)) != CA_OK) return st;

@@ -198,6 +198,11 @@ def test_backward_refusals():
     for bad in ((0, 4, 300, 0), (2, 0, 300, 0), (2, 4, 0, 0), (2, 4, 300, 257), (2, 4, 300, -1), (big, big, big, 1)):
         assert lib.ca_encoder_decoder_bwd_workspace_bytes(*bad) == 0
     assert lib.ca_cross_attention_workspace_bytes(L.CA_BF16, big, big, 1, big, big, 64, 0) == 0
+    # lengths that the calls refuse, the other sizes small
+    for q_len, kv_len in ((big, 1), (1, big), (1 << 23, 1)):
+        assert lib.ca_cross_attention_workspace_bytes(L.CA_BF16, 1, 1, 1, q_len, kv_len, 64, 1) == 0
+        assert lib.ca_relative_bias_attention_workspace_bytes(L.CA_BF16, 1, 1, 1, q_len, kv_len, 64, 0) == 0
+        assert _cross(sizes=(1, 1, 1, q_len, kv_len, 64)) == L.CA_INVALID_ARGUMENT
 
 
 def test_python_refusals():

@@ -101,6 +101,31 @@ def test_table_types(dev, dtype, table_dtype):
     dq.check_out(cuda_llm.relative_bias_decode(*dq.args(), dq.lens, max_distance=30))
 
 
+STARTS = [([0], True), ([0], False), ([0, 0, 0], False), ([0, 0, 5, 5], True), ([0, 3, 3, 40], False),
+          ([0, 2048], True), ([0, 2048], False), (list(range(0, 128)), False), (list(range(0, 256)), True)]
+
+
+@pytest.mark.parametrize("dtype", DT, ids=IDS.get)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("starts,causal", STARTS, ids=[f"{len(s)}-{s[-1]}-{c}" for s, c in STARTS])
+def test_bucket_lists(dev, monkeypatch, dtype, d, starts, causal):
+    """Any list of first distances: one bucket, empty ones, as many as there may be."""
+    import ctypes
+    array = (ctypes.c_int32 * len(starts))(*starts)
+    monkeypatch.setattr(api, "_bucket_starts", lambda *a: (array, ctypes.addressof(array)))
+
+    def bucket(distance, num_buckets, is_causal, max_distance):
+        n = max(-distance, 0) if is_causal else abs(distance)
+        return max(i for i, s in enumerate(starts) if s <= n) + (len(starts) if distance > 0 and not is_causal else 0)
+
+    monkeypatch.setattr(oracle.encdec, "relative_bucket", bucket)
+    nb = len(starts) if causal else 2 * len(starts)
+    _all(Problem(dev, dtype, 2, 4, 2, 130, 130, d, [130, 77], nb, causal=causal, junk=float("nan")))
+    if causal:
+        p = Problem(dev, dtype, 2, 4, 2, 1, 300, d, [300, 9], nb, causal=True, at_end=True, junk=float("nan"))
+        p.check_out(cuda_llm.relative_bias_decode(*p.args(), p.lens))
+
+
 @pytest.mark.parametrize("dtype", DT, ids=IDS.get)
 @pytest.mark.parametrize("buckets", [0, 32])
 def test_nan_stays_in_its_head_and_row(dev, dtype, buckets):
@@ -238,6 +263,21 @@ def test_queries_past_32_bits(dev, bias):
     p.check_grads([x[:, -1:] for x in grads], out[:, -1:])
 
 
+def test_shared_head_queries_past_32_bits(dev):
+    """The rows of a kv head's 32 query heads, 2.6e9 elements one after the other."""
+    h, s, n, d = 32, 640000, 64, 128
+    g = torch.Generator(device=dev).manual_seed(1)
+    q, dout = (torch.randn(1, h, s, d, device=dev, dtype=torch.bfloat16, generator=g) for _ in range(2))
+    k, v = (torch.randn(1, 1, n, d, device=dev, dtype=torch.bfloat16, generator=g) for _ in range(2))
+    out, lse = cuda_llm.cross_attention_forward_lse(q, k, v)
+    dq = cuda_llm.cross_attention_backward(dout, q, k, v, out, lse)[0]
+    last = lambda t: t[:, -1:, -1000:].contiguous()
+    p = _Slice(last(q), k, v, last(dout))
+    p.check_out(last(out))
+    p.check_lse(last(lse))
+    p.check_grads([last(dq)], last(out))
+
+
 # ---------------------------------------------------------------------------
 # The forms of a call
 # ---------------------------------------------------------------------------
@@ -285,6 +325,9 @@ def test_same_bytes_either_way(dev, general, dtype, form):
         lens = p.lens
         for big in (lens.long(), torch.where(lens == p.k.shape[2], 1 << 40, lens.long())):
             p.lens = big
+            _equal(ref, _calls(p))
+        for t in (torch.uint8, torch.int16):
+            p.lens = lens.to(t)
             _equal(ref, _calls(p))
         p.lens = torch.stack([lens, lens], 1)[:, 0]   # a strided view
         _equal(ref, _calls(p))
