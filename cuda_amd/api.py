@@ -326,17 +326,18 @@ def _bucket_starts(num_buckets, is_causal, max_distance):
     address of it: the first half of the side's buckets hold one distance each,
     the others distances that grow as a power up to max_distance: bucket e + j starts at
     the first n with (n / e) ** span >= (max_distance / e) ** j, e buckets
-    below it and span from it on, found in whole numbers."""
+    below it and span from it on, found in whole numbers (all of them e where
+    max_distance is no more)."""
     side = num_buckets if is_causal else num_buckets // 2
     _check(1 <= num_buckets <= 256 and (is_causal or num_buckets % 2 == 0) and side >= 2,
            "bias_table must have 2 to 256 buckets (4 or more, an even number, if not causal)")
     e = side // 2
     span = side - e
-    _check(e < max_distance <= 2048, f"max_distance must be in ({e}, 2048]")
+    _check(1 <= max_distance <= 2048, "max_distance must be in [1, 2048]")
     starts = list(range(e))
     for j in range(span):
         power = max_distance ** j * e ** span
-        lo, hi = e, max_distance       # (hi reaches every border: j < span)
+        lo, hi = e, max(max_distance, e)   # (hi reaches every border: j < span)
         while lo < hi:
             mid = (lo + hi) // 2
             if mid ** span * e ** j >= power:
@@ -494,8 +495,9 @@ def relative_bias_attention_forward(q, k, v, bias_table, kv_lens=None, is_causal
     query (j <= i) have the first half of the buckets and those after it the
     second, by |j - i|. Half of such a side's buckets hold one distance each
     (from 0 on), the other half distances that grow as a power up to
-    max_distance (at most 2048); what lies beyond is in the last one. No
-    reference counterpart."""
+    max_distance (at most 2048); what lies beyond is in the last one (all from
+    the second half on, where max_distance does not reach it). No reference
+    counterpart."""
     out = _native().relative_bias_attention_forward(q, k, v, bias_table, kv_lens, is_causal, softmax_scale,
                                                     _starts_address(bias_table, is_causal, max_distance))
     if out is not None:

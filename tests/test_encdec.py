@@ -104,6 +104,21 @@ def test_bucket_starts(buckets, causal, distance):
         assert all(oracle.relative_bucket(n, buckets, True, distance) == 0 for n in range(5))
 
 
+@pytest.mark.parametrize("buckets,causal,distance", [
+    (64, True, 20), (64, True, 32), (64, True, 33), (32, False, 8), (32, False, 1), (256, True, 128), (2, True, 1)])
+def test_bucket_starts_of_short_distances(buckets, causal, distance):
+    """A max_distance that the one-distance buckets pass: from their end on all
+    distances are in the last bucket (33: the powers are within one whole number)."""
+    starts = list(api._bucket_starts(buckets, causal, distance)[0])
+    side = buckets if causal else buckets // 2
+    e = side // 2
+    assert starts == list(range(e)) + [e] + [max(e, distance)] * (side - e - 1)
+    for n in range(3 * side):
+        assert oracle.relative_bucket(-n, buckets, causal, distance) == max(i for i in range(side) if starts[i] <= n)
+        if n >= max(e, distance):
+            assert oracle.relative_bucket(-n, buckets, causal, distance) == side - 1
+
+
 def test_wrong_buckets_are_noticed():
     """A border one off moves weights by far more than the GPU tests allow."""
     rng = np.random.default_rng(0)
@@ -214,7 +229,7 @@ def test_python_refusals():
         cuda_llm.relative_bias_attention(q, k, k, torch.zeros(8, 4))
     with pytest.raises(RuntimeError, match="CUDA"):
         cuda_llm.relative_bias_decode(q[:, :, :1].contiguous(), k, k, torch.zeros(8, 4))
-    for buckets, causal, distance in ((1, True, 8), (2, False, 8), (7, False, 8), (258, True, 300), (32, False, 8),
-                                      (32, False, 2049), (32, True, 16), (32, True, -3)):
+    for buckets, causal, distance in ((1, True, 8), (2, False, 8), (7, False, 8), (258, True, 300), (32, False, 0),
+                                      (32, False, 2049), (32, True, -3)):
         with pytest.raises(RuntimeError, match="buckets|max_distance"):
             api._bucket_starts(buckets, causal, distance)

@@ -172,6 +172,8 @@ BIAS = [
     (1, 2, 1, 40, 390, None, 32, 128, False),
     (1, 2, 1, 40, 390, None, 6, 30, True),
     (2, 1, 1, 1100, 1100, [1100, 500], 32, 128, True),
+    (2, 2, 1, 150, 150, [150, 99], 64, 20, True),
+    (1, 2, 2, 150, 150, [143], 64, 9, False),
 ]
 
 
@@ -215,6 +217,7 @@ def test_bias_backward(dev, dtype, d, b, hq, hkv, sq, skv, lens, buckets, distan
     (2, 32, 8, 1000, [1000, 333], 32, 128),
     (2, 40, 2, 300, [299, 17], 64, 500),
     (1, 2, 2, 3000, None, 256, 2048),
+    (2, 4, 1, 500, [500, 36], 64, 20),
     (4, 8, 8, 700, [700, 500, 130, 16], 10, 20),
 ])
 def test_bias_decode(dev, dtype, d, b, hq, hkv, s, lens, buckets, distance):

@@ -375,7 +375,7 @@ def test_refusals(dev):
             cuda_llm.cross_attention(q, k, k, lens)
     for tab, kw, word in ((new(8, 3), {}, "num_heads"), (new(8), {}, "num_buckets"), (new(7, 4), {}, "even"),
                           (new(8, 4, dtype=torch.int32), {}, "type"), (table.cpu(), {}, "device"),
-                          (table, dict(max_distance=1), "max_distance"), (table, dict(max_distance=1 << 40), "max_distance"),
+                          (table, dict(max_distance=0), "max_distance"), (table, dict(max_distance=1 << 40), "max_distance"),
                           (new(258, 4), {}, "buckets"), (table, dict(max_distance=20.0), "integer")):
         with pytest.raises(RuntimeError, match=word):
             cuda_llm.relative_bias_attention(q, k, k, tab, **kw)
