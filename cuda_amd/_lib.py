@@ -40,6 +40,7 @@ SIGNATURES = {
     "ca_relative_bias_attention_bwd": (_I, [_I, _P, _P, _P, _P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I,
                                             _I, _I, _I, _I, _F, _I, _P, _Z, _P]),
     "ca_encoder_decoder_bwd_workspace_bytes": (_Z, [_I, _I, _I, _I]),
+    "ca_relative_bias_decode_workspace_bytes": (_Z, [_I, _I, _I, _I, _I, _I]),
     "ca_relative_bias_decode": (_I, [_I, _P, _P, _P, _P, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _F, _P, _Z, _P]),
     "ca_stream_read": (_I, [_P, _Z, _P, _P]),
     "ca_paged_kv_append": (_I, [_I, _I, _P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I,
@@ -118,7 +119,8 @@ NATIVE_FUNCTIONS = (
     "ca_paged_kv_append", "ca_fused_microscaled_attention", "ca_mx_workspace_bytes", "ca_cross_attention",
     "ca_cross_attention_workspace_bytes", "ca_cross_attention_bwd", "ca_relative_bias_attention",
     "ca_relative_bias_attention_workspace_bytes", "ca_relative_bias_attention_bwd",
-    "ca_encoder_decoder_bwd_workspace_bytes", "ca_relative_bias_decode")
+    "ca_encoder_decoder_bwd_workspace_bytes", "ca_relative_bias_decode",
+    "ca_relative_bias_decode_workspace_bytes")
 
 
 def native():

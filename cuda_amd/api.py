@@ -583,9 +583,10 @@ def relative_bias_decode(q, k, v, bias_table, context_lens=None, softmax_scale=N
         table, starts = _bias_checks(q, bias_table, True, max_distance)
         q, k, v = _aligned(q), _aligned(k), _aligned(v)
         out = torch.empty_like(q)
-        ws, nbytes = _workspace(_lib.load().ca_flash_decode_workspace_bytes(dt, b, hq, hkv, skv, d), q.device)
-        _lib.call("ca_relative_bias_decode", dt, _ptr(q), _ptr(k), _ptr(v), _ptr(table), _DT[table.dtype], starts, table.shape[0],
-                  _ptr(lens), _ptr(out), b, hq, hkv, skv, d, _scale(softmax_scale, d), _ptr(ws), nbytes, _stream())
+        nbytes = _lib.load().ca_relative_bias_decode_workspace_bytes(dt, b, hq, hkv, skv, d)
+        ws, nbytes = _workspace(nbytes, q.device)
+        _lib.call("ca_relative_bias_decode", dt, _ptr(q), _ptr(k), _ptr(v), _ptr(table), _DT[table.dtype], starts,
+                  table.shape[0], _ptr(lens), _ptr(out), b, hq, hkv, skv, d, _scale(softmax_scale, d), _ptr(ws), nbytes, _stream())
     return out
 
 

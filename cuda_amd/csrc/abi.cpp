@@ -294,6 +294,12 @@ size_t ca_encoder_decoder_bwd_workspace_bytes(int batch, int num_q_heads, int q_
                                        num_buckets);
 }
 
+size_t ca_relative_bias_decode_workspace_bytes(ca_dtype dtype, int batch, int num_q_heads, int num_kv_heads, int kv_len,
+                                               int head_dim) {
+  if (!encdec_sizes_ok(dtype, batch, num_q_heads, num_kv_heads, 1, kv_len, head_dim)) return 0;
+  return ca::encdec_decode_bytes((int)dtype, batch, num_q_heads, num_kv_heads, head_dim, kv_len);
+}
+
 static ca_status encdec_forward(const char* what, ca_dtype dtype, const void* q, const void* k, const void* v, void* o,
                                 float* lse, const ca::EncDecShape& s, const ca::BiasSpec* bias, bool causal,
                                 void* workspace, size_t workspace_bytes, void* stream) {

@@ -608,8 +608,7 @@ struct CrossRows {
 
 size_t cross_workspace_bytes(int dtype, const EncDecShape& s, bool bias, bool causal, bool lse) {
   if (few_rows(s, bias, lse))
-    return std::max(decode_workspace_bytes(s.B, s.Hq * s.Sq, s.D, s.Skv),
-                    flash_decode_partials_bytes(dtype, s.B, s.Hq * s.Sq, s.Hkv, s.D, s.Skv));
+    return encdec_decode_bytes(dtype, s.B, s.Hq * s.Sq, s.Hkv, s.D, s.Skv);
   if (dtype == kDtypeF32) return 0;
   const CrossRows r(s, bias);
   const CrossPlan p = cross_plan(r.n_bh, r.rows, s.Skv, s.D, bias, causal);

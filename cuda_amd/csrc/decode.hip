@@ -1166,11 +1166,12 @@ __global__ __launch_bounds__(64) void decode_f32_kernel(
     const int32_t* __restrict__ block_tables, const int32_t* __restrict__ context_lens,
     float* __restrict__ O, float* __restrict__ ws_o, float* __restrict__ ws_lse, int Hq,
     int Hkv, int S_contig, int max_blocks, int num_blocks, int max_splits, int n_hc,
-    float scale_log2, X x) {
+    float scale_log2, X x, int cross_split_tokens) {
   constexpr bool PAGED = SRC != kSrcF32Contig;
   constexpr bool FP8 = SRC == kSrcFp8Paged;
   constexpr int PER = D / 64;
-  constexpr int kSplitTokens = kPagesPerWave * kDecodePage;
+  // (multiples of 64)
+  const int kSplitTokens = X::kCross ? cross_split_tokens : kPagesPerWave * kDecodePage;
   __shared__ float qs[G][D];
   __shared__ float ps[G][64];
 
@@ -1197,9 +1198,8 @@ __global__ __launch_bounds__(64) void decode_f32_kernel(
     const int g = i / D, d = i % D;
     qs[g][d] = (g < Gc) ? Q[((size_t)n * Hq + hq0 + g) * D + d] * scale_log2 : 0.f;
   }
-  __shared__ uint16_t first[X::kBias ? kMaxBuckets : 1];
-  if constexpr (X::kBias)
-    for (int i = lane; i < x.side; i += 64) first[i] = x.first[i];
+  extern __shared__ __attribute__((aligned(16))) unsigned char bias_mem[];
+  if constexpr (X::kBias) decode_bias_fill(x, hq0, Gc, bias_mem, 64, 0);
   __syncthreads();
 
   float m_run[G], l_run[G], o[G][PER];
@@ -1267,9 +1267,10 @@ __global__ __launch_bounds__(64) void decode_f32_kernel(
         }
       }
       if constexpr (X::kBias) {
-        const int bucket = bias_bucket(x, first, tc - (L - 1));
+        // the bucket ids lie behind the columns (decode_bias_fill)
+        const float* col = (const float*)bias_mem + 16 * bias_mem[64 * x.side + min(L - 1 - tc, x.reach)];
 #pragma unroll
-        for (int g = 0; g < G; ++g) s[g] += x.value(bucket, hq0 + min(g, Gc - 1));
+        for (int g = 0; g < G; ++g) s[g] += col[g];
       }
     }
 #pragma unroll
@@ -1369,30 +1370,49 @@ struct F32DecodeArgs {
   size_t ws_bytes;
 };
 
+// Pages per wave of the float32 kernel with an X of its own: eight waves to a CU
+// where the sequences are long enough, as far as the workspace holds their partials
+// (4 x 32 / 8 heads x 1626 keys x 64: 1024 tokens a wave 156 us, 64 with the merge 24).
+static int cross_f32_pages(int N, int Hq, int Hkv, int D, int S, size_t ws_bytes) {
+  const int pages = S / kDecodePage + (S % kDecodePage != 0);
+  const int Gq = Hq / Hkv, most = 8 * std::max(device_cus(), 1);
+  const long long segs = std::max<long long>((long long)N * Hkv * ((Gq + 7) / 8), 1);
+  const int splits = (int)std::min<long long>(std::max<long long>(most / segs, 1), std::max(pages, 1));
+  int per = ((pages + splits - 1) / splits + 3) / 4 * 4;
+  per = std::min(std::max(per, 4), kPagesPerWave);
+  while (per < kPagesPerWave && split_partials_bytes(N, Hq, D, (pages + per - 1) / per) > ws_bytes)
+    per = std::min(2 * per, kPagesPerWave);
+  return per;
+}
+
 template <int D, int SRC, int G, class X>
 static hipError_t launch_decode_f32_t(const F32DecodeArgs& a, const X& x, hipStream_t stream) {
   constexpr bool PAGED = SRC != kSrcF32Contig;
   const int max_tokens = PAGED ? a.max_blocks * kDecodePage : a.S_contig;
   const int pages = (max_tokens + kDecodePage - 1) / kDecodePage;
-  const int max_splits = max(1, (pages + kPagesPerWave - 1) / kPagesPerWave);
+  int per = kPagesPerWave;
+  size_t lds = 0;
+  if constexpr (X::kCross) per = cross_f32_pages(a.N, a.Hq, a.Hkv, D, max_tokens, a.ws_bytes);
+  if constexpr (X::kBias) lds = decode_bias_lds_bytes(x.side, x.reach);
+  const int max_splits = max(1, (pages + per - 1) / per);
   const int Gq = a.Hq / a.Hkv;
   const int n_hc = (Gq + G - 1) / G;
-  const size_t need = decode_workspace_bytes(a.N, a.Hq, D, max_tokens);
+  const size_t need = split_partials_bytes(a.N, a.Hq, D, max_splits);
   if (a.ws_bytes < need) return hipErrorInvalidValue;
   float* ws_o = (float*)a.ws;
   float* ws_lse = need ? ws_o + (size_t)a.N * a.Hq * max_splits * D : nullptr;
   const long long grid = (long long)a.N * a.Hkv * n_hc * max_splits;
   if (grid == 0) return hipSuccess;
   if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((decode_f32_kernel<D, SRC, G, X>), dim3((unsigned)grid), dim3(64), 0, stream,
+  hipLaunchKernelGGL((decode_f32_kernel<D, SRC, G, X>), dim3((unsigned)grid), dim3(64), lds, stream,
                      (const float*)a.q, a.kc, a.vc, a.k_scale, a.v_scale, a.per_block, a.bt, a.lens,
                      (float*)a.out, ws_o, ws_lse, a.Hq, a.Hkv, a.S_contig, a.max_blocks,
-                     a.num_blocks, max_splits, n_hc, a.scale * kLog2e, x);
+                     a.num_blocks, max_splits, n_hc, a.scale * kLog2e, x, per * kDecodePage);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || max_splits <= 1) return e;
   hipLaunchKernelGGL((decode_merge_kernel<F32, D>), dim3((unsigned)(a.N * a.Hq)), dim3(64), 0,
                      stream, a.lens, max_tokens, ws_o, ws_lse, a.out, a.Hq,
-                     max_splits, kPagesPerWave);
+                     max_splits, per);
   return hipGetLastError();
 }
 
@@ -1540,6 +1560,14 @@ hipError_t launch_flash_decode(int dtype, const void* q, const void* k, const vo
     return launch_decode_f32<kSrcF32Contig>(D, a, stream);
   }
   return hipErrorInvalidValue;
+}
+
+size_t encdec_decode_bytes(int dtype, int N, int Hq, int Hkv, int D, int S) {
+  if (dtype != kDtypeF32)
+    return std::max(decode_workspace_bytes(N, Hq, D, S), flash_decode_partials_bytes(dtype, N, Hq, Hkv, D, S));
+  const int pages = S / kDecodePage + (S % kDecodePage != 0);
+  const int per = cross_f32_pages(N, Hq, Hkv, D, S, SIZE_MAX);
+  return std::max(decode_workspace_bytes(N, Hq, D, S), split_partials_bytes(N, Hq, D, (pages + per - 1) / per));
 }
 
 hipError_t launch_encdec_decode(int dtype, const void* q, const void* k, const void* v, void* o,

@@ -110,15 +110,6 @@ __host__ __device__ __forceinline__ int bias_entries(const BiasX& x) {
 }
 __host__ __device__ __forceinline__ size_t bias_lds_bytes(const BiasX& x) { return 4 * (size_t)bias_entries(x); }
 
-// bucket of distance rel, `first` in LDS
-__device__ __forceinline__ int bias_bucket(const BiasX& x, const uint16_t* first, int rel) {
-  const int n = rel <= 0 ? -rel : x.one_sided ? 0 : rel;
-  int b = 0;
-  for (int s = 1 << (31 - __builtin_clz(x.side)); s > 0; s >>= 1)
-    if (b + s < x.side && (int)first[b + s] <= n) b += s;
-  return b + (rel > 0 && !x.one_sided ? x.side : 0);
-}
-
 __device__ __forceinline__ float bias_clamp(float v) {
   // (not by min and max: a NaN and -inf stay)
   v = v > kMaxBias && v != -kNegInf ? kMaxBias : v;

@@ -97,7 +97,9 @@ hipError_t launch_cross(int dtype, const void* q, const void* k, const void* v, 
 hipError_t launch_cross_f32(const void* q, const void* k, const void* v, void* o, float* lse, const EncDecShape& s,
                             const BiasSpec* bias, bool causal, hipStream_t stream);
 // Few query rows (decode.hip; without a bias Sq may pass 1; with one, Sq is 1 and
-// the query is at its last key): ws holds flash_decode_partials_bytes of Hq Sq heads.
+// the query is at its last key): ws holds decode_workspace_bytes of Hq Sq heads at
+// least, encdec_decode_bytes at best.
+size_t encdec_decode_bytes(int dtype, int N, int Hq, int Hkv, int D, int S);
 hipError_t launch_encdec_decode(int dtype, const void* q, const void* k, const void* v, void* o,
                                 const EncDecShape& s, const BiasSpec* bias, void* ws, size_t ws_bytes,
                                 hipStream_t stream);

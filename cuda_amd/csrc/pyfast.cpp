@@ -51,6 +51,7 @@ struct Abi {
   decltype(&ca_relative_bias_attention_bwd) relative_bias_attention_bwd;
   decltype(&ca_encoder_decoder_bwd_workspace_bytes) encoder_decoder_bwd_workspace_bytes;
   decltype(&ca_relative_bias_decode) relative_bias_decode;
+  decltype(&ca_relative_bias_decode_workspace_bytes) relative_bias_decode_workspace_bytes;
 } abi;
 
 bool type_code(at::ScalarType t, ca_dtype* out) {
@@ -501,7 +502,7 @@ PyObject* relative_bias_decode(PyObject* const* a) {
   if (!x.take(a[0], a[1], a[2], a[4], a[5]) || x.q->size(2) != 1 || !bias_of(a[3], a[6], *x.q, t, &tdt, &starts))
     return nullptr;
   const at::Tensor &q = *x.q, &k = *x.k, o = like(q);
-  const Workspace ws(abi.flash_decode_workspace_bytes(x.dt, n(q, 0), n(q, 1), n(k, 1), n(k, 2), n(q, 3)), q);
+  const Workspace ws(abi.relative_bias_decode_workspace_bytes(x.dt, n(q, 0), n(q, 1), n(k, 1), n(k, 2), n(q, 3)), q);
   if (!ok([&] {
         return abi.relative_bias_decode(x.dt, in(q), in(k), in(*x.v), in(*t), tdt, starts, n(*t, 0), x.kv_lens(), out(o),
                                         n(q, 0), n(q, 1), n(k, 1), n(k, 2), n(q, 3), x.scale, ws.ptr(), ws.bytes,

@@ -194,7 +194,9 @@ size_t ca_encoder_decoder_bwd_workspace_bytes(int batch, int num_q_heads, int q_
 /* Its single-token form: q [batch, num_q_heads, 1, head_dim] at the position of
  * the last of its sequence's first context_lens[b] keys (NULL: kv_len each) of a
  * contiguous cache; buckets as with is_causal. workspace:
- * ca_flash_decode_workspace_bytes(...). */
+ * ca_relative_bias_decode_workspace_bytes(...). */
+size_t ca_relative_bias_decode_workspace_bytes(ca_dtype dtype, int batch, int num_q_heads, int num_kv_heads,
+                                               int kv_len, int head_dim);
 ca_status ca_relative_bias_decode(ca_dtype dtype, const void* q, const void* k, const void* v,
                                   const void* bias_table, ca_dtype table_dtype, const int32_t* bucket_starts,
                                   int num_buckets, const int32_t* context_lens, void* o, int batch,

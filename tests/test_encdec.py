@@ -213,6 +213,13 @@ def test_backward_refusals():
     for bad in ((0, 4, 300, 0), (2, 0, 300, 0), (2, 4, 0, 0), (2, 4, 300, 257), (2, 4, 300, -1), (big, big, big, 1)):
         assert lib.ca_encoder_decoder_bwd_workspace_bytes(*bad) == 0
     assert lib.ca_cross_attention_workspace_bytes(L.CA_BF16, big, big, 1, big, big, 64, 0) == 0
+    # the step's: what its call asks at least, or more
+    for dt in (L.CA_F32, L.CA_F16, L.CA_BF16):
+        for n, hq, hkv, s, d in ((1, 32, 8, 3000, 128), (64, 32, 8, 8192, 64), (3, 5, 1, 1, 64), (1, 1, 1, 1 << 22, 64)):
+            least = lib.ca_decode_workspace_bytes(n, hq, d, s)
+            assert lib.ca_relative_bias_decode_workspace_bytes(dt, n, hq, hkv, s, d) >= least
+    for bad in ((0, 4, 2, 9, 64), (1, 4, 3, 9, 64), (1, 4, 2, 9, 96), (1, 4, 2, -9, 64), (big, big, 1, 9, 64)):
+        assert lib.ca_relative_bias_decode_workspace_bytes(L.CA_F32, *bad) == 0
     # lengths that the calls refuse, the other sizes small
     for q_len, kv_len in ((big, 1), (1, big), (1 << 23, 1)):
         assert lib.ca_cross_attention_workspace_bytes(L.CA_BF16, 1, 1, 1, q_len, kv_len, 64, 1) == 0

@@ -186,6 +186,28 @@ def test_split_walks(dev, dtype, d, buckets):
 
 
 @pytest.mark.parametrize("dtype", DT, ids=IDS.get)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("b,hq,hkv,s", [(1, 1, 1, 64), (1, 1, 1, 65), (3, 24, 2, 700), (2, 4, 4, 5000), (1, 16, 1, 20000)])
+def test_steps_in_any_workspace(dev, dtype, d, b, hq, hkv, s):
+    """The step's walk in as many parts as the workspace holds: from the least to
+    more than its query asks, through the C ABI."""
+    lens = [s, s // 3, 0][:b]
+    p = Problem(dev, dtype, b, hq, hkv, 1, s, d, lens, 32, 128, True, at_end=True, junk=float("nan"))
+    starts = api._bucket_starts(32, True, 128)[0]
+    dt = api._DT[dtype]
+    least = L.load().ca_decode_workspace_bytes(b, hq, d, s)
+    best = L.load().ca_relative_bias_decode_workspace_bytes(dt, b, hq, hkv, s, d)
+    for nbytes in sorted({least, (least + best) // 32 * 16, best, best + 4096}):
+        ws = torch.full((max(nbytes, 16),), 255, dtype=torch.uint8, device=dev)
+        out = torch.full_like(p.q, float("nan"))
+        L.call("ca_relative_bias_decode", dt, *(api._ptr(t) for t in (p.q, p.k, p.v, p.table)), api._DT[p.table.dtype],
+               starts, 32, api._ptr(p.lens), api._ptr(out), b, hq, hkv, s, d, p.s, api._ptr(ws), nbytes, api._stream())
+        p.check_out(out, f"{nbytes} bytes")
+    c = Problem(dev, dtype, b, hq, hkv, 1, s, d, lens, junk=float("nan"))
+    c.check_out(cuda_llm.cross_attention(*c.args(), **c.kw()))
+
+
+@pytest.mark.parametrize("dtype", DT, ids=IDS.get)
 def test_empty_sizes(dev, dtype):
     new = lambda *s: torch.randn(*s, device=dev).to(dtype)
     table = new(8, 4)
