@@ -588,8 +588,19 @@ hipError_t launch_t(CrossArgs a, const X& x, const CrossPlan& p, size_t lds, hip
 // head to be its heads, and no LSE, which that walk does not keep. (64 x 16 heads x
 // 1 x 1500 keys x 64: 41 us, 5.8 TB/s, where tiles of 64 rows, nearly all of them
 // empty, pay a whole tile's products for each head.)
-static bool few_rows(const EncDecShape& s, bool bias, bool lse) {
-  return !bias && !lse && (long long)(s.Hq / s.Hkv) * s.Sq <= 16 && (long long)s.B * s.Hq * s.Sq <= 0x7fffffff;
+// float32 goes there with more rows too, where its tiles would leave most of the
+// chip idle, each walking all keys. Times in us of both, fitted to 84 shapes (8
+// heads x 64 rows x 4000 keys x 64: 77 in tiles, 44 here; 32 heads x 40 rows x 4000 x
+// 128: 156 and 117, x 64: 82 and 92).
+static bool few_rows(int dtype, const EncDecShape& s, bool bias, bool lse) {
+  const long long rows = (long long)(s.Hq / s.Hkv) * s.Sq;
+  if (bias || lse || (long long)s.B * s.Hq * s.Sq > 0x7fffffff) return false;
+  if (rows <= 16 || rows > 256 || dtype != kDtypeF32) return rows <= 16;
+  const double cus = std::max(device_cus(), 1);
+  const double rounds = std::ceil((double)s.B * s.Hq * ((s.Sq + 31) / 32) / cus);
+  const double tiles = 4 + 0.3e-3 * s.Skv * s.D * rounds;
+  const double here = 18 + 20e-6 * s.B * s.Hkv * rows * s.Skv;
+  return here < 0.9 * tiles;
 }
 
 // A launch's rows: without positions a kv head's query heads are one run of rows.
@@ -607,7 +618,7 @@ struct CrossRows {
 };
 
 size_t cross_workspace_bytes(int dtype, const EncDecShape& s, bool bias, bool causal, bool lse) {
-  if (few_rows(s, bias, lse))
+  if (few_rows(dtype, s, bias, lse))
     return encdec_decode_bytes(dtype, s.B, s.Hq * s.Sq, s.Hkv, s.D, s.Skv);
   if (dtype == kDtypeF32) return 0;
   const CrossRows r(s, bias);
@@ -619,7 +630,7 @@ hipError_t launch_cross(int dtype, const void* q, const void* k, const void* v, 
                         const EncDecShape& s, const BiasSpec* bias, bool causal, void* ws, size_t ws_bytes,
                         hipStream_t stream) {
   if ((long long)s.B * s.Hq * s.Sq == 0) return hipSuccess;
-  if (few_rows(s, bias, lse)) return launch_encdec_decode(dtype, q, k, v, o, s, nullptr, ws, ws_bytes, stream);
+  if (few_rows(dtype, s, bias, lse)) return launch_encdec_decode(dtype, q, k, v, o, s, nullptr, ws, ws_bytes, stream);
   if (dtype == kDtypeF32) return launch_cross_f32(q, k, v, o, lse, s, bias, causal, stream);
   CrossArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (uint16_t*)o,
               bias ? (uint16_t*)bias->o_low : nullptr, lse};

@@ -207,6 +207,14 @@ def test_steps_in_any_workspace(dev, dtype, d, b, hq, hkv, s):
     c.check_out(cuda_llm.cross_attention(*c.args(), **c.kw()))
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("b,hq,hkv,sq,skv,lens", [
+    (1, 8, 8, 64, 4000, None), (2, 8, 2, 17, 3001, [3001, 5]), (1, 32, 8, 20, 2500, [0]), (1, 3, 1, 85, 5000, [4999])])
+def test_few_float32_rows(dev, d, b, hq, hkv, sq, skv, lens):
+    """Up to 256 rows of a kv head that the step's walk takes, and as tiles (with an LSE)."""
+    _all(Problem(dev, torch.float32, b, hq, hkv, sq, skv, d, lens, junk=float("nan")))
+
+
 @pytest.mark.parametrize("dtype", DT, ids=IDS.get)
 def test_empty_sizes(dev, dtype):
     new = lambda *s: torch.randn(*s, device=dev).to(dtype)
